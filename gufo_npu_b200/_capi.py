@@ -99,6 +99,40 @@ class ExpertBank(C.Structure):
                 ("experts", C.c_int), ("expert_ffn", C.c_int), ("hidden", C.c_int)]
 
 
+class RopeParams(C.Structure):
+    _fields_ = [("rope_dim", C.c_int), ("layout", C.c_int), ("scaling", C.c_int)] + \
+               [(n, C.c_double) for n in ("theta", "factor", "original_positions", "fast_turns", "slow_turns",
+                                          "magnitude")]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("in_token_stride", C.c_int64), ("in_head_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("heads", C.c_int), ("head_dim", C.c_int), ("norm_weight", C.c_void_p), ("rms_eps", C.c_float)]
+
+
+class Cache8Config(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("sequences", "kv_heads", "head_dim", "capacity", "format", "weights")]
+
+
+class Cache8Batch(C.Structure):
+    _fields_ = [("sequences", C.c_int), ("slots", C.c_void_p), ("tokens", C.c_void_p), ("positions", C.c_void_p)]
+
+
+class Cache8AttendArgs(C.Structure):
+    _fields_ = [("heads", C.c_int), ("scale", C.c_float), ("queries", C.c_void_p), ("query_token_stride", C.c_int64),
+                ("query_head_stride", C.c_int64), ("gate", C.c_void_p), ("gate_token_stride", C.c_int64),
+                ("gate_head_stride", C.c_int64), ("out", C.c_void_p), ("out_token_stride", C.c_int64),
+                ("out_head_stride", C.c_int64), ("visible", C.c_void_p), ("accumulate", C.c_int),
+                ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)]
+
+
+ROPE_LAYOUTS = {"halves": 0, "pairs": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "by_parts": 2}
+CACHE8_FORMATS = {"e4m3": 0, "int8": 1}
+CACHE8_BLOCK = 16
+
+
 class DecoderWeights(C.Structure):
     _fields_ = [("token_embd", C.c_int64), ("output", C.c_int64), ("output_norm", _f32p),
                 ("layers", C.POINTER(LayerWeights))]
@@ -162,6 +196,22 @@ SIGNATURES = {
                                                 C.c_void_p, C.c_void_p]),
     "gufo_cuda_swiglu_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "gufo_cuda_attention_device": (C.c_int, [C.c_void_p, C.POINTER(AttentionArgs)]),
+    "gufo_cuda_rope_frequencies": (C.c_int, [C.POINTER(RopeParams), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
+    "gufo_cuda_rope_create": (C.c_int, [C.c_void_p, C.POINTER(RopeParams), C.POINTER(C.c_int64)]),
+    "gufo_cuda_rope_free": (C.c_int, [C.c_void_p, C.c_int64]),
+    "gufo_cuda_rope_device": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(RopeRows), C.c_int, C.c_void_p, C.c_int]),
+    "gufo_cuda_cache8_create": (C.c_int, [C.c_void_p, C.POINTER(Cache8Config), C.POINTER(C.c_int64)]),
+    "gufo_cuda_cache8_free": (C.c_int, [C.c_void_p, C.c_int64]),
+    "gufo_cuda_cache8_weights": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(C.c_void_p)]),
+    "gufo_cuda_cache8_append_device": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(Cache8Batch), C.c_void_p, C.c_int64,
+                                                 C.c_int64, C.c_void_p, C.c_int64, C.c_int64]),
+    "gufo_cuda_cache8_rows_device": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(Cache8Batch), C.c_void_p, C.c_void_p]),
+    "gufo_cuda_cache8_attend_scratch": (C.c_int, [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                                  C.POINTER(C.c_size_t)]),
+    "gufo_cuda_cache8_attend_device": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(Cache8Batch),
+                                                 C.POINTER(Cache8AttendArgs)]),
+    "gufo_cuda_cache8_evict_device": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(Cache8Batch), C.c_int, C.c_int, C.c_int,
+                                                C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
     "gufo_cuda_route_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                          C.c_void_p, C.c_void_p]),
     "gufo_cuda_expert_ffn_device": (C.c_int, [C.c_void_p, C.POINTER(ExpertBank), C.c_void_p, C.c_int, C.c_void_p,

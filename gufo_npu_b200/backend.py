@@ -76,6 +76,28 @@ def _ptr(buf) -> int:
     return buf.data_ptr()
 
 
+def check_rows(what: str, *tensors) -> None:
+    """fp32 device tensors [tokens, heads, head_dim] whose heads' values stand side by side."""
+    for t in tensors:
+        if str(t.dtype) != "torch.float32" or t.dim() != 3 or not t.is_cuda or (t.shape[2] > 1 and t.stride(2) != 1) \
+                or t.device != tensors[0].device:
+            raise ValueError(f"{what}: rows are fp32 tensors [tokens, heads, head_dim] on one device, a head's values "
+                             "side by side")
+
+
+def check_ints(what: str, t) -> None:
+    if str(t.dtype) != "torch.int32" or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what}: an int32 tensor on the device, its values side by side")
+
+
+def rope_params(rope_dim: int, theta: float, layout: str, scaling: str, factor: float, original_positions: float,
+                fast_turns: float, slow_turns: float, magnitude: float) -> "_capi.RopeParams":
+    if layout not in _capi.ROPE_LAYOUTS or scaling not in _capi.ROPE_SCALINGS:
+        raise ValueError(f"rope: layouts are {sorted(_capi.ROPE_LAYOUTS)}, scalings {sorted(_capi.ROPE_SCALINGS)}")
+    return _capi.RopeParams(rope_dim, _capi.ROPE_LAYOUTS[layout], _capi.ROPE_SCALINGS[scaling], theta, factor,
+                            original_positions, fast_turns, slow_turns, magnitude)
+
+
 class Context:
     """One gufo_cuda_ctx: a device, a stream, its weights and scratch."""
 
@@ -225,6 +247,44 @@ class Context:
                                 _capi.EPILOGUE_SWIGLU if activate else _capi.EPILOGUE_NONE)
         self._check(self.lib.gufo_cuda_matmul_fused_device(self.handle, parts_arr, nparts, C.byref(args), tokens,
                                                            C.c_void_p(_ptr(y))))
+
+    # -- rotary positions -----------------------------------------------------
+    def rope_create(self, rope_dim: int, theta: float = 1e7, layout: str = "halves", scaling: str = "none",
+                    factor: float = 1.0, original_positions: float = 0, fast_turns: float = 32.0,
+                    slow_turns: float = 1.0, magnitude: float = 0.0) -> int:
+        """A table of rotary frequencies (gufo_cuda_rope_params says what the scalings are)."""
+        params = rope_params(rope_dim, theta, layout, scaling, factor, original_positions, fast_turns, slow_turns,
+                             magnitude)
+        out = C.c_int64()
+        self._check(self.lib.gufo_cuda_rope_create(self.handle, C.byref(params), C.byref(out)))
+        return int(out.value)
+
+    def rope_free(self, rope: int) -> None:
+        self._check(self.lib.gufo_cuda_rope_free(self.handle, rope))
+
+    def rope_parts(self, parts: Sequence, rms_eps: float = 0.0) -> "C.Array":
+        """[(x, out, norm weight or None)]: fp32 device tensors [tokens, heads, head_dim] (any token and head
+        strides) as the array that rope_device takes; the caller keeps the tensors."""
+        arr = (_capi.RopeRows * len(parts))()
+        for i, (x, out, norm) in enumerate(parts):
+            check_rows("rope", x, out)
+            if norm is not None and (norm.dtype != x.dtype or tuple(norm.shape) != (x.shape[2],) or not norm.is_contiguous()
+                                     or norm.device != x.device):
+                raise ValueError("rope: a norm weight is an fp32 value for each of a head's, beside the rows")
+            if x.shape != out.shape:
+                raise ValueError("rope: rows keep their shape")
+            arr[i] = _capi.RopeRows(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                    x.shape[1], x.shape[2], _ptr(norm) or None, rms_eps)
+        arr.tokens = min((p[0].shape[0] for p in parts), default=0)
+        return arr
+
+    def rope_device(self, rope: int, parts, positions) -> None:
+        """Turns the rows of `parts` (rope_parts), token t by positions[t] (an int32 device tensor)."""
+        check_ints("rope", positions)
+        if positions.numel() > parts.tokens:
+            raise ValueError("rope: more positions than rows")
+        self._check(self.lib.gufo_cuda_rope_device(self.handle, rope, parts, len(parts),
+                                                   C.c_void_p(positions.data_ptr()), positions.numel()))
 
     # -- routed experts -------------------------------------------------------
     def route_device(self, router, stride: int, tokens: int, experts: int, k: int, chosen, weights,

@@ -1,0 +1,188 @@
+"""The key / value cache in 8 bits: `CudaCache8` over the C ABI's gufo_cuda_cache8 entries.
+
+One cache holds the keys and values of one attention layer for a number of sequences. A call
+takes a batch of them (`batch`: made once, used for every layer and step); the number of rows a
+sequence holds is a device tensor of the caller's, one for all layers, as it is for the fp16
+cache of gufo_cuda_attention_device. Everything here only enqueues on the context's stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+from . import _capi
+from .backend import Context, _DeviceArray, check_ints, check_rows
+
+
+class Batch:
+    """Sequences of a call: slots and tokens as the library takes them, and the positions they start at."""
+
+    def __init__(self, positions, tokens: Optional[Sequence[int]], slots: Optional[Sequence[int]]):
+        check_ints("cache8", positions)
+        n = positions.numel()
+        for name, values in (("tokens", tokens), ("slots", slots)):
+            if values is not None and len(values) != n:
+                raise ValueError(f"cache8: {n} positions and {len(values)} {name}")
+        self.sequences = n
+        self.positions = positions
+        self.rows = n if tokens is None else sum(tokens)
+        self._tokens = None if tokens is None else (C.c_int * n)(*tokens)
+        self._slots = None if slots is None else (C.c_int * n)(*slots)
+        self.args = _capi.Cache8Batch(n, C.cast(self._slots, C.c_void_p) if slots is not None else None,
+                                      C.cast(self._tokens, C.c_void_p) if tokens is not None else None,
+                                      positions.data_ptr())
+
+
+class Scratch:
+    """Scratch of attention calls that run one after another: one for each stream or captured graph that
+    may be in flight beside others."""
+
+    def __init__(self, ctx: Context, nbytes: int):
+        self.ctx, self.bytes = ctx, nbytes
+        self.ptr = ctx.malloc(nbytes)
+        ctx.memset_zero(self.ptr, nbytes)
+
+    def close(self) -> None:
+        if self.ptr and self.ctx.handle:
+            self.ctx.free(self.ptr)
+        self.ptr = 0
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _Owner:
+    """The library's cache: freed when neither its CudaCache8 nor a tensor over its memory is left."""
+
+    def __init__(self, ctx: Context, config: "_capi.Cache8Config"):
+        self.ctx, self.handle = ctx, 0
+        out = C.c_int64()
+        ctx._check(ctx.lib.gufo_cuda_cache8_create(ctx.handle, C.byref(config), C.byref(out)))
+        self.handle = int(out.value)
+
+    def close(self) -> None:
+        if self.handle and self.ctx.handle:
+            self.ctx.lib.gufo_cuda_cache8_free(self.ctx.handle, self.handle)
+        self.handle = 0
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class CudaCache8:
+    """Keys and values of one attention layer, a byte a value (gufo_cuda_cache8)."""
+
+    def __init__(self, ctx: Context, sequences: int, kv_heads: int, head_dim: int, capacity: int, format: str = "e4m3",
+                 weights: bool = False):
+        if format not in _capi.CACHE8_FORMATS:
+            raise ValueError(f"cache8: formats are {sorted(_capi.CACHE8_FORMATS)}")
+        self.ctx = ctx
+        self.sequences, self.kv_heads, self.head_dim, self.capacity = sequences, kv_heads, head_dim, capacity
+        self.format = format
+        config = _capi.Cache8Config(sequences, kv_heads, head_dim, capacity, _capi.CACHE8_FORMATS[format], int(weights))
+        self._owner = _Owner(ctx, config)
+        self.handle = self._owner.handle
+        self._weights = None
+        if weights:
+            import torch
+            ptr = C.c_void_p()
+            ctx._check(ctx.lib.gufo_cuda_cache8_weights(ctx.handle, self.handle, C.byref(ptr)))
+            memory = _DeviceArray(int(ptr.value), sequences * kv_heads * capacity)
+            memory.owner = self._owner      # (the tensor keeps `memory`)
+            flat = torch.as_tensor(memory, device=torch.device("cuda", ctx.device))
+            self._weights = flat.view(sequences, kv_heads, capacity)
+
+    def close(self) -> None:
+        """Frees the cache at once; tensors over its weights must not be used after."""
+        self._owner.close()
+        self.handle = 0
+        self._weights = None
+
+    @property
+    def weights(self):
+        """The accumulated weights [sequences, kv_heads, capacity], the cache's own memory; None without."""
+        return self._weights
+
+    def batch(self, positions, tokens: Optional[Sequence[int]] = None, slots: Optional[Sequence[int]] = None) -> Batch:
+        """Sequences of a call: `positions` (int32, device) rows held ahead of it, `tokens` rows each (one
+        without), in `slots` (0, 1, ... without)."""
+        return Batch(positions, tokens, slots)
+
+    def scratch(self, heads: int, tokens: int, accumulate: bool = False) -> Scratch:
+        """Scratch of attend_device calls with up to `tokens` query tokens in all."""
+        nbytes = C.c_size_t()
+        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_attend_scratch(self.ctx.handle, self.handle, heads, tokens,
+                                                                     int(accumulate), C.byref(nbytes)))
+        return Scratch(self.ctx, nbytes.value)
+
+    def _check_kv(self, batch: Batch, *tensors) -> None:
+        check_rows("cache8", *tensors)
+        for t in tensors:
+            if tuple(t.shape) != (batch.rows, self.kv_heads, self.head_dim):
+                raise ValueError(f"cache8: rows [{batch.rows}, {self.kv_heads}, {self.head_dim}], not {list(t.shape)}")
+
+    def append_device(self, batch: Batch, keys, values) -> None:
+        """Writes the batch's rows, [rows, kv_heads, head_dim] each, at their positions."""
+        self._check_kv(batch, keys, values)
+        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_append_device(
+            self.ctx.handle, self.handle, C.byref(batch.args), C.c_void_p(keys.data_ptr()), keys.stride(0), keys.stride(1),
+            C.c_void_p(values.data_ptr()), values.stride(0), values.stride(1)))
+
+    def rows_device(self, batch: Batch, keys, values) -> None:
+        """What the rows of an append with this batch stand for, into contiguous [rows, kv_heads, head_dim]."""
+        self._check_kv(batch, keys, values)
+        if not (keys.is_contiguous() and values.is_contiguous()):
+            raise ValueError("cache8: rows are read into contiguous tensors")
+        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_rows_device(
+            self.ctx.handle, self.handle, C.byref(batch.args), C.c_void_p(keys.data_ptr()), C.c_void_p(values.data_ptr())))
+
+    def attend_device(self, batch: Batch, queries, out, scratch: Scratch, gate=None, scale: float = 0.0, visible=None,
+                      accumulate: bool = False) -> None:
+        """out = softmax(queries K^T scale) V [* sigmoid(gate)] for [rows, heads, head_dim] query rows. Token t of
+        a sequence sees the rows up to position + t, or the first visible[...] (int32, a value per row of
+        queries). `accumulate` adds what each cached row was given to `weights`."""
+        check_rows("cache8", queries, out, *([gate] if gate is not None else []))
+        heads = queries.shape[1]
+        for t in (queries, out, gate):
+            if t is not None and tuple(t.shape) != (batch.rows, heads, self.head_dim):
+                raise ValueError(f"cache8: query rows [{batch.rows}, {heads}, {self.head_dim}], not {list(t.shape)}")
+        if visible is not None:
+            check_ints("cache8", visible)
+            if visible.numel() != batch.rows:
+                raise ValueError(f"cache8: {batch.rows} query rows and {visible.numel()} numbers of rows they see")
+        args = _capi.Cache8AttendArgs(
+            heads, scale, queries.data_ptr(), queries.stride(0), queries.stride(1),
+            *((gate.data_ptr(), gate.stride(0), gate.stride(1)) if gate is not None else (None, 0, 0)),
+            out.data_ptr(), out.stride(0), out.stride(1), visible.data_ptr() if visible is not None else None,
+            int(accumulate), scratch.ptr, scratch.bytes)
+        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_attend_device(self.ctx.handle, self.handle, C.byref(batch.args),
+                                                                    C.byref(args)))
+
+    def evict_device(self, batch: Batch, budget: int, kept, first: int = 0, last: int = 0, held=None,
+                     into: Optional["CudaCache8"] = None, into_slots: Optional[Sequence[int]] = None) -> None:
+        """Brings the batch's sequences (their `positions` rows) down to `budget` rows: the first `first`, the
+        last `last`, and the rest by weight; in place, or into another cache's slots. `kept` (int32
+        [sequences, kv_heads, budget]) gets the rows that stayed, `held` (int32 [sequences]) how many."""
+        check_ints("cache8", kept)
+        if tuple(kept.shape) != (batch.sequences, self.kv_heads, budget):
+            raise ValueError(f"cache8: kept is [{batch.sequences}, {self.kv_heads}, {budget}], not {list(kept.shape)}")
+        if held is not None:
+            check_ints("cache8", held)
+            if held.numel() != batch.sequences:
+                raise ValueError("cache8: held has a value per sequence")
+        slots = None
+        if into_slots is not None:
+            if len(into_slots) != batch.sequences:
+                raise ValueError(f"cache8: {batch.sequences} sequences and {len(into_slots)} slots")
+            slots = (C.c_int * batch.sequences)(*into_slots)
+        if into is not None and into.ctx is not self.ctx:
+            raise ValueError("cache8: both caches belong to one context")
+        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_evict_device(
+            self.ctx.handle, self.handle, C.byref(batch.args), budget, first, last, C.c_void_p(kept.data_ptr()),
+            C.c_void_p(held.data_ptr()) if held is not None else None, into.handle if into is not None else 0, slots))

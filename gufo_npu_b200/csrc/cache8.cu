@@ -1,0 +1,378 @@
+// The key / value cache in 8 bits: its memory, the append, and its rows as fp32.
+//
+// The append. What a block of 16 rows of a head becomes depends on all its new rows, through
+// their largest magnitude, and on the scale of the rows that it holds already: four warps take
+// a block's keys and four its values, four rows each, and meet once in shared memory. The
+// rows that were there are read and rounded again only where the scale grew. Bound by the 4
+// bytes a value that come in; decode steps (a row or a few a sequence) by latency alone.
+#include "cache8.cuh"
+
+#include <new>
+
+namespace gufo {
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr float kLargest = 0x1p127f;   // magnitudes from here on saturate: what a code stands for is finite then
+
+struct AppendArgs {
+  CacheView cache;
+  const float* rows[2];
+  int64_t token_stride[2], head_stride[2];
+  int whole;      // rows may be read four values at a time
+};
+
+// Grid: (blocks that the batch may touch, KV heads).
+template <typename Format>
+__global__ void __launch_bounds__(kAppendThreads)
+AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ BatchArgs batch) {
+  __shared__ float tops[2][4];
+  GridLaunchDependents();
+  GridDependencyWait();
+  const BatchEntry& e = batch.of[SequenceOf(batch, blockIdx.x)];
+  const CacheView& c = a.cache;
+  const int held = batch.positions[e.index];
+  const int start = min(max(held, 0), c.capacity);
+  const int end = static_cast<int>(min(static_cast<int64_t>(held) + e.tokens, static_cast<int64_t>(c.capacity)));
+  const int nth = blockIdx.x - batch.first_item[&e - batch.of];
+  const int block = start / kCacheBlock + nth;
+  const int row0 = block * kCacheBlock;
+  if (row0 >= end) {
+    return;
+  }
+  const int head = blockIdx.y;
+  const int side = threadIdx.x / 128, warp = threadIdx.x / 32 & 3, lane = threadIdx.x & 31;
+  const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + head;
+  const int fours = c.head_dim / 4;
+  constexpr int kTimes = kCacheMaxDim / 128;
+
+  // This warp's new rows: r = row0 + 4 warp + i where start <= r < end.
+  float4 x[4][kTimes];
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row0 + 4 * warp + i;
+    const float* from = a.rows[side] + (static_cast<int64_t>(e.row) + (r - held)) * a.token_stride[side] + head * a.head_stride[side];
+#pragma unroll
+    for (int n = 0; n < kTimes; ++n) {
+      const int f = lane + 32 * n;
+      x[i][n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= start && r < end && f < fours) {
+        if (a.whole) {
+          x[i][n] = __ldcs(reinterpret_cast<const float4*>(from) + f);
+        } else {
+          x[i][n] = make_float4(__ldcs(from + 4 * f), __ldcs(from + 4 * f + 1), __ldcs(from + 4 * f + 2), __ldcs(from + 4 * f + 3));
+        }
+        const auto hold = [&](float& v) {
+          v = v != v ? v : fminf(fmaxf(v, -kLargest), kLargest);
+          top = fmaxf(top, fabsf(v));   // (passes NaN by)
+        };
+        hold(x[i][n].x), hold(x[i][n].y), hold(x[i][n].z), hold(x[i][n].w);
+      }
+    }
+  }
+  const bool joins = row0 < start;   // rows that stay are in the block
+  float* scale_at = c.scales[side] + of_head * (c.capacity / kCacheBlock) + block;
+  const float was = joins ? *scale_at : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  }
+  if (lane == 0) {
+    tops[side][warp] = top;
+  }
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[side][0], tops[side][1]), fmaxf(tops[side][2], tops[side][3]));
+  int exponent = ScaleExponentOf<Format>(top);
+  if (joins) {
+    exponent = max(exponent, ExponentOf(was));
+  }
+  const float inverse = PowerOfTwo(-exponent);   // (exponent is -126 .. 120)
+  uint8_t* codes = c.codes[side] + (of_head * c.capacity + row0 + 4 * warp) * c.head_dim;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row0 + 4 * warp + i;
+#pragma unroll
+    for (int n = 0; n < kTimes; ++n) {
+      const int f = lane + 32 * n;
+      if (f >= fours) {
+        continue;
+      }
+      uint32_t* to = reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(i) * c.head_dim) + f;
+      if (r >= start && r < end) {
+        const float4 v = x[i][n];
+        *to = Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+      } else if (r < start && exponent > ExponentOf(was)) {
+        const float4 v = DecodeFour<Format>(*to);
+        const float down = was * inverse;   // (0 where the scales are more than 2^149 apart, as the codes are then)
+        *to = Format::Encode(v.x * down, v.y * down, v.z * down, v.w * down);
+      }
+    }
+  }
+  if (warp == 0 && lane == 0) {
+    *scale_at = PowerOfTwo(exponent);
+  }
+  if (side == 0 && warp == 0 && lane < kCacheBlock && c.weights != nullptr && row0 + lane >= start && row0 + lane < end) {
+    c.weights[of_head * c.capacity + row0 + lane] = 0.f;
+  }
+}
+
+struct RowsArgs {
+  CacheView cache;
+  float* out[2];
+};
+constexpr int kRowsThreads = 256;
+constexpr int kRowsEach = 8;    // groups of four values of a thread
+
+// Items: kRowsThreads * kRowsEach groups of four values of a sequence's rows. Grid: (items, 2).
+template <typename Format>
+__global__ void __launch_bounds__(kRowsThreads)
+RowsKernel(const __grid_constant__ RowsArgs a, const __grid_constant__ BatchArgs batch) {
+  GridLaunchDependents();
+  GridDependencyWait();
+  const int side = blockIdx.y;
+  float* out = a.out[side];
+  if (out == nullptr) {
+    return;
+  }
+  const BatchEntry& e = batch.of[SequenceOf(batch, blockIdx.x)];
+  const CacheView& c = a.cache;
+  const int position = batch.positions[e.index];
+  const unsigned fours = c.head_dim / 4, width = fours * c.kv_heads;   // of a row
+  const int64_t first = static_cast<int64_t>(blockIdx.x - batch.first_item[&e - batch.of]) * (kRowsThreads * kRowsEach);
+  const int token0 = static_cast<int>(first / width);
+  const unsigned in_row0 = static_cast<unsigned>(first - static_cast<int64_t>(token0) * width) + threadIdx.x;
+  float4* to = reinterpret_cast<float4*>(out) + static_cast<int64_t>(e.row) * width + first + threadIdx.x;
+  uint32_t word[kRowsEach];
+  float scale[kRowsEach];
+#pragma unroll
+  for (int i = 0; i < kRowsEach; ++i) {
+    const unsigned beyond = (in_row0 + i * kRowsThreads) / width, in_row = in_row0 + i * kRowsThreads - beyond * width;
+    const int64_t token = static_cast<int64_t>(token0) + beyond;
+    const int64_t r = position + token;
+    word[i] = 0;
+    scale[i] = 0.f;
+    if (token < e.tokens && r >= 0 && r < c.capacity) {
+      const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + in_row / fours;
+      word[i] = __ldcs(reinterpret_cast<const uint32_t*>(c.codes[side] + (of_head * c.capacity + r) * c.head_dim) + in_row % fours);
+      scale[i] = c.scales[side][of_head * (c.capacity / kCacheBlock) + r / kCacheBlock];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRowsEach; ++i) {
+    if (static_cast<int64_t>(token0) + (in_row0 + i * kRowsThreads) / width < e.tokens) {
+      float4 v = DecodeFour<Format>(word[i]);
+      v.x *= scale[i], v.y *= scale[i], v.z *= scale[i], v.w *= scale[i];
+      __stcs(to + i * kRowsThreads, v);
+    }
+  }
+}
+
+int CheckConfig(const gufo_cuda_cache8_config& c) {
+  if (c.format != GUFO_CUDA_CACHE8_E4M3 && c.format != GUFO_CUDA_CACHE8_INT8) {
+    return Fail(GUFO_CUDA_UNSUPPORTED_TYPE, "cache8: formats are e4m3 and int8");
+  }
+  if (c.sequences < 1 || c.sequences > kCacheMaxSequences || c.kv_heads < 1 || c.kv_heads > 1024) {
+    return Fail(GUFO_CUDA_SHAPE, "cache8: 1 to 4096 sequences of 1 to 1024 KV heads");
+  }
+  if (c.head_dim < 16 || c.head_dim > kCacheMaxDim || c.head_dim % 16 != 0) {
+    return Fail(GUFO_CUDA_SHAPE, "cache8: head_dim is a multiple of 16, 16 to 256");
+  }
+  if (c.capacity < kCacheBlock || c.capacity % kCacheBlock != 0 || c.capacity > (1 << 28)) {
+    return Fail(GUFO_CUDA_SHAPE, "cache8: the capacity is a multiple of 16 rows, 2^28 at most");
+  }
+  return GUFO_CUDA_OK;
+}
+
+}  // namespace
+
+int CheckBatch(const Cache8& cache, const gufo_cuda_cache8_batch* b, const char* what, bool counted, int64_t* rows) {
+  const auto fail = [&](const char* why) { return Fail(GUFO_CUDA_BAD_ARGUMENT, std::string(what) + ": " + why); };
+  if (b == nullptr) {
+    return fail("null pointer");
+  }
+  if (b->sequences < 0 || b->sequences > cache.c.sequences) {
+    return fail("more sequences than the cache has");
+  }
+  if (b->positions == nullptr && b->sequences > 0) {
+    return fail("null pointer");
+  }
+  uint64_t seen[kCacheMaxSequences / 64] = {};
+  int64_t total = 0;
+  for (int i = 0; i < b->sequences; ++i) {
+    const int slot = b->slots != nullptr ? b->slots[i] : i;
+    if (slot < 0 || slot >= cache.c.sequences) {
+      return fail("no such slot");
+    }
+    if (seen[slot / 64] >> (slot % 64) & 1) {
+      return fail("a slot comes twice");
+    }
+    seen[slot / 64] |= 1ull << (slot % 64);
+    const int tokens = counted && b->tokens != nullptr ? b->tokens[i] : 1;
+    if (tokens < 0 || tokens > cache.c.capacity) {
+      return fail("a sequence has 0 to `capacity` tokens");
+    }
+    total += tokens;
+  }
+  if (total > (1 << 30)) {
+    return Fail(GUFO_CUDA_TOO_LARGE, std::string(what) + ": too many rows for one call");
+  }
+  *rows = total;
+  return GUFO_CUDA_OK;
+}
+
+int FindCache(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, const char* what, const Cache8** out) {
+  const auto it = ctx->caches.find(handle);
+  if (it == ctx->caches.end()) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, std::string(what) + ": unknown cache handle");
+  }
+  *out = &it->second;
+  return GUFO_CUDA_OK;
+}
+
+}  // namespace gufo
+
+using gufo::Fail;
+
+extern "C" {
+
+int gufo_cuda_cache8_create(gufo_cuda_ctx* ctx, const gufo_cuda_cache8_config* config, gufo_cuda_cache8* out) {
+  if (ctx == nullptr || config == nullptr || out == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_create: null pointer");
+  }
+  if (const int rc = gufo::CheckConfig(*config); rc != GUFO_CUDA_OK) {
+    return rc;
+  }
+  gufo::Cache8 cache;
+  cache.c = *config;
+  const size_t heads = static_cast<size_t>(config->sequences) * config->kv_heads;
+  const auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+  const size_t rows = heads * static_cast<size_t>(config->capacity);   // at most 2^50
+  const size_t codes = whole(rows * config->head_dim), scales = whole(rows / gufo::kCacheBlock * 4);
+  const size_t weights = config->weights != 0 ? whole(rows * 4) : 0;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
+  uint8_t* data = nullptr;
+  const size_t bytes = 2 * codes + 2 * scales + weights;
+  GUFO_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&data), bytes));
+  const cudaError_t e = cudaMemsetAsync(data, 0, bytes, ctx->stream);
+  if (e != cudaSuccess) {
+    cudaFree(data);
+    return gufo::CudaFail(e, "cache8_create");
+  }
+  cache.codes[0] = data;
+  cache.codes[1] = data + codes;
+  cache.scales[0] = reinterpret_cast<float*>(data + 2 * codes);
+  cache.scales[1] = reinterpret_cast<float*>(data + 2 * codes + scales);
+  cache.weights = weights != 0 ? reinterpret_cast<float*>(data + 2 * codes + 2 * scales) : nullptr;
+  const int64_t id = ctx->next_id++;
+  try {
+    ctx->caches.emplace(id, cache);
+  } catch (const std::bad_alloc&) {
+    cudaFree(data);
+    return Fail(GUFO_CUDA_OUT_OF_MEMORY, "cache8_create: host allocation failed");
+  }
+  *out = id;
+  return GUFO_CUDA_OK;
+}
+
+int gufo_cuda_cache8_free(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle) {
+  if (ctx == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_free: ctx is null");
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const auto it = ctx->caches.find(handle);
+  if (it == ctx->caches.end()) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_free: unknown cache handle");
+  }
+  GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
+  GUFO_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+  GUFO_CUDA_TRY(cudaFree(it->second.codes[0]));
+  ctx->caches.erase(it);
+  return GUFO_CUDA_OK;
+}
+
+int gufo_cuda_cache8_weights(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, float** weights) {
+  if (ctx == nullptr || weights == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_weights: null pointer");
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const gufo::Cache8* cache = nullptr;
+  if (const int rc = gufo::FindCache(ctx, handle, "cache8_weights", &cache); rc != GUFO_CUDA_OK) {
+    return rc;
+  }
+  *weights = cache->weights;
+  return GUFO_CUDA_OK;
+}
+
+int gufo_cuda_cache8_append_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, const gufo_cuda_cache8_batch* batch,
+                                   const float* keys, int64_t key_token_stride, int64_t key_head_stride,
+                                   const float* values, int64_t value_token_stride, int64_t value_head_stride) {
+  if (ctx == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_append: ctx is null");
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const gufo::Cache8* cache = nullptr;
+  int64_t rows = 0;
+  int rc = gufo::FindCache(ctx, handle, "cache8_append", &cache);
+  if (rc == GUFO_CUDA_OK) {
+    rc = gufo::CheckBatch(*cache, batch, "cache8_append", true, &rows);
+  }
+  if (rc != GUFO_CUDA_OK || rows == 0) {
+    return rc;
+  }
+  if (keys == nullptr || values == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_append: null pointer");
+  }
+  gufo::AppendArgs a{gufo::ViewOf(*cache), {keys, values}, {key_token_stride, value_token_stride},
+                     {key_head_stride, value_head_stride}, 0};
+  a.whole = ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15) == 0 &&
+            ((key_token_stride | key_head_stride | value_token_stride | value_head_stride) & 3) == 0;
+  GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
+  const auto kernel = cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::AppendKernel<gufo::E4m3> : gufo::AppendKernel<gufo::Int8>;
+  return gufo::ForEachRun(
+      *batch, [](int tokens) { return tokens > 0 ? (tokens - 1 + gufo::kCacheBlock - 1) / gufo::kCacheBlock + 1 : 0; },
+      [&](const gufo::BatchArgs& b, int blocks) -> int {
+        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(blocks, cache->c.kv_heads), dim3(gufo::kAppendThreads), 0, ctx->stream,
+                                             1, a, b));
+        ctx->launches.fetch_add(1);
+        return GUFO_CUDA_OK;
+      });
+}
+
+int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, const gufo_cuda_cache8_batch* batch, float* keys,
+                                 float* values) {
+  if (ctx == nullptr) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_rows: ctx is null");
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const gufo::Cache8* cache = nullptr;
+  int64_t rows = 0;
+  int rc = gufo::FindCache(ctx, handle, "cache8_rows", &cache);
+  if (rc == GUFO_CUDA_OK) {
+    rc = gufo::CheckBatch(*cache, batch, "cache8_rows", true, &rows);
+  }
+  if (rc != GUFO_CUDA_OK || rows == 0 || (keys == nullptr && values == nullptr)) {
+    return rc;
+  }
+  if (((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15) != 0) {
+    return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_rows: rows go to 16-byte boundaries");
+  }
+  const int64_t width = static_cast<int64_t>(cache->c.kv_heads) * cache->c.head_dim / 4;
+  constexpr int64_t kItem = gufo::kRowsThreads * gufo::kRowsEach;
+  if (rows * width / kItem + batch->sequences > INT32_MAX) {
+    return Fail(GUFO_CUDA_TOO_LARGE, "cache8_rows: too many rows for one call");
+  }
+  const gufo::RowsArgs a{gufo::ViewOf(*cache), {keys, values}};
+  GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
+  const auto kernel = cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::RowsKernel<gufo::E4m3> : gufo::RowsKernel<gufo::Int8>;
+  return gufo::ForEachRun(
+      *batch, [&](int tokens) { return static_cast<int>((tokens * width + kItem - 1) / kItem); },
+      [&](const gufo::BatchArgs& b, int items) -> int {
+        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(items, 2), dim3(gufo::kRowsThreads), 0, ctx->stream, 1, a, b));
+        ctx->launches.fetch_add(1);
+        return GUFO_CUDA_OK;
+      });
+}
+
+}  // extern "C"

@@ -83,6 +83,24 @@ struct DeltaNetLayer {
   float* ssm_norm = nullptr;
 };
 
+// A table of rotary frequencies (rope.cu).
+struct Rope {
+  unsigned long long* turns = nullptr;   // device [rope_dim / 2]: 2^-64 turns per position
+  int rope_dim = 0;
+  bool interleaved = false;
+  float magnitude = 1.f;
+};
+
+// A key / value cache in 8 bits (cache8.cu): device memory, laid out as
+// [sequences][kv_heads][capacity][head_dim] codes, [..][capacity / 16] scales and
+// [..][capacity] weights.
+struct Cache8 {
+  gufo_cuda_cache8_config c{};
+  uint8_t* codes[2] = {nullptr, nullptr};   // keys, values
+  float* scales[2] = {nullptr, nullptr};
+  float* weights = nullptr;                 // may be null
+};
+
 struct DeltaNetLayer;
 void SetError(const std::string& text);
 int Fail(int status, const std::string& text);
@@ -294,6 +312,8 @@ struct gufo_cuda_ctx {
   std::mutex mu;
   std::unordered_map<int64_t, gufo::Matrix> matrices;
   std::unordered_map<int64_t, gufo::DeltaNetLayer> deltanet_layers;
+  std::unordered_map<int64_t, gufo::Rope> ropes;
+  std::unordered_map<int64_t, gufo::Cache8> caches;
   int64_t next_id = 1;
   // Decoders on this context and what gives their resources back: a context that goes
   // first leaves them empty shells.

@@ -511,6 +511,12 @@ int gufo_cuda_ctx_destroy(gufo_cuda_ctx* ctx) {
     cudaFree(kv.second.dt_bias);
     cudaFree(kv.second.ssm_norm);
   }
+  for (auto& kv : ctx->ropes) {
+    cudaFree(kv.second.turns);
+  }
+  for (auto& kv : ctx->caches) {
+    cudaFree(kv.second.codes[0]);   // one allocation
+  }
   cudaFree(ctx->stage_x);
   cudaFree(ctx->stage_y);
   for (const auto& block : ctx->stream_blocks) {

@@ -1,7 +1,7 @@
 /* gufo_cuda.h - C ABI of the B200 (sm_100a) backend for gufo-npu's decode hot
  * path: GGUF Q4_K / Q6_K dequant-fused GEMV and small-M GEMM behind every
- * projection, bit-exact dequantization, the Gated DeltaNet decode step and the
- * routed-expert FFN of the MoE models.
+ * projection, bit-exact dequantization, the Gated DeltaNet decode step, the
+ * routed-expert FFN of the MoE models, and attention over a cache in 8 bits.
  *
  * This is the boundary a `src/cuda` backend binds beside the reference's
  * `src/npu`: plain pointers and sizes, no C++ types, no exceptions. Each entry
@@ -412,6 +412,175 @@ typedef struct gufo_cuda_attention_args {
 
 int gufo_cuda_attention_device(gufo_cuda_ctx* ctx,
                                const gufo_cuda_attention_args* args);
+
+/* ---- rotary positions ----------------------------------------------------- */
+
+/* Rotary positions by themselves, for rows of any number of tokens and any
+ * positions: what Mixer::Attention does to queries and keys ahead of the cache
+ * (src/models/qwen35/decoder.cpp:280-323), with the layouts and the scalings for
+ * long contexts that other checkpoints bring. */
+typedef int64_t gufo_cuda_rope; /* opaque handle of a frequency table (> 0) */
+enum {
+  GUFO_CUDA_ROPE_HALVES = 0, /* value i turns with value i + rope_dim / 2 */
+  GUFO_CUDA_ROPE_PAIRS = 1   /* value 2i turns with value 2i + 1 */
+};
+enum {
+  GUFO_CUDA_ROPE_UNSCALED = 0, /* theta^(-2i / rope_dim) per position */
+  GUFO_CUDA_ROPE_LINEAR = 1,   /* the same / factor */
+  /* Pairs that turn more than fast_turns times over original_positions as they are,
+   * those that turn less than slow_turns times / factor, the ones between mixed in
+   * proportion to the pair's number: low .. high, the pairs of fast_turns (rounded
+   * down) and slow_turns (rounded up) held inside 0 .. rope_dim / 2 - 1. */
+  GUFO_CUDA_ROPE_BY_PARTS = 2
+};
+typedef struct gufo_cuda_rope_params {
+  int rope_dim; /* even, 2 .. 512: how many of a head's first values turn */
+  int layout;
+  int scaling;
+  double theta;               /* > 1 */
+  double factor;              /* LINEAR, BY_PARTS: > 0 */
+  double original_positions;  /* BY_PARTS: > 0 */
+  double fast_turns, slow_turns; /* BY_PARTS: fast > slow > 0 */
+  double magnitude; /* factor of the rotated values; 0: 1, BY_PARTS 0.1 ln(factor) + 1 (at least 1) */
+} gufo_cuda_rope_params;
+
+/* The angles per position (radians, [rope_dim / 2]) and the factor that a handle of
+ * `params` has; needs no device. */
+int gufo_cuda_rope_frequencies(const gufo_cuda_rope_params* params, double* frequencies,
+                               double* magnitude);
+int gufo_cuda_rope_create(gufo_cuda_ctx* ctx, const gufo_cuda_rope_params* params,
+                          gufo_cuda_rope* out);
+int gufo_cuda_rope_free(gufo_cuda_ctx* ctx, gufo_cuda_rope rope);
+
+/* Rows that turn: `heads` heads of `head_dim` values (even, rope_dim .. 512) for each
+ * token, strides in floats. With norm_weight ([head_dim], device) a head's row goes
+ * through RMSNorm first. `out` may be `in` with the same strides; otherwise the two
+ * do not overlap. Values behind rope_dim are passed on (normed where asked). */
+typedef struct gufo_cuda_rope_rows {
+  const float* in;
+  int64_t in_token_stride, in_head_stride;
+  float* out;
+  int64_t out_token_stride, out_head_stride;
+  int heads;
+  int head_dim;
+  const float* norm_weight; /* may be NULL */
+  float rms_eps;
+} gufo_cuda_rope_rows;
+#define GUFO_CUDA_ROPE_PARTS 4
+/* Turns the rows of 1 to GUFO_CUDA_ROPE_PARTS parts (queries and keys, for example) in
+ * one launch: token t by positions[t] (device, any int). Angles are exact to some 2^-40
+ * of a turn whatever the position. Device pointers; only enqueues. */
+int gufo_cuda_rope_device(gufo_cuda_ctx* ctx, gufo_cuda_rope rope,
+                          const gufo_cuda_rope_rows* parts, int nparts,
+                          const int* positions, int tokens);
+
+/* ---- key / value cache in 8 bits -------------------------------------------- */
+
+/* Keys and values of one attention layer for a number of sequences, one byte a value:
+ * half of what the fp16 cache of gufo_cuda_attention_device holds. Sequence `slot`
+ * has `capacity` rows of kv_heads * head_dim keys and values. Blocks of
+ * GUFO_CUDA_CACHE8_BLOCK rows of a head share one scale for their keys and one for their
+ * values: the smallest power of two (2^-126 or more) with which the block's largest
+ * magnitude is no more than the format's largest code. A power of two, so that a scale
+ * that grows costs e4m3 codes nothing but what falls below their smallest value, and int8
+ * codes one more rounding.
+ * The caller keeps the number of rows that are held (as gufo_cuda_attention_args.position,
+ * one count for all layers); it may go back (a draft that is not kept) at any time.
+ * The reference has no counterpart (its cache is fp16). */
+typedef int64_t gufo_cuda_cache8; /* opaque handle (> 0) */
+enum {
+  GUFO_CUDA_CACHE8_E4M3 = 0, /* floating point, 3 fraction bits, largest 448 */
+  GUFO_CUDA_CACHE8_INT8 = 1  /* whole numbers -127 .. 127 */
+};
+#define GUFO_CUDA_CACHE8_BLOCK 16
+typedef struct gufo_cuda_cache8_config {
+  int sequences; /* 1 .. 4096 */
+  int kv_heads;  /* 1 .. 1024 */
+  int head_dim;  /* a multiple of 16, 16 .. 256 */
+  int capacity;  /* rows of a sequence: a multiple of 16 */
+  int format;
+  int weights;   /* != 0: room for a weight per row and KV head (gufo_cuda_cache8_evict_device) */
+} gufo_cuda_cache8_config;
+int gufo_cuda_cache8_create(gufo_cuda_ctx* ctx, const gufo_cuda_cache8_config* config,
+                            gufo_cuda_cache8* out);
+int gufo_cuda_cache8_free(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache);
+/* Device address of the accumulated weights, fp32 [sequences][kv_heads][capacity], zero
+ * at first; NULL without. */
+int gufo_cuda_cache8_weights(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache, float** weights);
+
+/* The sequences of a call. Rows of all sequences follow one another in the arrays of the
+ * call, tokens[i] of them for sequence i, which stand at positions[i] .. of slot slots[i].
+ * No slot may come twice. */
+typedef struct gufo_cuda_cache8_batch {
+  int sequences;
+  const int* slots;     /* host [sequences]; NULL: 0, 1, ... */
+  const int* tokens;    /* host [sequences], 0 .. capacity each; NULL: one each */
+  const int* positions; /* device [sequences]: rows held ahead of the call */
+} gufo_cuda_cache8_batch;
+
+/* Writes rows of keys and values [sum of tokens][kv_heads][head_dim] (fp32, device,
+ * strides in floats) at positions[i] .. of their slots and clears the rows' weights.
+ * Where a block holds rows already its scale grows if it has to, and their codes are
+ * rounded to it. Magnitudes above 2^127 and infinities saturate there; NaN stays NaN (int8:
+ * 0) and moves no scale. Rows that fall outside 0 .. capacity are left out. */
+int gufo_cuda_cache8_append_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
+                                   const gufo_cuda_cache8_batch* batch,
+                                   const float* keys, int64_t key_token_stride, int64_t key_head_stride,
+                                   const float* values, int64_t value_token_stride, int64_t value_head_stride);
+/* The values of the same rows: [sum of tokens][kv_heads][head_dim] fp32 each (either may be
+ * NULL); zeros for rows outside 0 .. capacity. */
+int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
+                                 const gufo_cuda_cache8_batch* batch, float* keys, float* values);
+
+/* Attention of each sequence's query tokens over its cached rows: for query head h, which
+ * reads KV head h / (heads / kv_heads),
+ *   out = softmax(q K^T * scale) V  [* sigmoid(gate)]
+ * Token t of a sequence sees rows 0 .. positions[i] + t (the rows of an append with the same
+ * batch included), or the first visible[...] rows where `visible` is given; a token that
+ * sees no row gets zeros. fp32 on the device, strides in floats; heads is a multiple of
+ * kv_heads. `out` overlaps none of the inputs.
+ * accumulate != 0 (caches with weights): adds the softmax weights, summed over the sequence's
+ * tokens and the query heads of a KV head, to the rows' weights.
+ * scratch: gufo_cuda_cache8_attend_scratch bytes, 16-byte aligned, cleared once before its
+ * first call (every call leaves its counters clear); calls that may be in flight together,
+ * those of captured graphs among them, need one each. Works in stream captures. */
+typedef struct gufo_cuda_cache8_attend_args {
+  int heads;
+  float scale; /* 0: 1 / sqrt(head_dim) */
+  const float* queries;
+  int64_t query_token_stride, query_head_stride;
+  const float* gate; /* may be NULL */
+  int64_t gate_token_stride, gate_head_stride;
+  float* out;
+  int64_t out_token_stride, out_head_stride;
+  const int* visible; /* device [sum of tokens]; may be NULL */
+  int accumulate;
+  void* scratch;
+  size_t scratch_bytes;
+} gufo_cuda_cache8_attend_args;
+/* Enough for calls of up to `tokens` query tokens in all. */
+int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache, int heads, int tokens,
+                                    int accumulate, size_t* bytes);
+int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
+                                   const gufo_cuda_cache8_batch* batch,
+                                   const gufo_cuda_cache8_attend_args* args);
+
+/* Brings every sequence of the batch that holds more than `budget` rows down to `budget`
+ * (batch->tokens is not read): for each KV head the first `first` rows stay, the last `last`
+ * ones, and of the rows between those of largest weight (of equal ones the lowest row; NaN
+ * counts as least), as far as the budget goes in this order. They move together, in their old
+ * order, to rows 0 .. budget - 1 with their weights; blocks get the scale of what they hold
+ * now. What stands in the rows behind them counts for nothing then. kept (device int32 [batch sequences][kv_heads]
+ * [budget]) receives the rows that stayed, -1 behind them where a sequence held fewer than
+ * budget, held (device int32 [batch sequences], may be NULL) the rows it holds now,
+ * min(positions[i], budget); held may not be positions. Queries keep the positions their
+ * keys were turned by: rotary positions do not go back with the rows.
+ * into != 0: the rows go to slots into_slots (host; NULL: the same slots) of that cache
+ * instead, which has the same kv_heads, head_dim and format and room for budget rows, and
+ * the source stays as it was; its weights go along where `into` has room for them. */
+int gufo_cuda_cache8_evict_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
+                                  const gufo_cuda_cache8_batch* batch, int budget, int first, int last,
+                                  int* kept, int* held, gufo_cuda_cache8 into, const int* into_slots);
 
 /* ---- routed experts (MoE models) ---------------------------------------- */
 
