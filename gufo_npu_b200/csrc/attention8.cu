@@ -18,14 +18,17 @@
 // of a key row, 8 of a value row are its own), which a sum over all of them does not see and
 // the output undoes.
 //
-// The split. Items are (sequence, KV head, group of query rows); each goes to `splits` blocks
-// of threads, of which those take part that the sequence is long enough for. The last of them to
-// arrive at a counter adds up the partial sums, in order.
+// The split. A unit of work is (sequence, group of query rows, KV head) with all the tiles
+// that the sequence is long. The device's resident blocks of threads share out the tiles of all
+// units, in order, to one tile: each finds its stretch from the lengths that it reads, whatever
+// they are, and goes through the units that it touches. A unit that several blocks have a part
+// of is put together by the last of them to arrive at a counter, part by part in order.
 //
 // The weights of the rows (for eviction) need every query's final maximum and sum: the scores
 // are written down as they come, 4 bytes against 2 * head_dim / group read for them, and a
 // second kernel turns them into weights and adds those up, one thread a row, in order.
 #include <climits>
+#include <type_traits>
 
 #include "cache8.cuh"
 #include "decode_device.cuh"
@@ -51,11 +54,9 @@ struct AttendArgs {
   int heads, group;
   float scale;             // times log2 e
   int whole;               // query rows may be read four values at a time
-  int splits;
-  int least_tiles;         // of a split
-  unsigned* arrived;       // [items][KV heads]
-  float* sums;             // [items][KV heads][splits][rows][head_dim]
-  float* stats;            // [items][KV heads][splits][rows][2]
+  unsigned* arrived;       // [blocks of threads]: of the unit that is cut behind a block's stretch
+  float* sums;             // [blocks][2: first, last unit][rows][head_dim]
+  float* stats;            // [blocks][2][rows][2]
   float* scores;           // [query rows][capacity]; null: no weights
   float* finals;           // [query rows][2]: maximum, 1 / sum
 };
@@ -87,37 +88,87 @@ __device__ __forceinline__ void Copy4(uint32_t to, const void* from) {
 // d = a b_low + a b_high: thirty-two products, added by the instruction.
 __device__ __forceinline__ void MmaHalves(float (&d)[4], const uint32_t (&a)[4], uint32_t high0, uint32_t high1, uint32_t low0,
                                           uint32_t low1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(low0), "r"(low1), "f"(0.f));
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(high0), "r"(high1));
 }
 __device__ __forceinline__ uint32_t Transpose(uint32_t v) {
   uint32_t t;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
   return t;
 }
 __device__ __forceinline__ uint32_t PackHalves(__half x, __half y) {
   return __half_as_ushort(x) | static_cast<uint32_t>(__half_as_ushort(y)) << 16;
 }
 
-// A task: query rows [row0, row0 + rows) of a sequence over rows 0 .. length of its cache.
+// A unit: query rows [row0, row0 + rows) of a sequence, one KV head.
 struct Task {
   BatchEntry e;
   int rows, row0;
   int position;
-  int length;    // rows that the sequence's tokens see, the most of them
 };
 
-__device__ __forceinline__ int SeenBy(const AttendArgs& a, const Task& t, int token) {
-  const int64_t seen = a.visible != nullptr ? a.visible[t.e.row + token] : static_cast<int64_t>(t.position) + token + 1;
+__device__ __forceinline__ int SeenBy(const AttendArgs& a, const BatchEntry& e, int position, int token) {
+  const int64_t seen = a.visible != nullptr ? a.visible[e.row + token] : static_cast<int64_t>(position) + token + 1;
   return static_cast<int>(min(max(seen, static_cast<int64_t>(0)), static_cast<int64_t>(a.cache.capacity)));
 }
 
-// Grid: (splits, KV heads, items).
+// Tiles of each sequence in `tiles` (one at least: a row that sees nothing is an output too) and
+// of the units of all sequences ahead of it in `ahead` ([sequences + 1]).
+__device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int* tiles, long long* ahead) {
+  __shared__ long long of_warp[kBatchSequences / 32];
+  const int n = batch.sequences, i = threadIdx.x, warp = i >> 5, lane = i & 31;
+  if (a.visible == nullptr) {
+    if (i < n) {
+      tiles[i] = SeenBy(a, batch.of[i], batch.positions[batch.of[i].index], batch.of[i].tokens - 1);
+    }
+  } else {
+    for (int s = warp; s < n; s += kWarps) {
+      int most = 0;
+      for (int token = lane; token < batch.of[s].tokens; token += 32) {
+        most = max(most, SeenBy(a, batch.of[s], 0, token));
+      }
+      most = __reduce_max_sync(0xFFFFFFFFu, most);
+      if (lane == 0) {
+        tiles[s] = most;
+      }
+    }
+  }
+  __syncthreads();
+  long long sum = 0;
+  if (i < kBatchSequences) {
+    long long mine = 0;
+    if (i < n) {
+      tiles[i] = max(1, (tiles[i] + kTile - 1) / kTile);
+      mine = static_cast<long long>(batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * tiles[i];
+    }
+    sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long below = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      sum += lane >= o ? below : 0;
+    }
+    if (lane == 31) {
+      of_warp[warp] = sum;
+    }
+  }
+  __syncthreads();
+  if (i < kBatchSequences) {
+    for (int w = 0; w < warp; ++w) {
+      sum += of_warp[w];
+    }
+    ahead[i + 1] = sum;
+    if (i == 0) {
+      ahead[0] = 0;
+    }
+  }
+  __syncthreads();
+}
+
+// Grid: resident blocks.
 template <typename Format, int NS, int RT>
 __global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
@@ -127,45 +178,31 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   __shared__ int row_seen[8 * RT];
   __shared__ float warp_top[kWarps][8 * RT], warp_total[kWarps][8 * RT];
   __shared__ float final_top[8 * RT], final_total[8 * RT];
+  __shared__ int tiles_of[kBatchSequences];
+  __shared__ long long tiles_ahead[kBatchSequences + 1];
   __shared__ int is_last;
   GridLaunchDependents();
   GridDependencyWait();
   const CacheView& c = a.cache;
-  const int split = blockIdx.x, kh = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  Task task;
-  const int at_entry = SequenceOf(batch, blockIdx.z);
-  task.e = batch.of[at_entry];
-  task.row0 = (blockIdx.z - batch.first_item[at_entry]) * 8 * RT;
-  task.rows = min(8 * RT, task.e.tokens * a.group - task.row0);
-  task.position = batch.positions[task.e.index];
-  if (threadIdx.x < 8 * RT) {
-    const int r = min(static_cast<int>(threadIdx.x), task.rows - 1);
-    row_seen[threadIdx.x] = SeenBy(a, task, (task.row0 + r) / a.group);
-  }
-  __syncthreads();
-  int length = 0, least = INT_MAX;
-#pragma unroll
-  for (int r = 0; r < 8 * RT; ++r) {
-    length = max(length, row_seen[r]);
-    least = min(least, row_seen[r]);
-  }
-  const int tiles = (length + kTile - 1) / kTile;
-  const int active = max(1, min(a.splits, tiles / a.least_tiles));
-  if (split >= active) {
+  ShareOut(a, batch, tiles_of, tiles_ahead);
+  const long long all = tiles_ahead[batch.sequences];
+  // A tile a warp at least.
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all / kWarps, 1ll)));
+  if (blockIdx.x >= blocks) {
     return;
   }
-  const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / active);
-  const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / active);
-  const size_t of_head = static_cast<size_t>(task.e.slot) * c.kv_heads + kh;
-  const uint8_t* keys = c.codes[0] + of_head * c.capacity * c.head_dim;
-  const uint8_t* values = c.codes[1] + of_head * c.capacity * c.head_dim;
-  const float* key_scales = c.scales[0] + of_head * (c.capacity / kTile);
-  const float* value_scales = c.scales[1] + of_head * (c.capacity / kTile);
+  const auto start_of = [&](long long block) { return all * block / blocks; };
+  const auto owner_of = [&](long long tile) {     // the block whose stretch it is in
+    int b = static_cast<int>(tile * blocks / all);
+    while (start_of(b + 1) <= tile) {
+      ++b;
+    }
+    return b;
+  };
+  const long long begin = start_of(blockIdx.x), end = start_of(blockIdx.x + 1ll);
 
-  // ---- the ring
-  uint8_t* ring = raw + warp * (S::kStages * S::kStage);
   constexpr int kPieces = S::kRowBytes / 16;    // of a row
   // Where a piece of a row stands, so that the eight lanes that read together meet eight
   // different places of 16 bytes: keys by four pieces of two rows, values by two pieces of
@@ -178,432 +215,513 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       return (r * kPieces + (piece ^ (2 * (r >> 1 & 3)))) * 16;
     }
   };
-  auto load = [&](int tile, int stage) {
-    if (tile < end) {
-      uint8_t* to = ring + stage * S::kStage;
-      const uint32_t to_keys = SharedAt(to), to_values = to_keys + S::kSide;
-#pragma unroll
-      for (int i = 0; i < kTile * kPieces / 32; ++i) {
-        const int at = lane + 32 * i, r = at / kPieces, piece = at % kPieces;
-        const bool there = tile * kTile + r < length && piece * 16 < c.head_dim;
-        const size_t from = there ? (static_cast<size_t>(tile) * kTile + r) * c.head_dim + piece * 16 : 0;
-        Copy16(to_keys + key_at(r, piece), keys + from, there);
-        Copy16(to_values + value_at(r, piece), values + from, there);
-      }
-      if (lane < 2) {
-        Copy4(to_keys + 2 * S::kSide + 4 * lane, (lane == 0 ? key_scales : value_scales) + tile);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  const int my_first = first + warp;
-#pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) {
-    load(my_first + i * kWarps, i);
-  }
-
-  // ---- the queries: row 8 rt + w to warp w, in the order of the B operands
+  uint8_t* ring = raw + warp * (S::kStages * S::kStage);
   uint4* query = reinterpret_cast<uint4*>(raw + S::kShared);   // [rt][seg * 4 + j][lane]: high pair, pair, low pair, pair
+
+#pragma unroll 1
+  for (long long from = begin; from < end;) {
+    // ---- the unit that this tile is of
+    int low = 0, high = batch.sequences - 1;
+    while (low < high) {
+      const int mid = (low + high + 1) / 2;
+      if (tiles_ahead[mid] <= from) {
+        low = mid;
+      } else {
+        high = mid - 1;
+      }
+    }
+    const int tiles = tiles_of[low];
+    const long long unit = (from - tiles_ahead[low]) / tiles;
+    const long long unit_start = tiles_ahead[low] + unit * tiles;
+    const int kh = static_cast<int>(unit % c.kv_heads);
+    const long long to = min(end, unit_start + tiles);
+    Task task;
+    task.e = batch.of[low];
+    task.row0 = static_cast<int>(unit / c.kv_heads) * 8 * RT;
+    task.rows = min(8 * RT, task.e.tokens * a.group - task.row0);
+    task.position = batch.positions[task.e.index];
+    if (threadIdx.x < 8 * RT) {
+      const int r = min(static_cast<int>(threadIdx.x), task.rows - 1);
+      row_seen[threadIdx.x] = SeenBy(a, task.e, task.position, (task.row0 + r) / a.group);
+    }
+    __syncthreads();
+    int length = 0, least = INT_MAX;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = 8 * rt + warp;
-    const bool there = r < task.rows;
-    const int flat = task.row0 + (there ? r : 0);
-    const int token = flat / a.group, head = kh * a.group + flat % a.group;
-    const float* from = a.queries + (static_cast<int64_t>(task.e.row) + token) * a.query_token_stride + head * a.query_head_stride;
-    constexpr int kTimes = (16 * NS + 31) / 32;
-    float4 x[kTimes];
-    uint32_t top = 0;
+    for (int r = 0; r < 8 * RT; ++r) {
+      length = max(length, row_seen[r]);
+      least = min(least, row_seen[r]);
+    }
+    // (These rows may see less than the sequence's last ones.)
+    const int first_tile = static_cast<int>(from - unit_start);
+    const int end_tile = min(static_cast<int>(to - unit_start), (length + kTile - 1) / kTile);
+    const size_t of_head = static_cast<size_t>(task.e.slot) * c.kv_heads + kh;
+    const uint8_t* keys = c.codes[0] + of_head * c.capacity * c.head_dim;
+    const uint8_t* values = c.codes[1] + of_head * c.capacity * c.head_dim;
+    const float* scale_from = c.scales[lane & 1] + of_head * (c.capacity / kTile);   // lane 0: keys, 1: values
+
+    // ---- the ring
+    const int whole_tiles = c.head_dim == S::kRowBytes ? length / kTile : 0;   // that can be copied as they are
+    auto load = [&](int tile, int stage) {
+      if (tile < end_tile) {
+        const uint32_t to_keys = SharedAt(ring + stage * S::kStage), to_values = to_keys + S::kSide;
+        constexpr int kEach = 32 / kPieces;     // rows that the lanes copy at a time
+        const int r0 = lane / kPieces, piece = lane % kPieces;
+        if (tile < whole_tiles) {
+          const uint8_t* k = keys + static_cast<size_t>(tile) * S::kSide + lane * 16;
+          const uint8_t* v = values + static_cast<size_t>(tile) * S::kSide + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kTimes; ++i) {
-      const int f = lane + 32 * i;
-      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (there && 4 * f < c.head_dim) {
-        if (a.whole) {
-          x[i] = *reinterpret_cast<const float4*>(from + 4 * f);
+          for (int i = 0; i < kTile / kEach; ++i) {
+            Copy16(to_keys + key_at(r0, piece) + 512 * i, k + 512 * i, true);
+          }
+#pragma unroll
+          for (int i = 0; i < kTile / kEach; ++i) {
+            Copy16(to_values + value_at(r0 + kEach * i, piece), v + 512 * i, true);
+          }
         } else {
-          x[i] = make_float4(from[4 * f], from[4 * f + 1], from[4 * f + 2], from[4 * f + 3]);
-        }
-      }
-      top = max(max(top, __float_as_uint(x[i].x) & 0x7FFFFFFFu), __float_as_uint(x[i].y) & 0x7FFFFFFFu);
-      top = max(max(top, __float_as_uint(x[i].z) & 0x7FFFFFFFu), __float_as_uint(x[i].w) & 0x7FFFFFFFu);
-    }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    // The largest to 2^14 .. 2^15. (Products with codes of up to 448 and their sums stay in fp32's range.)
-    const int e = min(max(static_cast<int>(top >> 23), 16), 250);
-    const float up = PowerOfTwo(141 - e);
-#pragma unroll
-    for (int i = 0; i < kTimes; ++i) {
-      const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
-      if (f < 16 * NS) {
-        const int seg = f / 16, of = f % 16 / 4, j = f % 4;
-        const float v[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
-        __half high[4], low[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          high[k] = __float2half_rn(v[k]);
-          low[k] = __float2half_rn(v[k] - __half2float(high[k]));
-        }
-        query[(rt * 4 * NS + seg * 4 + j) * 32 + warp * 4 + of] = make_uint4(
-            PackHalves(high[0], high[1]), PackHalves(high[2], high[3]), PackHalves(low[0], low[1]), PackHalves(low[2], low[3]));
-      }
-    }
-    if (lane == 0) {
-      row_factor[r] = a.scale * PowerOfTwo(e - 141);
-    }
-  }
-  __syncthreads();
-
-  // ---- the tiles
-  float factor[RT][2];
-  int seen[RT][2];
-  float top[RT][2], total[RT][2];      // of query rows 8 rt + 2 t, + 1; the sum is this lane's rows' part
-  float acc[RT][4 * NS][4];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      factor[rt][i] = row_factor[8 * rt + 2 * t + i];
-      seen[rt][i] = row_seen[8 * rt + 2 * t + i];
-      top[rt][i] = -INFINITY;
-      total[rt][i] = 0.f;
-    }
-#pragma unroll
-    for (int m = 0; m < 4 * NS; ++m) {
-      acc[rt][m][0] = acc[rt][m][1] = acc[rt][m][2] = acc[rt][m][3] = 0.f;
-    }
-  }
-  int stage = 0;
 #pragma unroll 1
-  for (int tile = my_first; tile < end; tile += kWarps) {
-    load(tile + (S::kStages - 1) * kWarps, stage == 0 ? S::kStages - 1 : stage - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
-    __syncwarp();
-    const uint8_t* here = ring + stage * S::kStage;
-    const float2 scales = *reinterpret_cast<const float2*>(here + 2 * S::kSide);
-    // Scores.
-    float s[RT][4];
+          for (int i = 0; i < kTile / kEach; ++i) {
+            const int r = r0 + kEach * i;
+            const bool there = tile * kTile + r < length && piece * 16 < c.head_dim;
+            const size_t at = there ? (static_cast<size_t>(tile) * kTile + r) * c.head_dim + piece * 16 : 0;
+            Copy16(to_keys + key_at(r, piece), keys + at, there);
+            Copy16(to_values + value_at(r, piece), values + at, there);
+          }
+        }
+        if (lane < 2) {
+          Copy4(to_keys + 2 * S::kSide + 4 * lane, scale_from + tile);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int my_first = first_tile + warp;
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) {
+      load(my_first + i * kWarps, i);
+    }
+
+    // ---- the queries: row 8 rt + w to warp w, in the order of the B operands
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
-    }
+      const int r = 8 * rt + warp;
+      const bool there = r < task.rows;
+      const int flat = task.row0 + (there ? r : 0);
+      const int token = flat / a.group, head = kh * a.group + flat % a.group;
+      const float* row = a.queries + (static_cast<int64_t>(task.e.row) + token) * a.query_token_stride + head * a.query_head_stride;
+      constexpr int kTimes = (16 * NS + 31) / 32;
+      float4 x[kTimes];
+      uint32_t top = 0;
 #pragma unroll
-    for (int seg = 0; seg < NS; ++seg) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(here + key_at(g, 4 * seg + t));
-      const uint4 k1 = *reinterpret_cast<const uint4*>(here + key_at(g + 8, 4 * seg + t));
-      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+      for (int i = 0; i < kTimes; ++i) {
+        const int f = lane + 32 * i;
+        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there && 4 * f < c.head_dim) {
+          if (a.whole) {
+            x[i] = *reinterpret_cast<const float4*>(row + 4 * f);
+          } else {
+            x[i] = make_float4(row[4 * f], row[4 * f + 1], row[4 * f + 2], row[4 * f + 3]);
+          }
+        }
+        top = max(max(top, __float_as_uint(x[i].x) & 0x7FFFFFFFu), __float_as_uint(x[i].y) & 0x7FFFFFFFu);
+        top = max(max(top, __float_as_uint(x[i].z) & 0x7FFFFFFFu), __float_as_uint(x[i].w) & 0x7FFFFFFFu);
+      }
+      top = __reduce_max_sync(0xFFFFFFFFu, top);
+      // The largest to 2^14 .. 2^15. (Products with codes of up to 448 and their sums stay in fp32's range.)
+      const int e = min(max(static_cast<int>(top >> 23), 16), 250);
+      const float up = PowerOfTwo(141 - e);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t k[4];
-        Format::Decode(w0[j], k[0], k[2]);
-        Format::Decode(w1[j], k[1], k[3]);
+      for (int i = 0; i < kTimes; ++i) {
+        const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
+        if (f < 16 * NS) {
+          const int seg = f / 16, of = f % 16 / 4, j = f % 4;
+          const float v[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
+          __half high[4], low[4];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const uint4 q = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
-          float d[4];
-          MmaHalves(d, k, q.x, q.y, q.z, q.w);
-          s[rt][0] += d[0], s[rt][1] += d[1], s[rt][2] += d[2], s[rt][3] += d[3];
+          for (int k = 0; k < 4; ++k) {
+            high[k] = __float2half_rn(v[k]);
+            low[k] = __float2half_rn(v[k] - __half2float(high[k]));
+          }
+          query[(rt * 4 * NS + seg * 4 + j) * 32 + warp * 4 + of] = make_uint4(
+              PackHalves(high[0], high[1]), PackHalves(high[2], high[3]), PackHalves(low[0], low[1]), PackHalves(low[2], low[3]));
         }
       }
+      if (lane == 0) {
+        row_factor[r] = a.scale * PowerOfTwo(e - 141);
+      }
     }
-    const int r0 = tile * kTile + g;
-    uint32_t p[RT][4];       // high pair of rows 0-7, of 8-15; low pairs
+    __syncthreads();
+
+    // ---- the tiles
+    float factor[RT][2];
+    int seen[RT][2];
+    float top[RT][2], total[RT][2];      // of query rows 8 rt + 2 t, + 1; the sum is this lane's rows' part
+    float acc[RT][4 * NS][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[rt][i] *= factor[rt][i & 1] * scales.x;
-      }
-      if (a.scores != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 8 * rt + 2 * t + (i & 1), row = r0 + 8 * (i >> 1);
-          if (r < task.rows && row < length) {
-            const int flat = task.row0 + r;
-            const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
-            __stcg(a.scores + at * c.capacity + row, s[rt][i]);
-          }
-        }
-      }
-      if ((tile + 1) * kTile > least) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[rt][i] = r0 + 8 * (i >> 1) < seen[rt][i & 1] ? s[rt][i] : -INFINITY;
-        }
-      }
-      const float m0 = fmaxf(s[rt][0], s[rt][2]), m1 = fmaxf(s[rt][1], s[rt][3]);
-      if (__any_sync(0xFFFFFFFFu, m0 > top[rt][0] || m1 > top[rt][1])) {
-        float n0 = fmaxf(m0, top[rt][0]), n1 = fmaxf(m1, top[rt][1]);
-#pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) {
-          n0 = fmaxf(n0, __shfl_xor_sync(0xFFFFFFFFu, n0, o));
-          n1 = fmaxf(n1, __shfl_xor_sync(0xFFFFFFFFu, n1, o));
-        }
-        const float keep0 = n0 == -INFINITY ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == -INFINITY ? 1.f : exp2f(top[rt][1] - n1);
-        top[rt][0] = n0, top[rt][1] = n1;
-        total[rt][0] *= keep0, total[rt][1] *= keep1;
-#pragma unroll
-        for (int m = 0; m < 4 * NS; ++m) {
-          acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
-        }
-      }
-      const float t0 = top[rt][0] == -INFINITY ? 0.f : top[rt][0], t1 = top[rt][1] == -INFINITY ? 0.f : top[rt][1];
-      const float e0 = exp2f(s[rt][0] - t0), e1 = exp2f(s[rt][1] - t1), e2 = exp2f(s[rt][2] - t0), e3 = exp2f(s[rt][3] - t1);
-      total[rt][0] += e0 + e2;
-      total[rt][1] += e1 + e3;
-      const float x[4] = {e0 * kProbScale, e1 * kProbScale, e2 * kProbScale, e3 * kProbScale};
-      __half high[4], low[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        high[i] = __float2half_rn(x[i]);
-        low[i] = __float2half_rn(x[i] - __half2float(high[i]));
-      }
-      p[rt][0] = Transpose(PackHalves(high[0], high[1]));
-      p[rt][1] = Transpose(PackHalves(high[2], high[3]));
-      p[rt][2] = Transpose(PackHalves(low[0], low[1]));
-      p[rt][3] = Transpose(PackHalves(low[2], low[3]));
-    }
-    if constexpr (Format::kHasNan) {
-      // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
-      // others, whose weight of 0 times NaN would: where some do not see all rows of a tile, such
-      // values are put into the sums by hand and taken out of the tile.
-      if ((tile + 1) * kTile > least) {
-        uint8_t* there = ring + stage * S::kStage + S::kSide;
-        const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
-        uint32_t found = 0;
-#pragma unroll
-        for (int i = 0; i < S::kSide / 16 / 32; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(there + 16 * (lane + 32 * i));
-          found |= marks(w.x) | marks(w.y) | marks(w.z) | marks(w.w);
-        }
-        if (__any_sync(0xFFFFFFFFu, found != 0)) {
-#pragma unroll
-          for (int m = 0; m < 4 * NS; ++m) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int dim = 64 * (m / 4) + 8 * g + 2 * (m % 4) + half;
-              int rows = INT_MAX;      // the first with NaN
-#pragma unroll 1
-              for (int r = kTile - 1; r >= 0; --r) {
-                rows = (there[value_at(r, dim >> 4) + (dim & 15)] & 0x7F) == 0x7F ? tile * kTile + r : rows;
-              }
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) {
-                acc[rt][m][2 * half] = rows < seen[rt][0] ? NAN : acc[rt][m][2 * half];
-                acc[rt][m][2 * half + 1] = rows < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
-              }
-            }
-          }
-          __syncwarp();
-#pragma unroll 1
-          for (int i = 0; i < S::kSide / 4 / 32; ++i) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(there) + lane + 32 * i;
-            *w &= ~((marks(*w) >> 7) * 255u);
-          }
-          __syncwarp();
-        }
-      }
-    }
-    // Weighted rows.
-    const float by = scales.y * (1.f / kProbScale);
-#pragma unroll
-    for (int seg = 0; seg < NS; ++seg) {
-      uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-        v[i] = *reinterpret_cast<const uint2*>(here + S::kSide + value_at(r, 4 * seg + (g >> 1)) + 8 * (g & 1));
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t w0 = half ? v[0].y : v[0].x, w1 = half ? v[1].y : v[1].x, w2 = half ? v[2].y : v[2].x, w3 = half ? v[3].y : v[3].x;
-#pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
-          uint32_t b[4];   // dimensions 2 pair, 2 pair + 1 of the word: rows beside one another
-          Format::Decode(__byte_perm(w0, w1, pair ? 0x7362 : 0x5140), b[0], b[1]);
-          Format::Decode(__byte_perm(w2, w3, pair ? 0x7362 : 0x5140), b[2], b[3]);
-          const int m = 4 * seg + 2 * half + pair;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            float d[4];
-            MmaHalves(d, b, p[rt][0], p[rt][1], p[rt][2], p[rt][3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              acc[rt][m][i] = fmaf(d[i], by, acc[rt][m][i]);
-            }
-          }
-        }
-      }
-    }
-    __syncwarp();      // the stage is free
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-
-  // ---- the warps' parts together
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum = total[rt][i];
-#pragma unroll
-      for (int o = 4; o <= 16; o <<= 1) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      }
-      if (g == 0) {
-        warp_top[warp][8 * rt + 2 * t + i] = top[rt][i];
-        warp_total[warp][8 * rt + 2 * t + i] = sum;
-      }
-    }
-  }
-  __syncthreads();     // the rings are free
-  float* join = reinterpret_cast<float*>(raw);      // [warp][row][64 NS]
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-    for (int seg = 0; seg < NS; ++seg) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float* to = join + (warp * 8 * RT + 8 * rt + 2 * t + i) * 64 * NS + 64 * seg + 8 * g;
-        *reinterpret_cast<float4*>(to) = make_float4(acc[rt][4 * seg][i], acc[rt][4 * seg][i + 2], acc[rt][4 * seg + 1][i],
-                                                     acc[rt][4 * seg + 1][i + 2]);
-        *reinterpret_cast<float4*>(to + 4) = make_float4(acc[rt][4 * seg + 2][i], acc[rt][4 * seg + 2][i + 2],
-                                                         acc[rt][4 * seg + 3][i], acc[rt][4 * seg + 3][i + 2]);
+        factor[rt][i] = row_factor[8 * rt + 2 * t + i];
+        seen[rt][i] = row_seen[8 * rt + 2 * t + i];
+        top[rt][i] = -INFINITY;
+        total[rt][i] = 0.f;
+      }
+#pragma unroll
+      for (int m = 0; m < 4 * NS; ++m) {
+        acc[rt][m][0] = acc[rt][m][1] = acc[rt][m][2] = acc[rt][m][3] = 0.f;
       }
     }
-  }
-  if (threadIdx.x < 8 * RT) {
-    const int r = threadIdx.x;
-    float most = -INFINITY;
+    // RA: groups of eight rows that there are.
+    const auto go = [&](auto groups) {
+      constexpr int RA = decltype(groups)::value;
+      int stage = 0;
+#pragma unroll 1
+      for (int tile = my_first; tile < end_tile; tile += kWarps) {
+        load(tile + (S::kStages - 1) * kWarps, stage == 0 ? S::kStages - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+        __syncwarp();
+        uint8_t* here = ring + stage * S::kStage;
+        const float2 scales = *reinterpret_cast<const float2*>(here + 2 * S::kSide);
+        // Scores.
+        float s[RA][4];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      most = fmaxf(most, warp_top[w][r]);
-    }
-    float sum = 0.f;
+        for (int rt = 0; rt < RA; ++rt) {
+          s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
+        }
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float by = most == -INFINITY ? 1.f : exp2f(warp_top[w][r] - most);
-      sum += warp_total[w][r] * by;
-      warp_top[w][r] = by;      // from now on the factor of the warp's sums
+        for (int seg = 0; seg < NS; ++seg) {
+          const uint4 k0 = *reinterpret_cast<const uint4*>(here + key_at(g, 4 * seg + t));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(here + key_at(g + 8, 4 * seg + t));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t k[4];
+            Format::Decode(w0[j], k[0], k[2]);
+            Format::Decode(w1[j], k[1], k[3]);
+#pragma unroll
+            for (int rt = 0; rt < RA; ++rt) {
+              const uint4 q = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
+              float d[4];
+              MmaHalves(d, k, q.x, q.y, q.z, q.w);
+              s[rt][0] += d[0], s[rt][1] += d[1], s[rt][2] += d[2], s[rt][3] += d[3];
+            }
+          }
+        }
+        const int r0 = tile * kTile + g;
+        const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
+        uint32_t p[RA][4];       // high pair of rows 0-7, of 8-15; low pairs
+#pragma unroll
+        for (int rt = 0; rt < RA; ++rt) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[rt][i] *= factor[rt][i & 1] * scales.x;
+          }
+          if (a.scores != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 8 * rt + 2 * t + (i & 1), row = r0 + 8 * (i >> 1);
+              if (r < task.rows && row < length) {
+                const int flat = task.row0 + r;
+                const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
+                __stcg(a.scores + at * c.capacity + row, s[rt][i]);
+              }
+            }
+          }
+          if (hides) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[rt][i] = r0 + 8 * (i >> 1) < seen[rt][i & 1] ? s[rt][i] : -INFINITY;
+            }
+          }
+          const float m0 = fmaxf(s[rt][0], s[rt][2]), m1 = fmaxf(s[rt][1], s[rt][3]);
+          if (__any_sync(0xFFFFFFFFu, m0 > top[rt][0] || m1 > top[rt][1])) {
+            float n0 = fmaxf(m0, top[rt][0]), n1 = fmaxf(m1, top[rt][1]);
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) {
+              n0 = fmaxf(n0, __shfl_xor_sync(0xFFFFFFFFu, n0, o));
+              n1 = fmaxf(n1, __shfl_xor_sync(0xFFFFFFFFu, n1, o));
+            }
+            const float keep0 = n0 == -INFINITY ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == -INFINITY ? 1.f : exp2f(top[rt][1] - n1);
+            top[rt][0] = n0, top[rt][1] = n1;
+            total[rt][0] *= keep0, total[rt][1] *= keep1;
+#pragma unroll
+            for (int m = 0; m < 4 * NS; ++m) {
+              acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
+            }
+          }
+          const float t0 = top[rt][0] == -INFINITY ? 0.f : top[rt][0], t1 = top[rt][1] == -INFINITY ? 0.f : top[rt][1];
+          const float e0 = exp2f(s[rt][0] - t0), e1 = exp2f(s[rt][1] - t1), e2 = exp2f(s[rt][2] - t0), e3 = exp2f(s[rt][3] - t1);
+          total[rt][0] += e0 + e2;
+          total[rt][1] += e1 + e3;
+          const float x[4] = {e0 * kProbScale, e1 * kProbScale, e2 * kProbScale, e3 * kProbScale};
+          __half high[4], low[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            high[i] = __float2half_rn(x[i]);
+            low[i] = __float2half_rn(x[i] - __half2float(high[i]));
+          }
+          p[rt][0] = Transpose(PackHalves(high[0], high[1]));
+          p[rt][1] = Transpose(PackHalves(high[2], high[3]));
+          p[rt][2] = Transpose(PackHalves(low[0], low[1]));
+          p[rt][3] = Transpose(PackHalves(low[2], low[3]));
+        }
+        if constexpr (Format::kHasNan) {
+          // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
+          // others, whose weight of 0 times NaN would: where some do not see all rows of a tile, such
+          // values are put into the sums by hand and taken out of the tile.
+          if (hides) {
+            uint8_t* there = here + S::kSide;
+            const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
+            uint32_t found = 0;
+#pragma unroll 1
+            for (int i = 0; i < S::kSide / 16 / 32; ++i) {
+              const uint4 w = *reinterpret_cast<const uint4*>(there + 16 * (lane + 32 * i));
+              found |= marks(w.x) | marks(w.y) | marks(w.z) | marks(w.w);
+            }
+            if (__any_sync(0xFFFFFFFFu, found != 0)) {
+#pragma unroll
+              for (int m = 0; m < 4 * NS; ++m) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const int dim = 64 * (m / 4) + 8 * g + 2 * (m % 4) + half;
+                  int rows = INT_MAX;      // the first with NaN
+#pragma unroll 1
+                  for (int r = kTile - 1; r >= 0; --r) {
+                    rows = (there[value_at(r, dim >> 4) + (dim & 15)] & 0x7F) == 0x7F ? tile * kTile + r : rows;
+                  }
+#pragma unroll
+                  for (int rt = 0; rt < RA; ++rt) {
+                    acc[rt][m][2 * half] = rows < seen[rt][0] ? NAN : acc[rt][m][2 * half];
+                    acc[rt][m][2 * half + 1] = rows < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
+                  }
+                }
+              }
+              __syncwarp();
+#pragma unroll 1
+              for (int i = 0; i < S::kSide / 4 / 32; ++i) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(there) + lane + 32 * i;
+                *w &= ~((marks(*w) >> 7) * 255u);
+              }
+              __syncwarp();
+            }
+          }
+        }
+        // Weighted rows.
+        const float by = scales.y * (1.f / kProbScale);
+#pragma unroll
+        for (int seg = 0; seg < NS; ++seg) {
+          uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+            v[i] = *reinterpret_cast<const uint2*>(here + S::kSide + value_at(r, 4 * seg + (g >> 1)) + 8 * (g & 1));
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t w0 = half ? v[0].y : v[0].x, w1 = half ? v[1].y : v[1].x, w2 = half ? v[2].y : v[2].x, w3 = half ? v[3].y : v[3].x;
+#pragma unroll
+            for (int pair = 0; pair < 2; ++pair) {
+              uint32_t b[4];   // dimensions 2 pair, 2 pair + 1 of the word: rows beside one another
+              Format::Decode(__byte_perm(w0, w1, pair ? 0x7362 : 0x5140), b[0], b[1]);
+              Format::Decode(__byte_perm(w2, w3, pair ? 0x7362 : 0x5140), b[2], b[3]);
+              const int m = 4 * seg + 2 * half + pair;
+#pragma unroll
+              for (int rt = 0; rt < RA; ++rt) {
+                float d[4];
+                MmaHalves(d, b, p[rt][0], p[rt][1], p[rt][2], p[rt][3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  acc[rt][m][i] = fmaf(d[i], by, acc[rt][m][i]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();      // the stage is free
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      }
+    };
+    if constexpr (RT == 1) {
+      go(std::integral_constant<int, 1>());
+    } else if (task.rows <= 8) {
+      go(std::integral_constant<int, 1>());
+    } else if (RT == 2 || task.rows <= 16) {
+      go(std::integral_constant<int, 2>());
+    } else {
+      go(std::integral_constant<int, RT>());
     }
-    final_top[r] = most;
-    final_total[r] = sum;
-  }
-  __syncthreads();
-  const int item = blockIdx.z * c.kv_heads + kh;
-  const int fours = c.head_dim / 4;
-  // Four dimensions of a row of the output, gated; a row that saw nothing is zero.
-  auto finish = [&](int r, int f, float4 v, float sum, int sees) {
-    const int flat = task.row0 + r;
-    const int64_t token = static_cast<int64_t>(task.e.row) + flat / a.group;
-    const int head = kh * a.group + flat % a.group;
-    const float by = 1.f / sum;
-    float o[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
-    if (a.gate != nullptr) {
-      const float* gate = a.gate + token * a.gate_token_stride + head * a.gate_head_stride + 4 * f;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+
+    // ---- the warps' parts together
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum = total[rt][i];
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) {
+          sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        }
+        if (g == 0) {
+          warp_top[warp][8 * rt + 2 * t + i] = top[rt][i];
+          warp_total[warp][8 * rt + 2 * t + i] = sum;
+        }
+      }
+    }
+    __syncthreads();     // the rings are free
+    float* join = reinterpret_cast<float*>(raw);      // [warp][row][64 NS]
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (8 * rt < task.rows) {
+#pragma unroll
+        for (int seg = 0; seg < NS; ++seg) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float* out = join + (warp * 8 * RT + 8 * rt + 2 * t + i) * 64 * NS + 64 * seg + 8 * g;
+            *reinterpret_cast<float4*>(out) = make_float4(acc[rt][4 * seg][i], acc[rt][4 * seg][i + 2], acc[rt][4 * seg + 1][i],
+                                                          acc[rt][4 * seg + 1][i + 2]);
+            *reinterpret_cast<float4*>(out + 4) = make_float4(acc[rt][4 * seg + 2][i], acc[rt][4 * seg + 2][i + 2],
+                                                              acc[rt][4 * seg + 3][i], acc[rt][4 * seg + 3][i + 2]);
+          }
+        }
+      }
+    }
+    if (threadIdx.x < 8 * RT) {
+      const int r = threadIdx.x;
+      float most = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        most = fmaxf(most, warp_top[w][r]);
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float by = most == -INFINITY ? 1.f : exp2f(warp_top[w][r] - most);
+        sum += warp_total[w][r] * by;
+        warp_top[w][r] = by;      // from now on the factor of the warp's sums
+      }
+      final_top[r] = most;
+      final_total[r] = sum;
+    }
+    __syncthreads();
+    const int fours = c.head_dim / 4;
+    // Four dimensions of a row of the output, gated; a row that saw nothing is zero.
+    auto finish = [&](int r, int f, float4 v, float sum, int sees) {
+      const int flat = task.row0 + r;
+      const int64_t token = static_cast<int64_t>(task.e.row) + flat / a.group;
+      const int head = kh * a.group + flat % a.group;
+      const float by = 1.f / sum;
+      float o[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
+      if (a.gate != nullptr) {
+        const float* gate = a.gate + token * a.gate_token_stride + head * a.gate_head_stride + 4 * f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] *= SigmoidDev(gate[i]);
+        }
+      }
+      float* out = a.out + token * a.out_token_stride + head * a.out_head_stride + 4 * f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[i] *= SigmoidDev(gate[i]);
+        out[i] = sees > 0 ? o[i] : 0.f;
+      }
+    };
+    auto note = [&](int r, float most, float sum) {     // for the weights
+      if (a.finals != nullptr) {
+        const int flat = task.row0 + r;
+        const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
+        a.finals[2 * at] = most;
+        a.finals[2 * at + 1] = 1.f / sum;
+      }
+    };
+    const bool alone = from == unit_start && to == unit_start + tiles;
+    // A block's part of a unit that it shares: the first one of its stretch, or the last.
+    const auto part_of = [&](long long block, bool opens) { return (block * 2 + (opens ? 0 : 1)) * 8 * RT; };
+    const size_t part = part_of(blockIdx.x, from == begin);
+    for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
+      const int r = at / fours, f = at % fours;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(join + (w * 8 * RT + r) * 64 * NS + 4 * f);
+        const float by = warp_top[w][r];
+        sum.x = fmaf(v.x, by, sum.x), sum.y = fmaf(v.y, by, sum.y), sum.z = fmaf(v.z, by, sum.z), sum.w = fmaf(v.w, by, sum.w);
+      }
+      if (alone) {
+        finish(r, f, sum, final_total[r], row_seen[r]);
+      } else {
+        __stcg(reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim) + f, sum);
       }
     }
-    float* to = a.out + token * a.out_token_stride + head * a.out_head_stride + 4 * f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      to[i] = sees > 0 ? o[i] : 0.f;
-    }
-  };
-  auto note = [&](int r, float most, float sum) {     // for the weights
-    if (a.finals != nullptr) {
-      const int flat = task.row0 + r;
-      const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
-      a.finals[2 * at] = most;
-      a.finals[2 * at + 1] = 1.f / sum;
-    }
-  };
-  for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
-    const int r = at / fours, f = at % fours;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(join + (w * 8 * RT + r) * 64 * NS + 4 * f);
-      const float by = warp_top[w][r];
-      sum.x = fmaf(v.x, by, sum.x), sum.y = fmaf(v.y, by, sum.y), sum.z = fmaf(v.z, by, sum.z), sum.w = fmaf(v.w, by, sum.w);
-    }
-    if (active == 1) {
-      finish(r, f, sum, final_total[r], row_seen[r]);
-    } else {
-      const size_t part = (static_cast<size_t>(item) * a.splits + split) * 8 * RT + r;
-      __stcg(reinterpret_cast<float4*>(a.sums + part * c.head_dim) + f, sum);
-    }
-  }
-  if (active == 1) {
-    if (threadIdx.x < task.rows) {
-      note(threadIdx.x, final_top[threadIdx.x], final_total[threadIdx.x]);
-    }
-    return;
-  }
-  if (threadIdx.x < 8 * RT) {
-    const size_t part = (static_cast<size_t>(item) * a.splits + split) * 8 * RT + threadIdx.x;
-    __stcg(reinterpret_cast<float2*>(a.stats) + part, make_float2(final_top[threadIdx.x], final_total[threadIdx.x]));
-  }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    is_last = atomicAdd(a.arrived + item, 1u) == static_cast<unsigned>(active - 1);
-  }
-  __syncthreads();
-  if (!is_last) {
-    return;
-  }
-  __threadfence();
-  if (threadIdx.x == 0) {
-    a.arrived[item] = 0;
-  }
-  // ---- the splits' parts together: their factors in shared memory, then the sums
-  float* by = reinterpret_cast<float*>(raw);     // [row][splits]
-  const size_t parts = static_cast<size_t>(item) * a.splits * 8 * RT;
-  for (int r = warp; r < task.rows; r += kWarps) {
-    const float2* stats = reinterpret_cast<const float2*>(a.stats) + parts + r;
-    float most = -INFINITY;
-    for (int i = lane; i < active; i += 32) {
-      most = fmaxf(most, __ldcg(stats + static_cast<size_t>(i) * 8 * RT).x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-    }
-    float sum = 0.f;
-    for (int i = lane; i < active; i += 32) {
-      const float2 s = __ldcg(stats + static_cast<size_t>(i) * 8 * RT);
-      const float f = most == -INFINITY ? 1.f : exp2f(s.x - most);
-      by[r * a.splits + i] = f;
-      sum += s.y * f;
-    }
-    sum = WarpSum(sum);
-    if (lane == 0) {
-      final_total[r] = sum;
-      note(r, most, sum);
-    }
-  }
-  __syncthreads();
-  for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
-    const int r = at / fours, f = at % fours;
-    const float4* from = reinterpret_cast<const float4*>(a.sums + (parts + r) * c.head_dim) + f;
-    const size_t stride = static_cast<size_t>(8 * RT) * fours;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < active; i0 += 8) {
-      float4 v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = i0 + i < active ? __ldcg(from + (i0 + i) * stride) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (alone) {
+      if (threadIdx.x < task.rows) {
+        note(threadIdx.x, final_top[threadIdx.x], final_total[threadIdx.x]);
       }
+      from = to;
+      __syncthreads();     // before the shared memory's next use
+      continue;
+    }
+    if (threadIdx.x < 8 * RT) {
+      __stcg(reinterpret_cast<float2*>(a.stats) + part + threadIdx.x, make_float2(final_top[threadIdx.x], final_total[threadIdx.x]));
+    }
+    const int first_block = owner_of(unit_start), count = owner_of(unit_start + tiles - 1) - first_block + 1;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      is_last = atomicAdd(a.arrived + first_block, 1u) == static_cast<unsigned>(count - 1);
+    }
+    __syncthreads();
+    if (is_last) {
+      __threadfence();
+      if (threadIdx.x == 0) {
+        a.arrived[first_block] = 0;
+      }
+      // ---- the blocks' parts together: their factors in shared memory, then the sums
+      float* by = reinterpret_cast<float*>(raw);     // [row][count]
+      const bool opens = start_of(first_block) == unit_start;     // for the first of them this unit is its first
+      const auto part_at = [&](int i) { return static_cast<size_t>(part_of(first_block + i, i > 0 || opens)); };
+      for (int r = warp; r < task.rows; r += kWarps) {
+        const float2* stats = reinterpret_cast<const float2*>(a.stats) + r;
+        float most = -INFINITY;
+        for (int i = lane; i < count; i += 32) {
+          most = fmaxf(most, __ldcg(stats + part_at(i)).x);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f2 = i0 + i < active ? by[r * a.splits + i0 + i] : 0.f;
-        sum.x = fmaf(v[i].x, f2, sum.x), sum.y = fmaf(v[i].y, f2, sum.y), sum.z = fmaf(v[i].z, f2, sum.z), sum.w = fmaf(v[i].w, f2, sum.w);
+        for (int o = 16; o > 0; o >>= 1) {
+          most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+        }
+        float sum = 0.f;
+        for (int i = lane; i < count; i += 32) {
+          const float2 s = __ldcg(stats + part_at(i));
+          const float f = most == -INFINITY ? 1.f : exp2f(s.x - most);
+          by[r * count + i] = f;
+          sum += s.y * f;
+        }
+        sum = WarpSum(sum);
+        if (lane == 0) {
+          final_total[r] = sum;
+          note(r, most, sum);
+        }
+      }
+      __syncthreads();
+      for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
+        const int r = at / fours, f = at % fours;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < count; i0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = i0 + i < count ? __ldcg(reinterpret_cast<const float4*>(a.sums + (part_at(i0 + i) + r) * c.head_dim) + f)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f2 = i0 + i < count ? by[r * count + i0 + i] : 0.f;
+            sum.x = fmaf(v[i].x, f2, sum.x), sum.y = fmaf(v[i].y, f2, sum.y), sum.z = fmaf(v[i].z, f2, sum.z), sum.w = fmaf(v[i].w, f2, sum.w);
+          }
+        }
+        finish(r, f, sum, final_total[r], row_seen[r]);
       }
     }
-    finish(r, f, sum, final_total[r], row_seen[r]);
+    from = to;
+    __syncthreads();     // before the shared memory's next use
   }
 }
 
@@ -614,61 +732,38 @@ WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batc
   GridDependencyWait();
   const CacheView& c = a.cache;
   const int kh = blockIdx.y;
-  Task task;
-  task.e = batch.of[blockIdx.z];
-  task.position = batch.positions[task.e.index];
+  const BatchEntry& e = batch.of[blockIdx.z];
+  const int position = batch.positions[e.index];
   int length = 0;
-  for (int token = 0; token < task.e.tokens; ++token) {
-    length = max(length, SeenBy(a, task, token));
+  for (int token = 0; token < e.tokens; ++token) {
+    length = max(length, SeenBy(a, e, position, token));
   }
   const int row = blockIdx.x * kThreads + threadIdx.x;
   if (row >= length) {
     return;
   }
   float sum = 0.f;
-  for (int token = 0; token < task.e.tokens; ++token) {
-    if (row >= SeenBy(a, task, token)) {
+  for (int token = 0; token < e.tokens; ++token) {
+    if (row >= SeenBy(a, e, position, token)) {
       continue;
     }
-    const int64_t first = (static_cast<int64_t>(task.e.row) + token) * a.heads + kh * a.group;
+    const int64_t first = (static_cast<int64_t>(e.row) + token) * a.heads + kh * a.group;
     for (int h = 0; h < a.group; ++h) {
       const float2 f = reinterpret_cast<const float2*>(a.finals)[first + h];
       sum += exp2f(__ldcs(a.scores + (first + h) * c.capacity + row) - f.x) * f.y;
     }
   }
-  c.weights[(static_cast<size_t>(task.e.slot) * c.kv_heads + kh) * c.capacity + row] += sum;
+  c.weights[(static_cast<size_t>(e.slot) * c.kv_heads + kh) * c.capacity + row] += sum;
 }
 
-// Splits of an item, and blocks of threads of a launch whose items are split at all.
-constexpr int kMostSplits = 256;
-constexpr int kMostBlocks = 2048;
-constexpr size_t kArrivedBytes = kMostBlocks * sizeof(unsigned);
-constexpr int kMostRows = 32;         // query rows of an item
-
-size_t PartialBytes() {
-  // An item's rows times dimensions: 8 rt * 64 ns with rt * ns <= 8, and two statistics a row.
-  return static_cast<size_t>(kMostBlocks) * (8 * 64 * 8 + 2 * kMostRows) * sizeof(float);
-}
-
-// How a launch of `all` (item, KV head) pairs is split. Few pairs: the blocks that the device
-// holds at once are shared out, a tile a warp at least. More: sequences of different lengths
-// have to even out, in parts of 512 rows at least.
-void Split(int64_t all, int slots, int capacity, int* splits, int* least_tiles) {
-  int64_t n = 1;
-  if (2 * all <= slots) {
-    n = slots / all;
-    *least_tiles = kWarps;
-  } else {
-    n = capacity / 512;
-    *least_tiles = 512 / kTile;
-  }
-  n = n > kMostSplits ? kMostSplits : n;
-  n = n * all > kMostBlocks ? kMostBlocks / all : n;
-  *splits = n < 1 ? 1 : static_cast<int>(n);
-}
+// Scratch of the blocks that a device holds at once: a counter each; two units' rows times
+// dimensions, 8 rt * 64 ns with rt * ns <= 8 where an SM holds one block and <= 2 where it holds
+// two, and two statistics a row.
+size_t ArrivedBytes(int sms) { return (static_cast<size_t>(2 * sms) * sizeof(unsigned) + 255) / 256 * 256; }
+size_t PartialBytes(int sms) { return static_cast<size_t>(2 * sms) * (8 * 64 * 8 + 2 * 32) * sizeof(float); }
 
 template <typename Format, int NS, int RT>
-int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int items) {
+int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b) {
   using S = Shape<NS, RT>;
   static std::atomic<bool> configured[64];
   if (ctx->device >= 64 || !configured[ctx->device].load()) {
@@ -677,23 +772,23 @@ int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, in
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(a.splits, a.cache.kv_heads, items), dim3(kThreads), S::kBytes,
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(ctx->sm_count * S::kBlocks), dim3(kThreads), S::kBytes,
                                  ctx->stream, 1, a, b));
   ctx->launches.fetch_add(1);
   return GUFO_CUDA_OK;
 }
 
 template <typename Format>
-int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int items, int ns, int rt) {
+int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int ns, int rt) {
   switch (ns * 8 + rt) {
-    case 8 + 1: return LaunchAttend<Format, 1, 1>(ctx, a, b, items);
-    case 8 + 2: return LaunchAttend<Format, 1, 2>(ctx, a, b, items);
-    case 8 + 4: return LaunchAttend<Format, 1, 4>(ctx, a, b, items);
-    case 16 + 1: return LaunchAttend<Format, 2, 1>(ctx, a, b, items);
-    case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b, items);
-    case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b, items);
-    case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b, items);
-    default: return LaunchAttend<Format, 4, 2>(ctx, a, b, items);
+    case 8 + 1: return LaunchAttend<Format, 1, 1>(ctx, a, b);
+    case 8 + 2: return LaunchAttend<Format, 1, 2>(ctx, a, b);
+    case 8 + 4: return LaunchAttend<Format, 1, 4>(ctx, a, b);
+    case 16 + 1: return LaunchAttend<Format, 2, 1>(ctx, a, b);
+    case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b);
+    case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b);
+    case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b);
+    default: return LaunchAttend<Format, 4, 2>(ctx, a, b);
   }
 }
 
@@ -721,7 +816,7 @@ int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle,
   if (accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / cache->c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend_scratch: too many query rows for one call");
   }
-  *bytes = gufo::kArrivedBytes + gufo::PartialBytes() + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
+  *bytes = gufo::ArrivedBytes(ctx->sm_count) + gufo::PartialBytes(ctx->sm_count) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
   return GUFO_CUDA_OK;
 }
 
@@ -754,7 +849,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_attend: null pointer");
   }
   const size_t rows = static_cast<size_t>(p->heads) * tokens;
-  const size_t own = gufo::kArrivedBytes + gufo::PartialBytes();
+  const size_t own = gufo::ArrivedBytes(ctx->sm_count) + gufo::PartialBytes(ctx->sm_count);
   if (p->accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
   }
@@ -780,7 +875,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   a.whole = reinterpret_cast<uintptr_t>(p->queries) % 16 == 0 && ((p->query_token_stride | p->query_head_stride) & 3) == 0;
   uint8_t* scratch = static_cast<uint8_t*>(p->scratch);
   a.arrived = reinterpret_cast<unsigned*>(scratch);
-  a.sums = reinterpret_cast<float*>(scratch + gufo::kArrivedBytes);
+  a.sums = reinterpret_cast<float*>(scratch + gufo::ArrivedBytes(ctx->sm_count));
   if (p->accumulate != 0) {
     a.finals = reinterpret_cast<float*>(scratch + own);
     a.scores = a.finals + 2 * rows;
@@ -794,6 +889,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
     most = n > most ? n : most;
   }
   const int64_t rows_each = static_cast<int64_t>(most) * a.group;
+  a.stats = a.sums + static_cast<size_t>(2 * ctx->sm_count) * 8 * 64 * 8;
   const int rt = rows_each <= 8 ? 1 : rows_each <= 16 || ns == 4 ? 2 : 4;
   if (tokens * a.group / (8 * rt) + batch->sequences > 65535) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
@@ -802,19 +898,15 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   const int group = a.group;
   return gufo::ForEachRun(
       *batch, [&](int n) { return static_cast<int>((static_cast<int64_t>(n) * group + 8 * rt - 1) / (8 * rt)); },
-      [&](const gufo::BatchArgs& b, int items) -> int {
-        const int64_t all = static_cast<int64_t>(items) * c.kv_heads;
-        gufo::AttendArgs of = a;
-        gufo::Split(all, ctx->sm_count * (ns * rt >= 4 ? 1 : 2), c.capacity, &of.splits, &of.least_tiles);
-        of.stats = of.sums + static_cast<size_t>(all) * of.splits * 8 * rt * c.head_dim;
-        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, of, b, items, ns, rt)
-                                                          : gufo::PickAttend<gufo::Int8>(ctx, of, b, items, ns, rt);
-        if (run != GUFO_CUDA_OK || of.scores == nullptr) {
+      [&](const gufo::BatchArgs& b, int) -> int {
+        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, ns, rt)
+                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, ns, rt);
+        if (run != GUFO_CUDA_OK || a.scores == nullptr) {
           return run;
         }
         GUFO_CUDA_TRY(gufo::LaunchOverlapped(gufo::WeightsKernel,
                                              dim3((c.capacity + gufo::kThreads - 1) / gufo::kThreads, c.kv_heads, b.sequences),
-                                             dim3(gufo::kThreads), 0, ctx->stream, 1, of, b));
+                                             dim3(gufo::kThreads), 0, ctx->stream, 1, a, b));
         ctx->launches.fetch_add(1);
         return GUFO_CUDA_OK;
       });
