@@ -4,11 +4,14 @@
 // the contexts that is all the time there is, if loads are never waited for and the arithmetic
 // stays hidden under them. Short contexts are bound by latency.
 //
-// The arithmetic. Warps are on their own: each streams tiles of 16 rows (one block of the cache:
-// one scale for the keys, one for the values) through a ring of its own in shared memory
-// (cp.async, nothing to meet at), and keeps its own running maximum, sum and weighted rows. The
-// cache rows are the A operand of mma.sync m16n8k16, eight query rows (tokens times the query
-// heads of the KV head) the B operand:
+// The arithmetic. A group of one, two or four warps (64 dimensions each) goes through tiles of
+// as many blocks of the cache (16 rows, one scale for the keys, one for the values), streamed
+// through rings in shared memory (cp.async). For each block one warp takes the scores, over all
+// dimensions; its weights then go to the group's warps, each of which adds up its 64 dimensions
+// of the group's blocks. So nothing is decoded twice, a warp's sums take 16 registers for eight
+// query rows whatever the head's size, and the group meets once a tile.
+// The cache rows are the A operand of mma.sync m16n8k16, eight query rows (tokens times the
+// query heads of the KV head) the B operand:
 //   S^T = K Q^T   [16 rows x 8 queries],     O^T = V^T P^T   [16 dimensions x 8 queries]
 // Codes become fp16 exactly, in registers. The fp32 operands (queries; probabilities) go in as
 // two fp16 halves, 22 bits of them, scaled by a power of two first so that small ones keep
@@ -17,6 +20,8 @@
 // in; P^T is turned into a B operand by movmatrix. A lane's dimensions are permuted (16 bytes
 // of a key row, 8 of a value row are its own), which a sum over all of them does not see and
 // the output undoes.
+// A block's weights are taken against the maximum that the group knew, or the block's own where
+// that is larger; only then, and with the first tiles, is anything rescaled.
 //
 // The split. A unit of work is (sequence, group of query rows, KV head) with all the tiles
 // that the sequence is long. The device's resident blocks of threads share out the tiles of all
@@ -36,9 +41,13 @@
 namespace gufo {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = 8;
-constexpr int kTile = kCacheBlock;
+constexpr int kThreads = 128;
+constexpr int kWarps = 4;
+constexpr int kTile = kWarps * kCacheBlock;   // rows that a block of threads takes at a time
+// What a unit costs besides its tiles (queries, the join), and the least that a block gets, in tiles.
+constexpr int kUnitCost = 4;
+constexpr int kLeastCost = 4;
+constexpr int kMostSms = 160;                 // whose blocks a call uses
 constexpr float kProbScale = 32768.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -61,19 +70,24 @@ struct AttendArgs {
   float* finals;           // [query rows][2]: maximum, 1 / sum
 };
 
-// NS: segments of 64 dimensions (1, 2, 4); RT: groups of eight query rows.
+// NS: segments of 64 dimensions (1, 2, 4), warps of a group; RT: groups of eight query rows.
 template <int NS, int RT>
 struct Shape {
+  static constexpr int kGroups = kWarps / NS;
   static constexpr int kRowBytes = 64 * NS;
-  static constexpr int kSide = kTile * kRowBytes;           // a tile's keys
-  static constexpr int kStage = 2 * kSide + 16;             // keys, values, the two scales
-  static constexpr int kBlocks = NS * RT >= 4 ? 1 : 2;      // of threads that an SM holds
-  static constexpr int kStages = NS == 4 ? 3 : NS * RT >= 4 ? 6 : NS == 2 ? 3 : 6;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kJoin = kWarps * 8 * RT * kRowBytes * 4;
-  static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kItem = kCacheBlock * kRowBytes;     // a block's keys or values
+  static constexpr int kSlot = kItem + 16;                  // and their scale
+  static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
+  static constexpr int kRing = kWarps * kSlots * kSlot;
+  static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
+  // Of threads that an SM holds: by registers (RT == 4: 168 a thread), or by shared memory.
+  static constexpr int kBlocks = RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
+  static constexpr int kParts = 8 * RT * kBlocks * kMostSms * 4;   // factors of a unit's parts
+  static constexpr int kLarger = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kShared = kLarger > kParts ? kLarger : kParts;
   static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order
-  static constexpr int kBytes = kShared + kQuery;
+  static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
+  static constexpr int kBytes = kShared + kQuery + kWeights;
 };
 
 __device__ __forceinline__ uint32_t SharedAt(const void* p) {
@@ -82,8 +96,17 @@ __device__ __forceinline__ uint32_t SharedAt(const void* p) {
 __device__ __forceinline__ void Copy16(uint32_t to, const void* from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void Copy4(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+__device__ __forceinline__ void Copy4(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+// The warps of a group meet.
+template <int NS>
+__device__ __forceinline__ void Meet(int group) {
+  if constexpr (NS == 1) {
+    __syncwarp();
+  } else {
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * NS) : "memory");
+  }
 }
 // d = a b_low + a b_high: thirty-two products, added by the instruction.
 __device__ __forceinline__ void MmaHalves(float (&d)[4], const uint32_t (&a)[4], uint32_t high0, uint32_t high1, uint32_t low0,
@@ -117,7 +140,7 @@ __device__ __forceinline__ int SeenBy(const AttendArgs& a, const BatchEntry& e, 
 }
 
 // Tiles of each sequence in `tiles` (one at least: a row that sees nothing is an output too) and
-// of the units of all sequences ahead of it in `ahead` ([sequences + 1]).
+// the cost of the units of all sequences ahead of it in `ahead` ([sequences + 1]).
 __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int* tiles, long long* ahead) {
   __shared__ long long of_warp[kBatchSequences / 32];
   const int n = batch.sequences, i = threadIdx.x, warp = i >> 5, lane = i & 31;
@@ -143,7 +166,7 @@ __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& b
     long long mine = 0;
     if (i < n) {
       tiles[i] = max(1, (tiles[i] + kTile - 1) / kTile);
-      mine = static_cast<long long>(batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * tiles[i];
+      mine = static_cast<long long>(batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * (tiles[i] + kUnitCost);
     }
     sum = mine;
 #pragma unroll
@@ -176,27 +199,29 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores
   __shared__ int row_seen[8 * RT];
-  __shared__ float warp_top[kWarps][8 * RT], warp_total[kWarps][8 * RT];
-  __shared__ float final_top[8 * RT], final_total[8 * RT];
+  __shared__ __align__(8) float block_top[2][kWarps][8 * RT];    // what a block's weights are taken against
+  __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT];
+  __shared__ float final_total[8 * RT];
   __shared__ int tiles_of[kBatchSequences];
-  __shared__ long long tiles_ahead[kBatchSequences + 1];
+  __shared__ long long cost_ahead[kBatchSequences + 1];
   __shared__ int is_last;
   GridLaunchDependents();
   GridDependencyWait();
   const CacheView& c = a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = warp / NS, member = warp % NS;
   const int g = lane >> 2, t = lane & 3;
-  ShareOut(a, batch, tiles_of, tiles_ahead);
-  const long long all = tiles_ahead[batch.sequences];
-  // A tile a warp at least.
-  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all / kWarps, 1ll)));
+  ShareOut(a, batch, tiles_of, cost_ahead);
+  const long long all = cost_ahead[batch.sequences];
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all / kLeastCost, 1ll)));
   if (blockIdx.x >= blocks) {
     return;
   }
+  // A unit's cost comes ahead of its tiles: a block whose stretch ends within it has no part of the unit.
   const auto start_of = [&](long long block) { return all * block / blocks; };
-  const auto owner_of = [&](long long tile) {     // the block whose stretch it is in
-    int b = static_cast<int>(tile * blocks / all);
-    while (start_of(b + 1) <= tile) {
+  const auto owner_of = [&](long long at) {     // the block whose stretch it is in
+    int b = static_cast<int>(at * blocks / all);
+    while (start_of(b + 1) <= at) {
       ++b;
     }
     return b;
@@ -215,26 +240,33 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       return (r * kPieces + (piece ^ (2 * (r >> 1 & 3)))) * 16;
     }
   };
-  uint8_t* ring = raw + warp * (S::kStages * S::kStage);
-  uint4* query = reinterpret_cast<uint4*>(raw + S::kShared);   // [rt][seg * 4 + j][lane]: high pair, pair, low pair, pair
+  const auto ring_of = [&](int w) { return raw + w * (S::kSlots * S::kSlot); };
+  uint8_t* const ring = ring_of(warp);
+  uint4* const query = reinterpret_cast<uint4*>(raw + S::kShared);   // [rt][seg * 4 + j][lane]: high pair, pair, low pair, pair
+  uint4* const shared_p = reinterpret_cast<uint4*>(raw + S::kShared + S::kQuery);   // [2][warp][rt][lane]
 
 #pragma unroll 1
   for (long long from = begin; from < end;) {
-    // ---- the unit that this tile is of
+    // ---- the unit that this is of
     int low = 0, high = batch.sequences - 1;
     while (low < high) {
       const int mid = (low + high + 1) / 2;
-      if (tiles_ahead[mid] <= from) {
+      if (cost_ahead[mid] <= from) {
         low = mid;
       } else {
         high = mid - 1;
       }
     }
     const int tiles = tiles_of[low];
-    const long long unit = (from - tiles_ahead[low]) / tiles;
-    const long long unit_start = tiles_ahead[low] + unit * tiles;
+    const long long unit = (from - cost_ahead[low]) / (tiles + kUnitCost);
+    const long long unit_start = cost_ahead[low] + unit * (tiles + kUnitCost) + kUnitCost;   // of its tiles
+    const int first_tile = static_cast<int>(max(from - unit_start, 0ll));
+    const int last_tile = static_cast<int>(min(end - unit_start, static_cast<long long>(tiles)));
+    from = unit_start + tiles;
+    if (last_tile <= first_tile) {
+      continue;
+    }
     const int kh = static_cast<int>(unit % c.kv_heads);
-    const long long to = min(end, unit_start + tiles);
     Task task;
     task.e = batch.of[low];
     task.row0 = static_cast<int>(unit / c.kv_heads) * 8 * RT;
@@ -252,57 +284,59 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       least = min(least, row_seen[r]);
     }
     // (These rows may see less than the sequence's last ones.)
-    const int first_tile = static_cast<int>(from - unit_start);
-    const int end_tile = min(static_cast<int>(to - unit_start), (length + kTile - 1) / kTile);
+    const int end_tile = min(last_tile, (length + kTile - 1) / kTile);
     const size_t of_head = static_cast<size_t>(task.e.slot) * c.kv_heads + kh;
-    const uint8_t* keys = c.codes[0] + of_head * c.capacity * c.head_dim;
-    const uint8_t* values = c.codes[1] + of_head * c.capacity * c.head_dim;
-    const float* scale_from = c.scales[lane & 1] + of_head * (c.capacity / kTile);   // lane 0: keys, 1: values
 
-    // ---- the ring
-    const int whole_tiles = c.head_dim == S::kRowBytes ? length / kTile : 0;   // that can be copied as they are
-    auto load = [&](int tile, int stage) {
-      if (tile < end_tile) {
-        const uint32_t to_keys = SharedAt(ring + stage * S::kStage), to_values = to_keys + S::kSide;
+    // ---- the ring: a warp copies its block of every tile, keys and values in turn
+    const int whole_blocks = c.head_dim == S::kRowBytes ? length / kCacheBlock : 0;   // that can be copied as they are
+    int next_tile = first_tile, next_side = 0, next_slot = 0;
+    auto load = [&]() {
+      if (next_tile < end_tile) {
+        const int block = next_tile * kWarps + warp;
+        const uint32_t to = SharedAt(ring + next_slot * S::kSlot);
+        const uint8_t* codes = c.codes[next_side] + of_head * c.capacity * c.head_dim;
         constexpr int kEach = 32 / kPieces;     // rows that the lanes copy at a time
         const int r0 = lane / kPieces, piece = lane % kPieces;
-        if (tile < whole_tiles) {
-          const uint8_t* k = keys + static_cast<size_t>(tile) * S::kSide + lane * 16;
-          const uint8_t* v = values + static_cast<size_t>(tile) * S::kSide + lane * 16;
+        if (block < whole_blocks) {
+          const uint8_t* k = codes + static_cast<size_t>(block) * S::kItem + lane * 16;
+          if (next_side == 0) {
 #pragma unroll
-          for (int i = 0; i < kTile / kEach; ++i) {
-            Copy16(to_keys + key_at(r0, piece) + 512 * i, k + 512 * i, true);
-          }
+            for (int i = 0; i < kCacheBlock / kEach; ++i) {
+              Copy16(to + key_at(r0, piece) + 512 * i, k + 512 * i, true);
+            }
+          } else {
 #pragma unroll
-          for (int i = 0; i < kTile / kEach; ++i) {
-            Copy16(to_values + value_at(r0 + kEach * i, piece), v + 512 * i, true);
+            for (int i = 0; i < kCacheBlock / kEach; ++i) {
+              Copy16(to + value_at(r0 + kEach * i, piece), k + 512 * i, true);
+            }
           }
         } else {
 #pragma unroll 1
-          for (int i = 0; i < kTile / kEach; ++i) {
+          for (int i = 0; i < kCacheBlock / kEach; ++i) {
             const int r = r0 + kEach * i;
-            const bool there = tile * kTile + r < length && piece * 16 < c.head_dim;
-            const size_t at = there ? (static_cast<size_t>(tile) * kTile + r) * c.head_dim + piece * 16 : 0;
-            Copy16(to_keys + key_at(r, piece), keys + at, there);
-            Copy16(to_values + value_at(r, piece), values + at, there);
+            const bool there = block * kCacheBlock + r < length && piece * 16 < c.head_dim;
+            const size_t at = there ? (static_cast<size_t>(block) * kCacheBlock + r) * c.head_dim + piece * 16 : 0;
+            Copy16(to + (next_side == 0 ? key_at(r, piece) : value_at(r, piece)), codes + at, there);
           }
         }
-        if (lane < 2) {
-          Copy4(to_keys + 2 * S::kSide + 4 * lane, scale_from + tile);
+        if (lane == 0) {
+          const bool there = block * kCacheBlock < length;
+          Copy4(to + S::kItem, c.scales[next_side] + of_head * (c.capacity / kCacheBlock) + (there ? block : 0), there);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
+      next_tile += next_side;
+      next_side ^= 1;
+      next_slot = next_slot + 1 == S::kSlots ? 0 : next_slot + 1;
     };
-    const int my_first = first_tile + warp;
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) {
-      load(my_first + i * kWarps, i);
+    for (int i = 0; i < S::kSlots - 1; ++i) {
+      load();
     }
 
-    // ---- the queries: row 8 rt + w to warp w, in the order of the B operands
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = 8 * rt + warp;
+    // ---- the queries: every fourth row to a warp, in the order of the B operands
+#pragma unroll 1
+    for (int r = warp; r < 8 * RT; r += kWarps) {
       const bool there = r < task.rows;
       const int flat = task.row0 + (there ? r : 0);
       const int token = flat / a.group, head = kh * a.group + flat % a.group;
@@ -340,7 +374,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             high[k] = __float2half_rn(v[k]);
             low[k] = __float2half_rn(v[k] - __half2float(high[k]));
           }
-          query[(rt * 4 * NS + seg * 4 + j) * 32 + warp * 4 + of] = make_uint4(
+          query[(r / 8 * 4 * NS + seg * 4 + j) * 32 + r % 8 * 4 + of] = make_uint4(
               PackHalves(high[0], high[1]), PackHalves(high[2], high[3]), PackHalves(low[0], low[1]), PackHalves(low[2], low[3]));
         }
       }
@@ -353,8 +387,8 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     // ---- the tiles
     float factor[RT][2];
     int seen[RT][2];
-    float top[RT][2], total[RT][2];      // of query rows 8 rt + 2 t, + 1; the sum is this lane's rows' part
-    float acc[RT][4 * NS][4];
+    float top[RT][2], total[RT][2];      // of query rows 8 rt + 2 t, + 1: the group's maximum, the sum of this lane's rows
+    float acc[RT][4][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -365,22 +399,21 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         total[rt][i] = 0.f;
       }
 #pragma unroll
-      for (int m = 0; m < 4 * NS; ++m) {
+      for (int m = 0; m < 4; ++m) {
         acc[rt][m][0] = acc[rt][m][1] = acc[rt][m][2] = acc[rt][m][3] = 0.f;
       }
     }
     // RA: groups of eight rows that there are.
     const auto go = [&](auto groups) {
       constexpr int RA = decltype(groups)::value;
-      int stage = 0;
+      int slot = 0, parity = 0;
 #pragma unroll 1
-      for (int tile = my_first; tile < end_tile; tile += kWarps) {
-        load(tile + (S::kStages - 1) * kWarps, stage == 0 ? S::kStages - 1 : stage - 1);
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+      for (int tile = first_tile; tile < end_tile; ++tile) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 2) : "memory");
         __syncwarp();
-        uint8_t* here = ring + stage * S::kStage;
-        const float2 scales = *reinterpret_cast<const float2*>(here + 2 * S::kSide);
-        // Scores.
+        // Scores of this warp's block.
+        const uint8_t* keys = ring + slot * S::kSlot;
+        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
         float s[RA][4];
 #pragma unroll
         for (int rt = 0; rt < RA; ++rt) {
@@ -388,8 +421,8 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         }
 #pragma unroll
         for (int seg = 0; seg < NS; ++seg) {
-          const uint4 k0 = *reinterpret_cast<const uint4*>(here + key_at(g, 4 * seg + t));
-          const uint4 k1 = *reinterpret_cast<const uint4*>(here + key_at(g + 8, 4 * seg + t));
+          const uint4 k0 = *reinterpret_cast<const uint4*>(keys + key_at(g, 4 * seg + t));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(keys + key_at(g + 8, 4 * seg + t));
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -405,14 +438,17 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             }
           }
         }
-        const int r0 = tile * kTile + g;
+        const float key_scale = *reinterpret_cast<const float*>(keys + S::kItem);
+        const int r0 = (tile * kWarps + warp) * kCacheBlock + g;
         const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
-        uint32_t p[RA][4];       // high pair of rows 0-7, of 8-15; low pairs
+        uint4 p[RA];             // high pair of rows 0-7, of 8-15; low pairs
+        float sum[RA][2];        // of this lane's weights
+        float own[RA][2];        // what they are taken against
 #pragma unroll
         for (int rt = 0; rt < RA; ++rt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[rt][i] *= factor[rt][i & 1] * scales.x;
+            s[rt][i] *= factor[rt][i & 1] * key_scale;
           }
           if (a.scores != nullptr) {
 #pragma unroll
@@ -431,26 +467,24 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
               s[rt][i] = r0 + 8 * (i >> 1) < seen[rt][i & 1] ? s[rt][i] : -INFINITY;
             }
           }
-          const float m0 = fmaxf(s[rt][0], s[rt][2]), m1 = fmaxf(s[rt][1], s[rt][3]);
+          float m0 = fmaxf(fmaxf(s[rt][0], s[rt][2]), top[rt][0]), m1 = fmaxf(fmaxf(s[rt][1], s[rt][3]), top[rt][1]);
           if (__any_sync(0xFFFFFFFFu, m0 > top[rt][0] || m1 > top[rt][1])) {
-            float n0 = fmaxf(m0, top[rt][0]), n1 = fmaxf(m1, top[rt][1]);
 #pragma unroll
             for (int o = 4; o <= 16; o <<= 1) {
-              n0 = fmaxf(n0, __shfl_xor_sync(0xFFFFFFFFu, n0, o));
-              n1 = fmaxf(n1, __shfl_xor_sync(0xFFFFFFFFu, n1, o));
-            }
-            const float keep0 = n0 == -INFINITY ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == -INFINITY ? 1.f : exp2f(top[rt][1] - n1);
-            top[rt][0] = n0, top[rt][1] = n1;
-            total[rt][0] *= keep0, total[rt][1] *= keep1;
-#pragma unroll
-            for (int m = 0; m < 4 * NS; ++m) {
-              acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
+              m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
+              m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
             }
           }
-          const float t0 = top[rt][0] == -INFINITY ? 0.f : top[rt][0], t1 = top[rt][1] == -INFINITY ? 0.f : top[rt][1];
+          own[rt][0] = m0, own[rt][1] = m1;
+          if constexpr (NS > 1) {
+            if (g == 0) {
+              *reinterpret_cast<float2*>(&block_top[parity][warp][8 * rt + 2 * t]) = make_float2(m0, m1);
+            }
+          }
+          const float t0 = m0 == -INFINITY ? 0.f : m0, t1 = m1 == -INFINITY ? 0.f : m1;
           const float e0 = exp2f(s[rt][0] - t0), e1 = exp2f(s[rt][1] - t1), e2 = exp2f(s[rt][2] - t0), e3 = exp2f(s[rt][3] - t1);
-          total[rt][0] += e0 + e2;
-          total[rt][1] += e1 + e3;
+          sum[rt][0] = e0 + e2;
+          sum[rt][1] = e1 + e3;
           const float x[4] = {e0 * kProbScale, e1 * kProbScale, e2 * kProbScale, e3 * kProbScale};
           __half high[4], low[4];
 #pragma unroll
@@ -458,85 +492,137 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             high[i] = __float2half_rn(x[i]);
             low[i] = __float2half_rn(x[i] - __half2float(high[i]));
           }
-          p[rt][0] = Transpose(PackHalves(high[0], high[1]));
-          p[rt][1] = Transpose(PackHalves(high[2], high[3]));
-          p[rt][2] = Transpose(PackHalves(low[0], low[1]));
-          p[rt][3] = Transpose(PackHalves(low[2], low[3]));
-        }
-        if constexpr (Format::kHasNan) {
-          // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
-          // others, whose weight of 0 times NaN would: where some do not see all rows of a tile, such
-          // values are put into the sums by hand and taken out of the tile.
-          if (hides) {
-            uint8_t* there = here + S::kSide;
-            const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
-            uint32_t found = 0;
-#pragma unroll 1
-            for (int i = 0; i < S::kSide / 16 / 32; ++i) {
-              const uint4 w = *reinterpret_cast<const uint4*>(there + 16 * (lane + 32 * i));
-              found |= marks(w.x) | marks(w.y) | marks(w.z) | marks(w.w);
-            }
-            if (__any_sync(0xFFFFFFFFu, found != 0)) {
-#pragma unroll
-              for (int m = 0; m < 4 * NS; ++m) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  const int dim = 64 * (m / 4) + 8 * g + 2 * (m % 4) + half;
-                  int rows = INT_MAX;      // the first with NaN
-#pragma unroll 1
-                  for (int r = kTile - 1; r >= 0; --r) {
-                    rows = (there[value_at(r, dim >> 4) + (dim & 15)] & 0x7F) == 0x7F ? tile * kTile + r : rows;
-                  }
-#pragma unroll
-                  for (int rt = 0; rt < RA; ++rt) {
-                    acc[rt][m][2 * half] = rows < seen[rt][0] ? NAN : acc[rt][m][2 * half];
-                    acc[rt][m][2 * half + 1] = rows < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
-                  }
-                }
-              }
-              __syncwarp();
-#pragma unroll 1
-              for (int i = 0; i < S::kSide / 4 / 32; ++i) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(there) + lane + 32 * i;
-                *w &= ~((marks(*w) >> 7) * 255u);
-              }
-              __syncwarp();
-            }
+          p[rt] = make_uint4(Transpose(PackHalves(high[0], high[1])), Transpose(PackHalves(high[2], high[3])),
+                             Transpose(PackHalves(low[0], low[1])), Transpose(PackHalves(low[2], low[3])));
+          if constexpr (NS > 1) {
+            shared_p[((parity * kWarps + warp) * RT + rt) * 32 + lane] = p[rt];
           }
         }
-        // Weighted rows.
-        const float by = scales.y * (1.f / kProbScale);
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 3) : "memory");
+        Meet<NS>(group);       // weights and values are there; the last tile's values and this one's keys are done with
+        load();
+        load();
+        // Where a block has raised the maximum: the sums to it.
+        bool raised = false;
 #pragma unroll
-        for (int seg = 0; seg < NS; ++seg) {
+        for (int rt = 0; rt < RA; ++rt) {
+          float n0 = own[rt][0], n1 = own[rt][1];
+          if constexpr (NS > 1) {
+#pragma unroll
+            for (int b = 0; b < NS; ++b) {
+              const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
+              n0 = fmaxf(n0, of.x), n1 = fmaxf(n1, of.y);
+            }
+          }
+          if (__any_sync(0xFFFFFFFFu, n0 > top[rt][0] || n1 > top[rt][1])) {
+            raised = true;
+            const float keep0 = n0 == top[rt][0] ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == top[rt][1] ? 1.f : exp2f(top[rt][1] - n1);
+            top[rt][0] = n0, top[rt][1] = n1;
+            const float mine0 = own[rt][0] == n0 ? 1.f : exp2f(own[rt][0] - n0), mine1 = own[rt][1] == n1 ? 1.f : exp2f(own[rt][1] - n1);
+            total[rt][0] = total[rt][0] * keep0 + sum[rt][0] * mine0;
+            total[rt][1] = total[rt][1] * keep1 + sum[rt][1] * mine1;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
+            }
+          } else {
+            total[rt][0] += sum[rt][0];
+            total[rt][1] += sum[rt][1];
+          }
+        }
+        // This warp's dimensions of the group's blocks.
+#pragma unroll
+        for (int b = 0; b < NS; ++b) {
+          uint8_t* values = ring_of(group * NS + b) + slot * S::kSlot;
+          if constexpr (Format::kHasNan) {
+            // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
+            // others, whose weight of 0 times NaN would: where some do not see all rows of a tile, such
+            // values are put into the sums by hand and taken out of the tile.
+            if (hides) {
+              const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
+              const auto word_at = [&](int i) {       // of this warp's dimensions: 16 rows of 16 words
+                const int r = i / 16, w = i % 16;
+                return reinterpret_cast<uint32_t*>(values + value_at(r, 4 * member + w / 4)) + w % 4;
+              };
+              uint32_t found = 0;
+#pragma unroll 1
+              for (int i = lane; i < 256; i += 32) {
+                found |= marks(*word_at(i));
+              }
+              if (__any_sync(0xFFFFFFFFu, found != 0)) {
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                  for (int half = 0; half < 2; ++half) {
+                    const int dim = 8 * g + 2 * m + half;
+                    int row = INT_MAX;      // the first with NaN
+#pragma unroll 1
+                    for (int r = kCacheBlock - 1; r >= 0; --r) {
+                      const uint8_t code = values[value_at(r, 4 * member + dim / 16) + dim % 16];
+                      row = (code & 0x7F) == 0x7F ? (tile * kWarps + group * NS + b) * kCacheBlock + r : row;
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RA; ++rt) {
+                      acc[rt][m][2 * half] = row < seen[rt][0] ? NAN : acc[rt][m][2 * half];
+                      acc[rt][m][2 * half + 1] = row < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
+                    }
+                  }
+                }
+                __syncwarp();
+#pragma unroll 1
+                for (int i = lane; i < 256; i += 32) {
+                  *word_at(i) &= ~((marks(*word_at(i)) >> 7) * 255u);
+                }
+                __syncwarp();
+              }
+            }
+          }
+          const float by = *reinterpret_cast<const float*>(values + S::kItem) * (1.f / kProbScale);
+          float each[RA][2];
+#pragma unroll
+          for (int rt = 0; rt < RA; ++rt) {
+            each[rt][0] = each[rt][1] = by;
+            if constexpr (NS > 1) {
+              p[rt] = shared_p[((parity * kWarps + group * NS + b) * RT + rt) * 32 + lane];
+              if (raised) {
+                const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
+                each[rt][0] *= of.x == top[rt][0] ? 1.f : exp2f(of.x - top[rt][0]);
+                each[rt][1] *= of.y == top[rt][1] ? 1.f : exp2f(of.y - top[rt][1]);
+              }
+            }
+          }
           uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-            v[i] = *reinterpret_cast<const uint2*>(here + S::kSide + value_at(r, 4 * seg + (g >> 1)) + 8 * (g & 1));
+            v[i] = *reinterpret_cast<const uint2*>(values + value_at(r, 4 * member + (g >> 1)) + 8 * (g & 1));
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t w0 = half ? v[0].y : v[0].x, w1 = half ? v[1].y : v[1].x, w2 = half ? v[2].y : v[2].x, w3 = half ? v[3].y : v[3].x;
 #pragma unroll
             for (int pair = 0; pair < 2; ++pair) {
-              uint32_t b[4];   // dimensions 2 pair, 2 pair + 1 of the word: rows beside one another
-              Format::Decode(__byte_perm(w0, w1, pair ? 0x7362 : 0x5140), b[0], b[1]);
-              Format::Decode(__byte_perm(w2, w3, pair ? 0x7362 : 0x5140), b[2], b[3]);
-              const int m = 4 * seg + 2 * half + pair;
+              uint32_t d_of[4];   // dimensions 2 pair, 2 pair + 1 of the word: rows beside one another
+              Format::Decode(__byte_perm(w0, w1, pair ? 0x7362 : 0x5140), d_of[0], d_of[1]);
+              Format::Decode(__byte_perm(w2, w3, pair ? 0x7362 : 0x5140), d_of[2], d_of[3]);
+              const int m = 2 * half + pair;
 #pragma unroll
               for (int rt = 0; rt < RA; ++rt) {
                 float d[4];
-                MmaHalves(d, b, p[rt][0], p[rt][1], p[rt][2], p[rt][3]);
+                MmaHalves(d, d_of, p[rt].x, p[rt].y, p[rt].z, p[rt].w);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  acc[rt][m][i] = fmaf(d[i], by, acc[rt][m][i]);
+                  acc[rt][m][i] = fmaf(d[i], each[rt][i & 1], acc[rt][m][i]);
                 }
               }
             }
           }
         }
-        __syncwarp();      // the stage is free
-        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+        parity ^= 1;
+        if constexpr (NS == 1) {
+          __syncwarp();
+        }
       }
     };
     if constexpr (RT == 1) {
@@ -550,7 +636,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 
-    // ---- the warps' parts together
+    // ---- the groups' parts together
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -561,47 +647,44 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         }
         if (g == 0) {
-          warp_top[warp][8 * rt + 2 * t + i] = top[rt][i];
+          if (member == 0) {
+            group_top[group][8 * rt + 2 * t + i] = top[rt][i];
+          }
           warp_total[warp][8 * rt + 2 * t + i] = sum;
         }
       }
     }
     __syncthreads();     // the rings are free
-    float* join = reinterpret_cast<float*>(raw);      // [warp][row][64 NS]
+    float* join = reinterpret_cast<float*>(raw);      // [group][row][64 NS]
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (8 * rt < task.rows) {
 #pragma unroll
-        for (int seg = 0; seg < NS; ++seg) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float* out = join + (warp * 8 * RT + 8 * rt + 2 * t + i) * 64 * NS + 64 * seg + 8 * g;
-            *reinterpret_cast<float4*>(out) = make_float4(acc[rt][4 * seg][i], acc[rt][4 * seg][i + 2], acc[rt][4 * seg + 1][i],
-                                                          acc[rt][4 * seg + 1][i + 2]);
-            *reinterpret_cast<float4*>(out + 4) = make_float4(acc[rt][4 * seg + 2][i], acc[rt][4 * seg + 2][i + 2],
-                                                              acc[rt][4 * seg + 3][i], acc[rt][4 * seg + 3][i + 2]);
-          }
+        for (int i = 0; i < 2; ++i) {
+          float* out = join + (group * 8 * RT + 8 * rt + 2 * t + i) * S::kRowBytes + 64 * member + 8 * g;
+          *reinterpret_cast<float4*>(out) = make_float4(acc[rt][0][i], acc[rt][0][i + 2], acc[rt][1][i], acc[rt][1][i + 2]);
+          *reinterpret_cast<float4*>(out + 4) = make_float4(acc[rt][2][i], acc[rt][2][i + 2], acc[rt][3][i], acc[rt][3][i + 2]);
         }
       }
     }
-    if (threadIdx.x < 8 * RT) {
-      const int r = threadIdx.x;
+    __syncthreads();
+    // A row's maximum and sum, and the factor of a group's part.
+    const auto factor_of = [&](int r, int of, float most) {
+      return group_top[of][r] == most ? 1.f : exp2f(group_top[of][r] - most);
+    };
+    const auto row_stats = [&](int r) {
       float most = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        most = fmaxf(most, warp_top[w][r]);
+      for (int of = 0; of < S::kGroups; ++of) {
+        most = fmaxf(most, group_top[of][r]);
       }
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float by = most == -INFINITY ? 1.f : exp2f(warp_top[w][r] - most);
-        sum += warp_total[w][r] * by;
-        warp_top[w][r] = by;      // from now on the factor of the warp's sums
+        sum += warp_total[w][r] * factor_of(r, w / NS, most);
       }
-      final_top[r] = most;
-      final_total[r] = sum;
-    }
-    __syncthreads();
+      return make_float2(most, sum);
+    };
     const int fours = c.head_dim / 4;
     // Four dimensions of a row of the output, gated; a row that saw nothing is zero.
     auto finish = [&](int r, int f, float4 v, float sum, int sees) {
@@ -631,35 +714,38 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         a.finals[2 * at + 1] = 1.f / sum;
       }
     };
-    const bool alone = from == unit_start && to == unit_start + tiles;
-    // A block's part of a unit that it shares: the first one of its stretch, or the last.
-    const auto part_of = [&](long long block, bool opens) { return (block * 2 + (opens ? 0 : 1)) * 8 * RT; };
-    const size_t part = part_of(blockIdx.x, from == begin);
+    const bool alone = first_tile == 0 && last_tile == tiles;
+    // A block's part of a unit that others have parts of too: of the one that it goes on with, or
+    // of the one that it begins.
+    const auto part_of = [&](int block, bool begins) { return (static_cast<size_t>(block) * 2 + (begins ? 1 : 0)) * 8 * RT; };
+    const size_t part = part_of(blockIdx.x, first_tile == 0);
     for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
       const int r = at / fours, f = at % fours;
+      const float2 stats = row_stats(r);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float4 v = *reinterpret_cast<const float4*>(join + (w * 8 * RT + r) * 64 * NS + 4 * f);
-        const float by = warp_top[w][r];
+      for (int of = 0; of < S::kGroups; ++of) {
+        const float4 v = *reinterpret_cast<const float4*>(join + (of * 8 * RT + r) * S::kRowBytes + 4 * f);
+        const float by = factor_of(r, of, stats.x);
         sum.x = fmaf(v.x, by, sum.x), sum.y = fmaf(v.y, by, sum.y), sum.z = fmaf(v.z, by, sum.z), sum.w = fmaf(v.w, by, sum.w);
       }
       if (alone) {
-        finish(r, f, sum, final_total[r], row_seen[r]);
+        finish(r, f, sum, stats.y, row_seen[r]);
       } else {
         __stcg(reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim) + f, sum);
       }
     }
-    if (alone) {
-      if (threadIdx.x < task.rows) {
-        note(threadIdx.x, final_top[threadIdx.x], final_total[threadIdx.x]);
+    if (threadIdx.x < task.rows) {
+      const float2 stats = row_stats(threadIdx.x);
+      if (alone) {
+        note(threadIdx.x, stats.x, stats.y);
+      } else {
+        __stcg(reinterpret_cast<float2*>(a.stats) + part + threadIdx.x, stats);
       }
-      from = to;
+    }
+    if (alone) {
       __syncthreads();     // before the shared memory's next use
       continue;
-    }
-    if (threadIdx.x < 8 * RT) {
-      __stcg(reinterpret_cast<float2*>(a.stats) + part + threadIdx.x, make_float2(final_top[threadIdx.x], final_total[threadIdx.x]));
     }
     const int first_block = owner_of(unit_start), count = owner_of(unit_start + tiles - 1) - first_block + 1;
     __threadfence();
@@ -675,8 +761,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
       // ---- the blocks' parts together: their factors in shared memory, then the sums
       float* by = reinterpret_cast<float*>(raw);     // [row][count]
-      const bool opens = start_of(first_block) == unit_start;     // for the first of them this unit is its first
-      const auto part_at = [&](int i) { return static_cast<size_t>(part_of(first_block + i, i > 0 || opens)); };
+      const auto part_at = [&](int i) { return part_of(first_block + i, i == 0); };
       for (int r = warp; r < task.rows; r += kWarps) {
         const float2* stats = reinterpret_cast<const float2*>(a.stats) + r;
         float most = -INFINITY;
@@ -690,7 +775,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         float sum = 0.f;
         for (int i = lane; i < count; i += 32) {
           const float2 s = __ldcg(stats + part_at(i));
-          const float f = most == -INFINITY ? 1.f : exp2f(s.x - most);
+          const float f = s.x == most ? 1.f : exp2f(s.x - most);
           by[r * count + i] = f;
           sum += s.y * f;
         }
@@ -720,7 +805,6 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         finish(r, f, sum, final_total[r], row_seen[r]);
       }
     }
-    from = to;
     __syncthreads();     // before the shared memory's next use
   }
 }
@@ -756,15 +840,20 @@ WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batc
   c.weights[(static_cast<size_t>(e.slot) * c.kv_heads + kh) * c.capacity + row] += sum;
 }
 
-// Scratch of the blocks that a device holds at once: a counter each; two units' rows times
-// dimensions, 8 rt * 64 ns with rt * ns <= 8 where an SM holds one block and <= 2 where it holds
-// two, and two statistics a row.
-size_t ArrivedBytes(int sms) { return (static_cast<size_t>(2 * sms) * sizeof(unsigned) + 255) / 256 * 256; }
-size_t PartialBytes(int sms) { return static_cast<size_t>(2 * sms) * (8 * 64 * 8 + 2 * 32) * sizeof(float); }
+// Scratch of the blocks of threads that a device holds at once, four an SM at most: a counter
+// each; two units' rows times dimensions, 8 rt * 64 ns with rt, ns <= 4 (two blocks an SM then; one
+// half as large has three or four), and two statistics a row.
+int Sms(const gufo_cuda_ctx* ctx) { return ctx->sm_count < kMostSms ? ctx->sm_count : kMostSms; }
+size_t ArrivedBytes(int sms) { return (static_cast<size_t>(4 * sms) * sizeof(unsigned) + 255) / 256 * 256; }
+constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
+constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
+size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * (kPartialFloats + kStatsFloats) * sizeof(float); }
 
 template <typename Format, int NS, int RT>
 int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b) {
   using S = Shape<NS, RT>;
+  static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
+                "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
   if (ctx->device >= 64 || !configured[ctx->device].load()) {
     GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
@@ -772,7 +861,7 @@ int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b) {
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(ctx->sm_count * S::kBlocks), dim3(kThreads), S::kBytes,
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(Sms(ctx) * S::kBlocks), dim3(kThreads), S::kBytes,
                                  ctx->stream, 1, a, b));
   ctx->launches.fetch_add(1);
   return GUFO_CUDA_OK;
@@ -788,7 +877,8 @@ int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int 
     case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b);
     case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b);
     case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b);
-    default: return LaunchAttend<Format, 4, 2>(ctx, a, b);
+    case 32 + 2: return LaunchAttend<Format, 4, 2>(ctx, a, b);
+    default: return LaunchAttend<Format, 4, 4>(ctx, a, b);
   }
 }
 
@@ -816,7 +906,7 @@ int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle,
   if (accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / cache->c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend_scratch: too many query rows for one call");
   }
-  *bytes = gufo::ArrivedBytes(ctx->sm_count) + gufo::PartialBytes(ctx->sm_count) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
+  *bytes = gufo::ArrivedBytes(gufo::Sms(ctx)) + gufo::PartialBytes(gufo::Sms(ctx)) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
   return GUFO_CUDA_OK;
 }
 
@@ -849,7 +939,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_attend: null pointer");
   }
   const size_t rows = static_cast<size_t>(p->heads) * tokens;
-  const size_t own = gufo::ArrivedBytes(ctx->sm_count) + gufo::PartialBytes(ctx->sm_count);
+  const size_t own = gufo::ArrivedBytes(gufo::Sms(ctx)) + gufo::PartialBytes(gufo::Sms(ctx));
   if (p->accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
   }
@@ -875,13 +965,12 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   a.whole = reinterpret_cast<uintptr_t>(p->queries) % 16 == 0 && ((p->query_token_stride | p->query_head_stride) & 3) == 0;
   uint8_t* scratch = static_cast<uint8_t*>(p->scratch);
   a.arrived = reinterpret_cast<unsigned*>(scratch);
-  a.sums = reinterpret_cast<float*>(scratch + gufo::ArrivedBytes(ctx->sm_count));
+  a.sums = reinterpret_cast<float*>(scratch + gufo::ArrivedBytes(gufo::Sms(ctx)));
   if (p->accumulate != 0) {
     a.finals = reinterpret_cast<float*>(scratch + own);
     a.scores = a.finals + 2 * rows;
   }
-  // Query rows of an item: as few groups of eight as hold a sequence's, up to what a warp's
-  // registers do (eight groups of 64 dimensions).
+  // Query rows of an item: as few groups of eight as hold a sequence's, four at most.
   const int ns = c.head_dim <= 64 ? 1 : c.head_dim <= 128 ? 2 : 4;
   int most = 1;
   for (int i = 0; i < batch->sequences; ++i) {
@@ -889,8 +978,8 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
     most = n > most ? n : most;
   }
   const int64_t rows_each = static_cast<int64_t>(most) * a.group;
-  a.stats = a.sums + static_cast<size_t>(2 * ctx->sm_count) * 8 * 64 * 8;
-  const int rt = rows_each <= 8 ? 1 : rows_each <= 16 || ns == 4 ? 2 : 4;
+  a.stats = a.sums + static_cast<size_t>(gufo::Sms(ctx)) * gufo::kPartialFloats;
+  const int rt = rows_each <= 8 ? 1 : rows_each <= 16 ? 2 : 4;
   if (tokens * a.group / (8 * rt) + batch->sequences > 65535) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
   }
