@@ -41,9 +41,7 @@
 namespace gufo {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = 4;
-constexpr int kTile = kWarps * kCacheBlock;   // rows that a block of threads takes at a time
+constexpr int kFewWarps = 4;                  // of a block of threads where there are many units
 // What a unit costs besides its tiles (queries, the join), and the least that a block gets, in tiles.
 constexpr int kUnitCost = 4;
 constexpr int kLeastCost = 4;
@@ -70,23 +68,26 @@ struct AttendArgs {
   float* finals;           // [query rows][2]: maximum, 1 / sum
 };
 
-// NS: segments of 64 dimensions (1, 2, 4), warps of a group; RT: groups of eight query rows.
-template <int NS, int RT>
+// NS: segments of 64 dimensions (1, 2, 4), warps of a group; RT: groups of eight query rows; W:
+// warps of a block of threads.
+template <int NS, int RT, int W>
 struct Shape {
-  static constexpr int kGroups = kWarps / NS;
+  static constexpr int kThreads = 32 * W;
+  static constexpr int kTile = W * kCacheBlock;             // rows that a block of threads takes at a time
+  static constexpr int kGroups = W / NS;
   static constexpr int kRowBytes = 64 * NS;
   static constexpr int kItem = kCacheBlock * kRowBytes;     // a block's keys or values
   static constexpr int kSlot = kItem + 16;                  // and their scale
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
-  static constexpr int kRing = kWarps * kSlots * kSlot;
+  static constexpr int kRing = W * kSlots * kSlot;
   static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
-  // Of threads that an SM holds: by registers (RT == 4: 168 a thread), or by shared memory.
-  static constexpr int kBlocks = RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
-  static constexpr int kParts = 8 * RT * kBlocks * kMostSms * 4;   // factors of a unit's parts
+  // Of threads that an SM holds: by registers (128, 168 or 255 a thread), or by shared memory.
+  static constexpr int kBlocks = W > kFewWarps ? 1 : RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
+  static constexpr int kParts = (8 * RT * kBlocks * kMostSms + 4 * kThreads) * 4;   // a unit's parts: factors, sums
   static constexpr int kLarger = kRing > kJoin ? kRing : kJoin;
   static constexpr int kShared = kLarger > kParts ? kLarger : kParts;
   static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order
-  static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
+  static constexpr int kWeights = NS == 1 ? 0 : 2 * W * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
 };
 
@@ -108,15 +109,16 @@ __device__ __forceinline__ void Meet(int group) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * NS) : "memory");
   }
 }
-// d = a b_low + a b_high: thirty-two products, added by the instruction.
-__device__ __forceinline__ void MmaHalves(float (&d)[4], const uint32_t (&a)[4], uint32_t high0, uint32_t high1, uint32_t low0,
-                                          uint32_t low1) {
+// d = a b, sixteen products added by the instruction; d += a b.
+__device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(low0), "r"(low1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void MmaMore(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(high0), "r"(high1));
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t Transpose(uint32_t v) {
   uint32_t t;
@@ -140,16 +142,18 @@ __device__ __forceinline__ int SeenBy(const AttendArgs& a, const BatchEntry& e, 
 }
 
 // Tiles of each sequence in `tiles` (one at least: a row that sees nothing is an output too) and
-// the cost of the units of all sequences ahead of it in `ahead` ([sequences + 1]).
-__device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int* tiles, long long* ahead) {
-  __shared__ long long of_warp[kBatchSequences / 32];
+// the cost of the units of all sequences ahead of it in `ahead` ([sequences + 1]). (The sum of
+// all is an int: the caller has made sure.)
+template <int W>
+__device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int* tiles, int* ahead) {
+  __shared__ int of_warp[kBatchSequences / 32];
   const int n = batch.sequences, i = threadIdx.x, warp = i >> 5, lane = i & 31;
   if (a.visible == nullptr) {
     if (i < n) {
       tiles[i] = SeenBy(a, batch.of[i], batch.positions[batch.of[i].index], batch.of[i].tokens - 1);
     }
   } else {
-    for (int s = warp; s < n; s += kWarps) {
+    for (int s = warp; s < n; s += W) {
       int most = 0;
       for (int token = lane; token < batch.of[s].tokens; token += 32) {
         most = max(most, SeenBy(a, batch.of[s], 0, token));
@@ -159,19 +163,20 @@ __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& b
         tiles[s] = most;
       }
     }
+    __syncthreads();
   }
-  __syncthreads();
-  long long sum = 0;
+  int sum = 0;
   if (i < kBatchSequences) {
-    long long mine = 0;
+    int mine = 0;
     if (i < n) {
-      tiles[i] = max(1, (tiles[i] + kTile - 1) / kTile);
-      mine = static_cast<long long>(batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * (tiles[i] + kUnitCost);
+      const int of = max(1, (tiles[i] + W * kCacheBlock - 1) / (W * kCacheBlock));
+      tiles[i] = of;
+      mine = (batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * (of + kUnitCost);
     }
     sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long below = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      const int below = __shfl_up_sync(0xFFFFFFFFu, sum, o);
       sum += lane >= o ? below : 0;
     }
     if (lane == 31) {
@@ -192,10 +197,11 @@ __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& b
 }
 
 // Grid: resident blocks.
-template <typename Format, int NS, int RT>
-__global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
+template <typename Format, int NS, int RT, int W>
+__global__ void __launch_bounds__(32 * W, (Shape<NS, RT, W>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
-  using S = Shape<NS, RT>;
+  using S = Shape<NS, RT, W>;
+  constexpr int kWarps = W, kThreads = S::kThreads, kTile = S::kTile;
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores
   __shared__ int row_seen[8 * RT];
@@ -203,7 +209,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT];
   __shared__ float final_total[8 * RT];
   __shared__ int tiles_of[kBatchSequences];
-  __shared__ long long cost_ahead[kBatchSequences + 1];
+  __shared__ int cost_ahead[kBatchSequences + 1];
   __shared__ int is_last;
   GridLaunchDependents();
   GridDependencyWait();
@@ -211,22 +217,21 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / NS, member = warp % NS;
   const int g = lane >> 2, t = lane & 3;
-  ShareOut(a, batch, tiles_of, cost_ahead);
-  const long long all = cost_ahead[batch.sequences];
-  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), max(all / kLeastCost, 1ll)));
+  ShareOut<W>(a, batch, tiles_of, cost_ahead);
+  const int all = cost_ahead[batch.sequences];
+  const int blocks = min(static_cast<int>(gridDim.x), max(all / kLeastCost, 1));
   if (blockIdx.x >= blocks) {
     return;
   }
-  // A unit's cost comes ahead of its tiles: a block whose stretch ends within it has no part of the unit.
-  const auto start_of = [&](long long block) { return all * block / blocks; };
-  const auto owner_of = [&](long long at) {     // the block whose stretch it is in
-    int b = static_cast<int>(at * blocks / all);
-    while (start_of(b + 1) <= at) {
-      ++b;
-    }
-    return b;
+  // A block's stretch: one more for the first `more` of them. A unit's cost comes ahead of its
+  // tiles: a block whose stretch ends within it has no part of the unit.
+  const int each = all / blocks, more = all - each * blocks;
+  const auto start_of = [&](int block) { return each * block + min(block, more); };
+  const auto owner_of = [&](int at) {     // the block whose stretch it is in
+    const int split = (each + 1) * more;
+    return at < split ? at / (each + 1) : more + (at - split) / each;
   };
-  const long long begin = start_of(blockIdx.x), end = start_of(blockIdx.x + 1ll);
+  const int begin = start_of(blockIdx.x), end = start_of(blockIdx.x + 1);
 
   constexpr int kPieces = S::kRowBytes / 16;    // of a row
   // Where a piece of a row stands, so that the eight lanes that read together meet eight
@@ -246,7 +251,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   uint4* const shared_p = reinterpret_cast<uint4*>(raw + S::kShared + S::kQuery);   // [2][warp][rt][lane]
 
 #pragma unroll 1
-  for (long long from = begin; from < end;) {
+  for (int from = begin; from < end;) {
     // ---- the unit that this is of
     int low = 0, high = batch.sequences - 1;
     while (low < high) {
@@ -258,18 +263,18 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
     }
     const int tiles = tiles_of[low];
-    const long long unit = (from - cost_ahead[low]) / (tiles + kUnitCost);
-    const long long unit_start = cost_ahead[low] + unit * (tiles + kUnitCost) + kUnitCost;   // of its tiles
-    const int first_tile = static_cast<int>(max(from - unit_start, 0ll));
-    const int last_tile = static_cast<int>(min(end - unit_start, static_cast<long long>(tiles)));
+    const int unit = (from - cost_ahead[low]) / (tiles + kUnitCost);
+    const int unit_start = cost_ahead[low] + unit * (tiles + kUnitCost) + kUnitCost;   // of its tiles
+    const int first_tile = max(from - unit_start, 0);
+    const int last_tile = min(end - unit_start, tiles);
     from = unit_start + tiles;
     if (last_tile <= first_tile) {
       continue;
     }
-    const int kh = static_cast<int>(unit % c.kv_heads);
+    const int chunk = unit / c.kv_heads, kh = unit - chunk * c.kv_heads;
     Task task;
     task.e = batch.of[low];
-    task.row0 = static_cast<int>(unit / c.kv_heads) * 8 * RT;
+    task.row0 = chunk * 8 * RT;
     task.rows = min(8 * RT, task.e.tokens * a.group - task.row0);
     task.position = batch.positions[task.e.index];
     if (threadIdx.x < 8 * RT) {
@@ -335,7 +340,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     }
 
     // ---- the queries: every fourth row to a warp, in the order of the B operands
-#pragma unroll 1
+#pragma unroll 2
     for (int r = warp; r < 8 * RT; r += kWarps) {
       const bool there = r < task.rows;
       const int flat = task.row0 + (there ? r : 0);
@@ -424,17 +429,29 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           const uint4 k0 = *reinterpret_cast<const uint4*>(keys + key_at(g, 4 * seg + t));
           const uint4 k1 = *reinterpret_cast<const uint4*>(keys + key_at(g + 8, 4 * seg + t));
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          uint32_t k[4][4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint32_t k[4];
-            Format::Decode(w0[j], k[0], k[2]);
-            Format::Decode(w1[j], k[1], k[3]);
+            Format::Decode(w0[j], k[j][0], k[j][2]);
+            Format::Decode(w1[j], k[j][1], k[j][3]);
+          }
+          // Four products at a time, low halves first: an instruction's result is not waited for.
 #pragma unroll
-            for (int rt = 0; rt < RA; ++rt) {
-              const uint4 q = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
-              float d[4];
-              MmaHalves(d, k, q.x, q.y, q.z, q.w);
-              s[rt][0] += d[0], s[rt][1] += d[1], s[rt][2] += d[2], s[rt][3] += d[3];
+          for (int rt = 0; rt < RA; ++rt) {
+            uint4 q[4];
+            float d[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              q[j] = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
+              MmaFirst(d[j], k[j], q[j].z, q[j].w);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              MmaMore(d[j], k[j], q[j].x, q[j].y);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[rt][i] += (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]);
             }
           }
         }
@@ -597,23 +614,30 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             const int r = 2 * t + (i & 1) + 8 * (i >> 1);
             v[i] = *reinterpret_cast<const uint2*>(values + value_at(r, 4 * member + (g >> 1)) + 8 * (g & 1));
           }
+          uint32_t of[4][4];   // dimensions 2 m, 2 m + 1 of the eight: rows beside one another
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t w0 = half ? v[0].y : v[0].x, w1 = half ? v[1].y : v[1].x, w2 = half ? v[2].y : v[2].x, w3 = half ? v[3].y : v[3].x;
+          for (int m = 0; m < 4; ++m) {
+            const uint32_t w0 = m < 2 ? v[0].x : v[0].y, w1 = m < 2 ? v[1].x : v[1].y;
+            const uint32_t w2 = m < 2 ? v[2].x : v[2].y, w3 = m < 2 ? v[3].x : v[3].y;
+            Format::Decode(__byte_perm(w0, w1, m & 1 ? 0x7362 : 0x5140), of[m][0], of[m][1]);
+            Format::Decode(__byte_perm(w2, w3, m & 1 ? 0x7362 : 0x5140), of[m][2], of[m][3]);
+          }
 #pragma unroll
-            for (int pair = 0; pair < 2; ++pair) {
-              uint32_t d_of[4];   // dimensions 2 pair, 2 pair + 1 of the word: rows beside one another
-              Format::Decode(__byte_perm(w0, w1, pair ? 0x7362 : 0x5140), d_of[0], d_of[1]);
-              Format::Decode(__byte_perm(w2, w3, pair ? 0x7362 : 0x5140), d_of[2], d_of[3]);
-              const int m = 2 * half + pair;
+          for (int rt = 0; rt < RA; ++rt) {
+            float d[4][4];
 #pragma unroll
-              for (int rt = 0; rt < RA; ++rt) {
-                float d[4];
-                MmaHalves(d, d_of, p[rt].x, p[rt].y, p[rt].z, p[rt].w);
+            for (int m = 0; m < 4; ++m) {
+              MmaFirst(d[m], of[m], p[rt].z, p[rt].w);
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  acc[rt][m][i] = fmaf(d[i], each[rt][i & 1], acc[rt][m][i]);
-                }
+            for (int m = 0; m < 4; ++m) {
+              MmaMore(d[m], of[m], p[rt].x, p[rt].y);
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                acc[rt][m][i] = fmaf(d[m][i], each[rt][i & 1], acc[rt][m][i]);
               }
             }
           }
@@ -785,32 +809,53 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           note(r, most, sum);
         }
       }
+      // Where there are more threads than outputs, several take a part of the parts each.
+      const int outputs = task.rows * fours;
+      const int takers = outputs >= kThreads ? 1 : min(kThreads / outputs, 8);
+      float4* partial = reinterpret_cast<float4*>(by + 8 * RT * S::kBlocks * kMostSms);    // [taker][output]
       __syncthreads();
-      for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
-        const int r = at / fours, f = at % fours;
+      for (int at = threadIdx.x; at < outputs * takers; at += kThreads) {
+        const int taker = at / outputs, r = (at - taker * outputs) / fours, f = (at - taker * outputs) % fours;
+        const int i_first = count * taker / takers, i_end = count * (taker + 1) / takers;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < count; i0 += 8) {
+        for (int i0 = i_first; i0 < i_end; i0 += 8) {
           float4 v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            v[i] = i0 + i < count ? __ldcg(reinterpret_cast<const float4*>(a.sums + (part_at(i0 + i) + r) * c.head_dim) + f)
+            v[i] = i0 + i < i_end ? __ldcg(reinterpret_cast<const float4*>(a.sums + (part_at(i0 + i) + r) * c.head_dim) + f)
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float f2 = i0 + i < count ? by[r * count + i0 + i] : 0.f;
+            const float f2 = i0 + i < i_end ? by[r * count + i0 + i] : 0.f;
             sum.x = fmaf(v[i].x, f2, sum.x), sum.y = fmaf(v[i].y, f2, sum.y), sum.z = fmaf(v[i].z, f2, sum.z), sum.w = fmaf(v[i].w, f2, sum.w);
           }
         }
-        finish(r, f, sum, final_total[r], row_seen[r]);
+        if (takers == 1) {
+          finish(r, f, sum, final_total[r], row_seen[r]);
+        } else {
+          partial[at] = sum;
+        }
+      }
+      if (takers > 1) {
+        __syncthreads();
+        for (int at = threadIdx.x; at < outputs; at += kThreads) {
+          float4 sum = partial[at];
+          for (int i = 1; i < takers; ++i) {
+            const float4 v = partial[i * outputs + at];
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+          }
+          finish(at / fours, at % fours, sum, final_total[at / fours], row_seen[at / fours]);
+        }
       }
     }
     __syncthreads();     // before the shared memory's next use
   }
 }
 
-// Weights of the rows: grid (groups of kThreads rows, KV heads, sequences).
-__global__ void __launch_bounds__(kThreads)
+// Weights of the rows: grid (groups of kWeightsThreads rows, KV heads, sequences).
+constexpr int kWeightsThreads = 128;
+__global__ void __launch_bounds__(kWeightsThreads)
 WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
   GridLaunchDependents();
   GridDependencyWait();
@@ -822,7 +867,7 @@ WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batc
   for (int token = 0; token < e.tokens; ++token) {
     length = max(length, SeenBy(a, e, position, token));
   }
-  const int row = blockIdx.x * kThreads + threadIdx.x;
+  const int row = blockIdx.x * kWeightsThreads + threadIdx.x;
   if (row >= length) {
     return;
   }
@@ -849,36 +894,45 @@ constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
 constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
 size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * (kPartialFloats + kStatsFloats) * sizeof(float); }
 
-template <typename Format, int NS, int RT>
+template <typename Format, int NS, int RT, int W>
 int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b) {
-  using S = Shape<NS, RT>;
+  using S = Shape<NS, RT, W>;
   static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
                 "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
   if (ctx->device >= 64 || !configured[ctx->device].load()) {
-    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     if (ctx->device < 64) {
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(Sms(ctx) * S::kBlocks), dim3(kThreads), S::kBytes,
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT, W>, dim3(Sms(ctx) * S::kBlocks), dim3(S::kThreads), S::kBytes,
                                  ctx->stream, 1, a, b));
   ctx->launches.fetch_add(1);
   return GUFO_CUDA_OK;
 }
 
+// Few units: one block of as many warps as registers and shared memory hold, so that a unit has
+// few parts. Many: small blocks, several of which an SM holds, so that one's queries and join
+// pass under another's tiles.
+template <typename Format, int NS, int RT>
+int PickWarps(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units) {
+  constexpr int kMany = RT == 1 ? 16 : RT == 2 ? (NS == 1 ? 16 : 12) : NS == 1 ? 12 : 8;
+  return units < Sms(ctx) ? LaunchAttend<Format, NS, RT, kMany>(ctx, a, b) : LaunchAttend<Format, NS, RT, kFewWarps>(ctx, a, b);
+}
+
 template <typename Format>
-int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int ns, int rt) {
+int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units, int ns, int rt) {
   switch (ns * 8 + rt) {
-    case 8 + 1: return LaunchAttend<Format, 1, 1>(ctx, a, b);
-    case 8 + 2: return LaunchAttend<Format, 1, 2>(ctx, a, b);
-    case 8 + 4: return LaunchAttend<Format, 1, 4>(ctx, a, b);
-    case 16 + 1: return LaunchAttend<Format, 2, 1>(ctx, a, b);
-    case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b);
-    case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b);
-    case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b);
-    case 32 + 2: return LaunchAttend<Format, 4, 2>(ctx, a, b);
-    default: return LaunchAttend<Format, 4, 4>(ctx, a, b);
+    case 8 + 1: return PickWarps<Format, 1, 1>(ctx, a, b, units);
+    case 8 + 2: return PickWarps<Format, 1, 2>(ctx, a, b, units);
+    case 8 + 4: return PickWarps<Format, 1, 4>(ctx, a, b, units);
+    case 16 + 1: return PickWarps<Format, 2, 1>(ctx, a, b, units);
+    case 16 + 2: return PickWarps<Format, 2, 2>(ctx, a, b, units);
+    case 16 + 4: return PickWarps<Format, 2, 4>(ctx, a, b, units);
+    case 32 + 1: return PickWarps<Format, 4, 1>(ctx, a, b, units);
+    case 32 + 2: return PickWarps<Format, 4, 2>(ctx, a, b, units);
+    default: return PickWarps<Format, 4, 4>(ctx, a, b, units);
   }
 }
 
@@ -987,15 +1041,20 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   const int group = a.group;
   return gufo::ForEachRun(
       *batch, [&](int n) { return static_cast<int>((static_cast<int64_t>(n) * group + 8 * rt - 1) / (8 * rt)); },
-      [&](const gufo::BatchArgs& b, int) -> int {
-        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, ns, rt)
-                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, ns, rt);
+      [&](const gufo::BatchArgs& b, int items) -> int {
+        const int64_t units = static_cast<int64_t>(items) * c.kv_heads;
+        if (units * (c.capacity / (gufo::kFewWarps * gufo::kCacheBlock) + 1 + gufo::kUnitCost) > INT32_MAX) {
+          return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
+        }
+        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, units, ns, rt)
+                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, units, ns, rt);
         if (run != GUFO_CUDA_OK || a.scores == nullptr) {
           return run;
         }
         GUFO_CUDA_TRY(gufo::LaunchOverlapped(gufo::WeightsKernel,
-                                             dim3((c.capacity + gufo::kThreads - 1) / gufo::kThreads, c.kv_heads, b.sequences),
-                                             dim3(gufo::kThreads), 0, ctx->stream, 1, a, b));
+                                             dim3((c.capacity + gufo::kWeightsThreads - 1) / gufo::kWeightsThreads, c.kv_heads,
+                                                  b.sequences),
+                                             dim3(gufo::kWeightsThreads), 0, ctx->stream, 1, a, b));
         ctx->launches.fetch_add(1);
         return GUFO_CUDA_OK;
       });
