@@ -6,7 +6,7 @@
 //
 // The arithmetic. A group of one, two or four warps (64 dimensions each) goes through tiles of
 // as many blocks of the cache (16 rows, one scale for the keys, one for the values), streamed
-// through rings in shared memory (cp.async). For each block one warp takes the scores, over all
+// through rings in shared memory (bulk copies). For each block one warp takes the scores, over all
 // dimensions; its weights then go to the group's warps, each of which adds up its 64 dimensions
 // of the group's blocks. So nothing is decoded twice, a warp's sums take 16 registers for eight
 // query rows whatever the head's size, and the group meets once a tile.
@@ -37,6 +37,7 @@
 
 #include "cache8.cuh"
 #include "decode_device.cuh"
+#include "mma_common.cuh"
 
 namespace gufo {
 namespace {
@@ -76,8 +77,7 @@ struct Shape {
   static constexpr int kTile = W * kCacheBlock;             // rows that a block of threads takes at a time
   static constexpr int kGroups = W / NS;
   static constexpr int kRowBytes = 64 * NS;
-  static constexpr int kItem = kCacheBlock * kRowBytes;     // a block's keys or values
-  static constexpr int kSlot = kItem + 16;                  // and their scale
+  static constexpr int kSlot = kCacheBlock * kRowBytes + 16;   // a block's keys or values, their scale
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
   static constexpr int kRing = W * kSlots * kSlot;
   static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
@@ -86,20 +86,23 @@ struct Shape {
   static constexpr int kParts = (8 * RT * kBlocks * kMostSms + 4 * kThreads) * 4;   // a unit's parts: factors, sums
   static constexpr int kLarger = kRing > kJoin ? kRing : kJoin;
   static constexpr int kShared = kLarger > kParts ? kLarger : kParts;
-  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order
+  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4)
   static constexpr int kWeights = NS == 1 ? 0 : 2 * W * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
 };
 
-__device__ __forceinline__ uint32_t SharedAt(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+// Waits until a copy that this kernel asked for has landed; false, once, where it has not after
+// about a second: what comes of it is made NaN then, and nothing is waited for any more.
+__device__ __noinline__ bool LandedLate(uint32_t bar, uint32_t parity) {
+  const long long began = clock64();
+  while (!MbarTryWait(bar, parity)) {
+    if (clock64() - began > kLandLimit) {
+      return false;
+    }
+  }
+  return true;
 }
-__device__ __forceinline__ void Copy16(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void Copy4(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
-}
+
 // The warps of a group meet.
 template <int NS>
 __device__ __forceinline__ void Meet(int group) {
@@ -109,16 +112,25 @@ __device__ __forceinline__ void Meet(int group) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * NS) : "memory");
   }
 }
-// d = a b, sixteen products added by the instruction; d += a b.
+// d = a b, sixteen products added by the instruction; d += a b. Volatile, so that a product stays
+// ahead of the barrier behind which its operands' place in shared memory is given back: its
+// issue is what waits for their loads.
 __device__ __forceinline__ void MmaFirst(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void MmaMore(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d += a b in whole numbers, thirty-two products.
+__device__ __forceinline__ void MmaWhole(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t Transpose(uint32_t v) {
   uint32_t t;
@@ -211,6 +223,15 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   __shared__ int tiles_of[kBatchSequences];
   __shared__ int cost_ahead[kBatchSequences + 1];
   __shared__ int is_last;
+  __shared__ __align__(16) uint4 nothing;        // a piece of zeros
+  __shared__ __align__(8) uint64_t bars[W][S::kSlots];
+  if (threadIdx.x < W * S::kSlots) {
+    MbarInit(SharedAddress(&bars[0][0] + threadIdx.x), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    nothing = make_uint4(0, 0, 0, 0);
+  }
   GridLaunchDependents();
   GridDependencyWait();
   const CacheView& c = a.cache;
@@ -233,20 +254,31 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   };
   const int begin = start_of(blockIdx.x), end = start_of(blockIdx.x + 1);
 
-  constexpr int kPieces = S::kRowBytes / 16;    // of a row
-  // Where a piece of a row stands, so that the eight lanes that read together meet eight
-  // different places of 16 bytes: keys by four pieces of two rows, values by two pieces of
-  // every second row of eight.
-  auto key_at = [](int r, int piece) { return (r * kPieces + (piece ^ (NS >= 2 ? 4 * (r & 1) : 0))) * 16; };
-  auto value_at = [](int r, int piece) {
-    if constexpr (NS == 1) {
-      return (r >> 1) * 128 + ((((r & 1) * 4 + piece) ^ (2 * (r >> 1 & 3))) * 16);
-    } else {
-      return (r * kPieces + (piece ^ (2 * (r >> 1 & 3)))) * 16;
-    }
-  };
   const auto ring_of = [&](int w) { return raw + w * (S::kSlots * S::kSlot); };
   uint8_t* const ring = ring_of(warp);
+  const int codes_bytes = kCacheBlock * c.head_dim, block_bytes = BlockBytes(c.head_dim);
+  const int pieces = c.head_dim / 16;
+  // This lane's places in a block: keys of row g (g + 8: 128 further), piece t of a segment
+  // (a segment: 1024 further); values of rows 2 t and 2 t + 1 (+ 8), eight dimensions of this
+  // warp's segment (past the last piece any: nobody asks for them).
+  const int key_place = PieceAt(0, g, t);
+  const int value_piece = min(4 * member + (g >> 1), pieces - 1);
+  const int value_place = PieceAt(1, 2 * t, value_piece) + 8 * (g & 1);
+  // The ring's slots go round, through all units: the next to be filled, the next to be read.
+  int fill_slot = 0, slot = 0, phase = 0;
+  bool late = false;
+  const auto wait_for = [&](int of_warp) {
+    const uint32_t bar = SharedAddress(&bars[of_warp][slot]);
+    if (!late && !MbarTryWait(bar, phase)) {
+      late = !LandedLate(bar, phase);
+    }
+  };
+  const auto next_slot = [&]() {
+    if (++slot == S::kSlots) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
   uint4* const query = reinterpret_cast<uint4*>(raw + S::kShared);   // [rt][seg * 4 + j][lane]: high pair, pair, low pair, pair
   uint4* const shared_p = reinterpret_cast<uint4*>(raw + S::kShared + S::kQuery);   // [2][warp][rt][lane]
 
@@ -292,47 +324,29 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     const int end_tile = min(last_tile, (length + kTile - 1) / kTile);
     const size_t of_head = static_cast<size_t>(task.e.slot) * c.kv_heads + kh;
 
-    // ---- the ring: a warp copies its block of every tile, keys and values in turn
-    const int whole_blocks = c.head_dim == S::kRowBytes ? length / kCacheBlock : 0;   // that can be copied as they are
-    int next_tile = first_tile, next_side = 0, next_slot = 0;
+    // ---- the ring: a warp copies its block of every tile, keys and values in turn (a block that
+    // nobody sees is not copied)
+    const uint8_t* const keys_from = BlocksOf(c, 0, of_head);
+    const uint8_t* const values_from = BlocksOf(c, 1, of_head);
+    int next_tile = first_tile;
+    bool next_values = false;
     auto load = [&]() {
       if (next_tile < end_tile) {
-        const int block = next_tile * kWarps + warp;
-        const uint32_t to = SharedAt(ring + next_slot * S::kSlot);
-        const uint8_t* codes = c.codes[next_side] + of_head * c.capacity * c.head_dim;
-        constexpr int kEach = 32 / kPieces;     // rows that the lanes copy at a time
-        const int r0 = lane / kPieces, piece = lane % kPieces;
-        if (block < whole_blocks) {
-          const uint8_t* k = codes + static_cast<size_t>(block) * S::kItem + lane * 16;
-          if (next_side == 0) {
-#pragma unroll
-            for (int i = 0; i < kCacheBlock / kEach; ++i) {
-              Copy16(to + key_at(r0, piece) + 512 * i, k + 512 * i, true);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kCacheBlock / kEach; ++i) {
-              Copy16(to + value_at(r0 + kEach * i, piece), k + 512 * i, true);
-            }
-          }
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < kCacheBlock / kEach; ++i) {
-            const int r = r0 + kEach * i;
-            const bool there = block * kCacheBlock + r < length && piece * 16 < c.head_dim;
-            const size_t at = there ? (static_cast<size_t>(block) * kCacheBlock + r) * c.head_dim + piece * 16 : 0;
-            Copy16(to + (next_side == 0 ? key_at(r, piece) : value_at(r, piece)), codes + at, there);
-          }
-        }
         if (lane == 0) {
-          const bool there = block * kCacheBlock < length;
-          Copy4(to + S::kItem, c.scales[next_side] + of_head * (c.capacity / kCacheBlock) + (there ? block : 0), there);
+          const int block = next_tile * kWarps + warp;
+          const uint32_t bar = SharedAddress(&bars[warp][fill_slot]);
+          if (block * kCacheBlock < length) {
+            MbarArriveExpectTx(bar, block_bytes);
+            BulkCopy(SharedAddress(ring + fill_slot * S::kSlot),
+                     (next_values ? values_from : keys_from) + static_cast<size_t>(block) * block_bytes, block_bytes, bar);
+          } else {
+            MbarArrive(bar);
+          }
         }
+        next_tile += next_values;
+        next_values = !next_values;
+        fill_slot = fill_slot + 1 == S::kSlots ? 0 : fill_slot + 1;
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      next_tile += next_side;
-      next_side ^= 1;
-      next_slot = next_slot + 1 == S::kSlots ? 0 : next_slot + 1;
     };
 #pragma unroll
     for (int i = 0; i < S::kSlots - 1; ++i) {
@@ -364,27 +378,61 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         top = max(max(top, __float_as_uint(x[i].z) & 0x7FFFFFFFu), __float_as_uint(x[i].w) & 0x7FFFFFFFu);
       }
       top = __reduce_max_sync(0xFFFFFFFFu, top);
-      // The largest to 2^14 .. 2^15. (Products with codes of up to 448 and their sums stay in fp32's range.)
-      const int e = min(max(static_cast<int>(top >> 23), 16), 250);
-      const float up = PowerOfTwo(141 - e);
+      if constexpr (Format::kWhole) {
+        // Whole numbers of 23 bits (the largest 2^21 .. 2^22) as three signed bytes, base 256:
+        // rounded to half of 2^-21 of the largest. A row that is not finite: any, its factor is NaN.
+        const int e = min(max(static_cast<int>(top >> 23), 23), 250);
+        const float up = PowerOfTwo(148 - e);
 #pragma unroll
-      for (int i = 0; i < kTimes; ++i) {
-        const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
-        if (f < 16 * NS) {
-          const int seg = f / 16, of = f % 16 / 4, j = f % 4;
-          const float v[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
-          __half high[4], low[4];
+        for (int i = 0; i < kTimes; ++i) {
+          const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
+          if (f < 16 * NS) {
+            const int seg = f / 16, of = f % 16 / 4, j = f % 4;
+            const int v[4] = {__float2int_rn(x[i].x * up), __float2int_rn(x[i].y * up), __float2int_rn(x[i].z * up),
+                              __float2int_rn(x[i].w * up)};
+            uint32_t digits[3] = {0, 0, 0};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            high[k] = __float2half_rn(v[k]);
-            low[k] = __float2half_rn(v[k] - __half2float(high[k]));
+            for (int k = 0; k < 4; ++k) {
+              // Offset by 128, the bytes of v + 0x808080 are the balanced digits.
+              const uint32_t z = (static_cast<uint32_t>(v[k]) + 0x808080u) ^ 0x808080u;
+#pragma unroll
+              for (int l = 0; l < 3; ++l) {
+                digits[l] |= (z >> (8 * l) & 0xFFu) << (8 * k);
+              }
+            }
+            uint32_t* to = reinterpret_cast<uint32_t*>(query);     // [rt][seg][digit][lane][j]
+#pragma unroll
+            for (int l = 0; l < 3; ++l) {
+              to[((((r / 8 * NS + seg) * 3 + l) * 32) + r % 8 * 4 + of) * 4 + j] = digits[l];
+            }
           }
-          query[(r / 8 * 4 * NS + seg * 4 + j) * 32 + r % 8 * 4 + of] = make_uint4(
-              PackHalves(high[0], high[1]), PackHalves(high[2], high[3]), PackHalves(low[0], low[1]), PackHalves(low[2], low[3]));
         }
-      }
-      if (lane == 0) {
-        row_factor[r] = a.scale * PowerOfTwo(e - 141);
+        if (lane == 0) {
+          row_factor[r] = top < 0x7F800000u ? a.scale * PowerOfTwo(e - 148) : NAN;
+        }
+      } else {
+        // The largest to 2^14 .. 2^15. (Products with codes of up to 448 and their sums stay in fp32's range.)
+        const int e = min(max(static_cast<int>(top >> 23), 16), 250);
+        const float up = PowerOfTwo(141 - e);
+#pragma unroll
+        for (int i = 0; i < kTimes; ++i) {
+          const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
+          if (f < 16 * NS) {
+            const int seg = f / 16, of = f % 16 / 4, j = f % 4;
+            const float v[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
+            __half high[4], low[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              high[k] = __float2half_rn(v[k]);
+              low[k] = __float2half_rn(v[k] - __half2float(high[k]));
+            }
+            query[(r / 8 * 4 * NS + seg * 4 + j) * 32 + r % 8 * 4 + of] = make_uint4(
+                PackHalves(high[0], high[1]), PackHalves(high[2], high[3]), PackHalves(low[0], low[1]), PackHalves(low[2], low[3]));
+          }
+        }
+        if (lane == 0) {
+          row_factor[r] = a.scale * PowerOfTwo(e - 141);
+        }
       }
     }
     __syncthreads();
@@ -411,51 +459,85 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     // RA: groups of eight rows that there are.
     const auto go = [&](auto groups) {
       constexpr int RA = decltype(groups)::value;
-      int slot = 0, parity = 0;
+      int parity = 0;
 #pragma unroll 1
       for (int tile = first_tile; tile < end_tile; ++tile) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 2) : "memory");
-        __syncwarp();
+        wait_for(warp);
         // Scores of this warp's block.
         const uint8_t* keys = ring + slot * S::kSlot;
-        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+        next_slot();
         float s[RA][4];
-#pragma unroll
-        for (int rt = 0; rt < RA; ++rt) {
-          s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
-        }
-#pragma unroll
-        for (int seg = 0; seg < NS; ++seg) {
-          const uint4 k0 = *reinterpret_cast<const uint4*>(keys + key_at(g, 4 * seg + t));
-          const uint4 k1 = *reinterpret_cast<const uint4*>(keys + key_at(g + 8, 4 * seg + t));
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-          uint32_t k[4][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            Format::Decode(w0[j], k[j][0], k[j][2]);
-            Format::Decode(w1[j], k[j][1], k[j][3]);
-          }
-          // Four products at a time, low halves first: an instruction's result is not waited for.
+        const auto key_words = [&](int seg, int more) {
+          const uint8_t* at = keys + key_place + 1024 * seg + more;
+          return *reinterpret_cast<const uint4*>(4 * seg + t < pieces ? at : reinterpret_cast<const uint8_t*>(&nothing));
+        };
+        if constexpr (Format::kWhole) {
+          int d[RA][3][4];      // by the queries' digits
 #pragma unroll
           for (int rt = 0; rt < RA; ++rt) {
-            uint4 q[4];
-            float d[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              q[j] = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
-              MmaFirst(d[j], k[j], q[j].z, q[j].w);
+            for (int l = 0; l < 3; ++l) {
+              d[rt][l][0] = d[rt][l][1] = d[rt][l][2] = d[rt][l][3] = 0;
             }
+          }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              MmaMore(d[j], k[j], q[j].x, q[j].y);
+          for (int seg = 0; seg < NS; ++seg) {
+            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 128);
+#pragma unroll
+            for (int rt = 0; rt < RA; ++rt) {
+#pragma unroll
+              for (int l = 0; l < 3; ++l) {
+                const uint4 q = query[((rt * NS + seg) * 3 + l) * 32 + lane];
+                MmaWhole(d[rt][l], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
+                MmaWhole(d[rt][l], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
+              }
             }
+          }
+          // (A digit's sum is at most 256 * 128 * 127: two of them fit an int, the lowest a float.)
+#pragma unroll
+          for (int rt = 0; rt < RA; ++rt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              s[rt][i] += (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]);
+              s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int rt = 0; rt < RA; ++rt) {
+            s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
+          }
+#pragma unroll
+          for (int seg = 0; seg < NS; ++seg) {
+            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 128);
+            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+            uint32_t k[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              Format::Decode(w0[j], k[j][0], k[j][2]);
+              Format::Decode(w1[j], k[j][1], k[j][3]);
+            }
+            // Four products at a time, low halves first: an instruction's result is not waited for.
+#pragma unroll
+            for (int rt = 0; rt < RA; ++rt) {
+              uint4 q[4];
+              float d[4][4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                q[j] = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
+                MmaFirst(d[j], k[j], q[j].z, q[j].w);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                MmaMore(d[j], k[j], q[j].x, q[j].y);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                s[rt][i] += (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]);
+              }
             }
           }
         }
-        const float key_scale = *reinterpret_cast<const float*>(keys + S::kItem);
+        const float key_scale = *reinterpret_cast<const float*>(keys + codes_bytes);
         const int r0 = (tile * kWarps + warp) * kCacheBlock + g;
         const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
         uint4 p[RA];             // high pair of rows 0-7, of 8-15; low pairs
@@ -515,8 +597,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             shared_p[((parity * kWarps + warp) * RT + rt) * 32 + lane] = p[rt];
           }
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(S::kSlots - 3) : "memory");
-        Meet<NS>(group);       // weights and values are there; the last tile's values and this one's keys are done with
+        Meet<NS>(group);       // the weights are there; the last tile's values and this one's keys are done with
         load();
         load();
         // Where a block has raised the maximum: the sums to it.
@@ -550,6 +631,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         // This warp's dimensions of the group's blocks.
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
+          wait_for(group * NS + b);
           uint8_t* values = ring_of(group * NS + b) + slot * S::kSlot;
           if constexpr (Format::kHasNan) {
             // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
@@ -557,14 +639,13 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             // values are put into the sums by hand and taken out of the tile.
             if (hides) {
               const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
-              const auto word_at = [&](int i) {       // of this warp's dimensions: 16 rows of 16 words
-                const int r = i / 16, w = i % 16;
-                return reinterpret_cast<uint32_t*>(values + value_at(r, 4 * member + w / 4)) + w % 4;
-              };
+              // This warp's pieces: 64 words each.
+              uint32_t* const words = reinterpret_cast<uint32_t*>(values) + 256 * member;
+              const int count = 64 * min(4, pieces - 4 * member);
               uint32_t found = 0;
 #pragma unroll 1
-              for (int i = lane; i < 256; i += 32) {
-                found |= marks(*word_at(i));
+              for (int i = lane; i < count; i += 32) {
+                found |= marks(words[i]);
               }
               if (__any_sync(0xFFFFFFFFu, found != 0)) {
 #pragma unroll
@@ -575,7 +656,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
                     int row = INT_MAX;      // the first with NaN
 #pragma unroll 1
                     for (int r = kCacheBlock - 1; r >= 0; --r) {
-                      const uint8_t code = values[value_at(r, 4 * member + dim / 16) + dim % 16];
+                      const uint8_t code = values[PieceAt(1, r, value_piece) + dim % 16];
                       row = (code & 0x7F) == 0x7F ? (tile * kWarps + group * NS + b) * kCacheBlock + r : row;
                     }
 #pragma unroll
@@ -587,14 +668,19 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
                 }
                 __syncwarp();
 #pragma unroll 1
-                for (int i = lane; i < 256; i += 32) {
-                  *word_at(i) &= ~((marks(*word_at(i)) >> 7) * 255u);
+                for (int i = lane; i < count; i += 32) {
+                  words[i] &= ~((marks(words[i]) >> 7) * 255u);
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // ahead of the slot's next copy
                 __syncwarp();
               }
             }
           }
-          const float by = *reinterpret_cast<const float*>(values + S::kItem) * (1.f / kProbScale);
+          // (Read ahead of the values, which the products wait for: the slot is given back behind
+          // those. A block that was not copied adds nothing, whatever stands there.)
+          float by;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(SharedAddress(values + codes_bytes)) : "memory");
+          by = (tile * kWarps + group * NS + b) * kCacheBlock < length ? by * (1.f / kProbScale) : 0.f;
           float each[RA][2];
 #pragma unroll
           for (int rt = 0; rt < RA; ++rt) {
@@ -611,8 +697,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-            v[i] = *reinterpret_cast<const uint2*>(values + value_at(r, 4 * member + (g >> 1)) + 8 * (g & 1));
+            v[i] = *reinterpret_cast<const uint2*>(values + (value_place ^ (16 * (i & 1))) + 128 * (i >> 1));
           }
           uint32_t of[4][4];   // dimensions 2 m, 2 m + 1 of the eight: rows beside one another
 #pragma unroll
@@ -642,11 +727,8 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             }
           }
         }
-        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+        next_slot();
         parity ^= 1;
-        if constexpr (NS == 1) {
-          __syncwarp();
-        }
       }
     };
     if constexpr (RT == 1) {
@@ -658,7 +740,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     } else {
       go(std::integral_constant<int, RT>());
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (late) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        total[rt][0] = total[rt][1] = NAN;
+      }
+    }
 
     // ---- the groups' parts together
 #pragma unroll
@@ -768,7 +855,8 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
     }
     if (alone) {
-      __syncthreads();     // before the shared memory's next use
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rings are written by copies again
+      __syncthreads();
       continue;
     }
     const int first_block = owner_of(unit_start), count = owner_of(unit_start + tiles - 1) - first_block + 1;
@@ -849,7 +937,8 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         }
       }
     }
-    __syncthreads();     // before the shared memory's next use
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rings are written by copies again
+    __syncthreads();
   }
 }
 

@@ -72,7 +72,8 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
     }
   }
   const bool joins = row0 < start;   // rows that stay are in the block
-  float* scale_at = c.scales[side] + of_head * (c.capacity / kCacheBlock) + block;
+  uint8_t* codes = BlocksOf(c, side, of_head) + static_cast<size_t>(block) * BlockBytes(c.head_dim);
+  float* scale_at = ScaleOf(codes, c.head_dim);
   const float was = joins ? *scale_at : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -88,7 +89,6 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
     exponent = max(exponent, ExponentOf(was));
   }
   const float inverse = PowerOfTwo(-exponent);   // (exponent is -126 .. 120)
-  uint8_t* codes = c.codes[side] + (of_head * c.capacity + row0 + 4 * warp) * c.head_dim;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = row0 + 4 * warp + i;
@@ -98,7 +98,7 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
       if (f >= fours) {
         continue;
       }
-      uint32_t* to = reinterpret_cast<uint32_t*>(codes + static_cast<size_t>(i) * c.head_dim) + f;
+      uint32_t* to = reinterpret_cast<uint32_t*>(codes + PieceAt(side, 4 * warp + i, f / 4)) + f % 4;
       if (r >= start && r < end) {
         const float4 v = x[i][n];
         *to = Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
@@ -154,8 +154,10 @@ RowsKernel(const __grid_constant__ RowsArgs a, const __grid_constant__ BatchArgs
     scale[i] = 0.f;
     if (token < e.tokens && r >= 0 && r < c.capacity) {
       const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + in_row / fours;
-      word[i] = __ldcs(reinterpret_cast<const uint32_t*>(c.codes[side] + (of_head * c.capacity + r) * c.head_dim) + in_row % fours);
-      scale[i] = c.scales[side][of_head * (c.capacity / kCacheBlock) + r / kCacheBlock];
+      const unsigned f = in_row % fours;
+      const uint8_t* block = BlocksOf(c, side, of_head) + (r / kCacheBlock) * BlockBytes(c.head_dim);
+      word[i] = *(reinterpret_cast<const uint32_t*>(block + PieceAt(side, r % kCacheBlock, f / 4)) + f % 4);
+      scale[i] = *ScaleOf(block, c.head_dim);
     }
   }
 #pragma unroll
@@ -248,23 +250,21 @@ int gufo_cuda_cache8_create(gufo_cuda_ctx* ctx, const gufo_cuda_cache8_config* c
   const size_t heads = static_cast<size_t>(config->sequences) * config->kv_heads;
   const auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   const size_t rows = heads * static_cast<size_t>(config->capacity);   // at most 2^50
-  const size_t codes = whole(rows * config->head_dim), scales = whole(rows / gufo::kCacheBlock * 4);
+  const size_t side = whole(rows / gufo::kCacheBlock * gufo::BlockBytes(config->head_dim));
   const size_t weights = config->weights != 0 ? whole(rows * 4) : 0;
   std::lock_guard<std::mutex> lock(ctx->mu);
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   uint8_t* data = nullptr;
-  const size_t bytes = 2 * codes + 2 * scales + weights;
+  const size_t bytes = 2 * side + weights;
   GUFO_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&data), bytes));
   const cudaError_t e = cudaMemsetAsync(data, 0, bytes, ctx->stream);
   if (e != cudaSuccess) {
     cudaFree(data);
     return gufo::CudaFail(e, "cache8_create");
   }
-  cache.codes[0] = data;
-  cache.codes[1] = data + codes;
-  cache.scales[0] = reinterpret_cast<float*>(data + 2 * codes);
-  cache.scales[1] = reinterpret_cast<float*>(data + 2 * codes + scales);
-  cache.weights = weights != 0 ? reinterpret_cast<float*>(data + 2 * codes + 2 * scales) : nullptr;
+  cache.sides[0] = data;
+  cache.sides[1] = data + side;
+  cache.weights = weights != 0 ? reinterpret_cast<float*>(data + 2 * side) : nullptr;
   const int64_t id = ctx->next_id++;
   try {
     ctx->caches.emplace(id, cache);
@@ -287,7 +287,7 @@ int gufo_cuda_cache8_free(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle) {
   }
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   GUFO_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-  GUFO_CUDA_TRY(cudaFree(it->second.codes[0]));
+  GUFO_CUDA_TRY(cudaFree(it->second.sides[0]));
   ctx->caches.erase(it);
   return GUFO_CUDA_OK;
 }

@@ -26,15 +26,33 @@ struct BatchArgs {
   const int* positions;
 };
 
-// What a kernel sees of a cache.
+// What a kernel sees of a cache. A block of 16 rows of a head is 16 * head_dim codes, then their
+// scale and 12 bytes of nothing: one contiguous copy. The codes stand piece by piece (16 values),
+// the 16 rows' bytes of a piece together, in an order of the rows that lets the attention's
+// lanes read them in fragments from different places of shared memory: for keys eight lanes read
+// four pieces of two rows, for values two pieces of every second row.
 struct CacheView {
-  uint8_t* codes[2];
-  float* scales[2];
+  uint8_t* sides[2];
   float* weights;
   int kv_heads, head_dim, capacity;
 };
 inline CacheView ViewOf(const Cache8& c) {
-  return {{c.codes[0], c.codes[1]}, {c.scales[0], c.scales[1]}, c.weights, c.c.kv_heads, c.c.head_dim, c.c.capacity};
+  return {{c.sides[0], c.sides[1]}, c.weights, c.c.kv_heads, c.c.head_dim, c.c.capacity};
+}
+__host__ __device__ inline int BlockBytes(int head_dim) { return kCacheBlock * head_dim + 16; }
+// The first block of a head of a slot, and of a side's block its scale.
+__device__ __forceinline__ uint8_t* BlocksOf(const CacheView& c, int side, size_t of_head) {
+  return c.sides[side] + of_head * (c.capacity / kCacheBlock) * BlockBytes(c.head_dim);
+}
+__device__ __forceinline__ float* ScaleOf(uint8_t* block, int head_dim) {
+  return reinterpret_cast<float*>(block + kCacheBlock * head_dim);
+}
+__device__ __forceinline__ const float* ScaleOf(const uint8_t* block, int head_dim) {
+  return reinterpret_cast<const float*>(block + kCacheBlock * head_dim);
+}
+// Where a piece of a row stands in its block.
+__device__ __forceinline__ int PieceAt(int side, int row, int piece) {
+  return (piece * kCacheBlock + (row ^ (side == 0 ? 2 * (piece & 3) : piece & 7))) * 16;
 }
 
 // Calls launch(args) for every run of at most kBatchSequences sequences with work; items(tokens)
@@ -100,6 +118,7 @@ __device__ __forceinline__ int PositionOf(const CacheView& c, const BatchArgs& b
 
 struct E4m3 {
   static constexpr bool kHasNan = true;    // codes 0x7F and 0xFF
+  static constexpr bool kWhole = false;    // codes are not whole numbers
   // The power of two of the smallest scale that holds a magnitude with these fp32 bits: 448 = 1.75 * 2^8.
   __device__ static int ScaleExponent(uint32_t bits) {
     return static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7);
@@ -119,6 +138,7 @@ struct E4m3 {
 
 struct Int8 {
   static constexpr bool kHasNan = false;
+  static constexpr bool kWhole = true;
   // 127 = 1.984375 * 2^6.
   __device__ static int ScaleExponent(uint32_t bits) {
     return static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) <= 0x7E0000u ? 6 : 5);

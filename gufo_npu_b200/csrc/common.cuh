@@ -91,13 +91,11 @@ struct Rope {
   float magnitude = 1.f;
 };
 
-// A key / value cache in 8 bits (cache8.cu): device memory, laid out as
-// [sequences][kv_heads][capacity][head_dim] codes, [..][capacity / 16] scales and
-// [..][capacity] weights.
+// A key / value cache in 8 bits (cache8.cu): device memory, laid out as keys and values
+// [sequences][kv_heads][capacity / 16] blocks and weights [sequences][kv_heads][capacity].
 struct Cache8 {
   gufo_cuda_cache8_config c{};
-  uint8_t* codes[2] = {nullptr, nullptr};   // keys, values
-  float* scales[2] = {nullptr, nullptr};
+  uint8_t* sides[2] = {nullptr, nullptr};   // keys, values
   float* weights = nullptr;                 // may be null
 };
 

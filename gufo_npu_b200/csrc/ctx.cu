@@ -515,7 +515,7 @@ int gufo_cuda_ctx_destroy(gufo_cuda_ctx* ctx) {
     cudaFree(kv.second.turns);
   }
   for (auto& kv : ctx->caches) {
-    cudaFree(kv.second.codes[0]);   // one allocation
+    cudaFree(kv.second.sides[0]);   // one allocation
   }
   cudaFree(ctx->stage_x);
   cudaFree(ctx->stage_y);

@@ -194,10 +194,9 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
   const int* kept = a.kept + (static_cast<size_t>(e.index) * c.kv_heads + head) * a.budget;
   const size_t source = static_cast<size_t>(e.slot) * c.kv_heads + head;
   const size_t target = static_cast<size_t>(a.into_slots[blockIdx.z]) * c.kv_heads + head;
-  const uint8_t* from = c.codes[side] + source * c.capacity * c.head_dim;
-  const float* from_scales = c.scales[side] + source * (c.capacity / kCacheBlock);
-  uint8_t* to = a.into.codes[side] + target * a.into.capacity * c.head_dim;
-  float* to_scales = a.into.scales[side] + target * (a.into.capacity / kCacheBlock);
+  const uint8_t* from = BlocksOf(c, side, source);
+  uint8_t* to = BlocksOf(a.into, side, target);
+  const int bytes = BlockBytes(c.head_dim);
   const int pieces = c.head_dim / 16;   // of a row
   const int blocks = (a.budget + kCacheBlock - 1) / kCacheBlock;
   for (int first = blockIdx.x * kMoveWarps; first - static_cast<int>(blockIdx.x * kMoveWarps) < blocks;
@@ -206,23 +205,24 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
     const int row = block * kCacheBlock + lane;
     const int mine = block < blocks && lane < kCacheBlock && row < a.budget ? kept[row] : -1;
     const bool moves = __any_sync(0xFFFFFFFFu, mine >= 0 && (!kInPlace || mine != row));
-    const float was = moves && mine >= 0 ? from_scales[mine / kCacheBlock] : 0.f;
+    const float was = moves && mine >= 0 ? *ScaleOf(from + static_cast<size_t>(mine / kCacheBlock) * bytes, c.head_dim) : 0.f;
     uint4 word[kTimes];
     float top = 0.f;
     if (moves) {
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        const int at = lane + 32 * i, r = at / pieces;
-        const int row_of = __shfl_sync(0xFFFFFFFFu, mine, r & 15);
+        // (Sixteen lanes gather a piece of all rows: what they write is together.)
+        const int r = lane & 15, piece = (lane >> 4) + 2 * i;
+        const int row_of = __shfl_sync(0xFFFFFFFFu, mine, r);
         word[i] = make_uint4(0, 0, 0, 0);
-        if (r < kCacheBlock && row_of >= 0) {
-          word[i] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<size_t>(row_of) * c.head_dim) + (at - r * pieces));
+        if (piece < pieces && row_of >= 0) {
+          word[i] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<size_t>(row_of / kCacheBlock) * bytes +
+                                                          PieceAt(side, row_of % kCacheBlock, piece)));
         }
       }
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        const int r = (lane + 32 * i) / pieces;
-        const float scale = __shfl_sync(0xFFFFFFFFu, was, r & 15);
+        const float scale = __shfl_sync(0xFFFFFFFFu, was, lane & 15);
         __half2 most = __float2half2_rn(0.f);
         const uint32_t w[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
 #pragma unroll
@@ -232,7 +232,7 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
           most = __hmax2(most, __hmax2(__habs2(*reinterpret_cast<const __half2*>(&x)), __habs2(*reinterpret_cast<const __half2*>(&y))));
         }
         const float m = fmaxf(__low2float(most), __high2float(most));   // (maxima pass NaN by)
-        top = fmaxf(top, r < kCacheBlock ? m * scale : 0.f);
+        top = fmaxf(top, m * scale);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -247,10 +247,10 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
       const float now = PowerOfTwo(exponent), inverse = PowerOfTwo(-exponent);
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        const int at = lane + 32 * i, r = at / pieces;
-        const float scale = __shfl_sync(0xFFFFFFFFu, was, r & 15);
-        const int there = __shfl_sync(0xFFFFFFFFu, mine, r & 15);
-        if (r >= kCacheBlock || there < 0) {
+        const int r = lane & 15, piece = (lane >> 4) + 2 * i;
+        const float scale = __shfl_sync(0xFFFFFFFFu, was, r);
+        const int there = __shfl_sync(0xFFFFFFFFu, mine, r);
+        if (piece >= pieces || there < 0) {
           continue;
         }
         uint4 out = word[i];
@@ -262,10 +262,10 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
           };
           out = make_uint4(again(out.x), again(out.y), again(out.z), again(out.w));
         }
-        *(reinterpret_cast<uint4*>(to + static_cast<size_t>(block * kCacheBlock + r) * c.head_dim) + (at - r * pieces)) = out;
+        *reinterpret_cast<uint4*>(to + static_cast<size_t>(block) * bytes + PieceAt(side, r, piece)) = out;
       }
       if (lane == 0) {
-        to_scales[block] = now;
+        *ScaleOf(to + static_cast<size_t>(block) * bytes, c.head_dim) = now;
       }
     }
   }
