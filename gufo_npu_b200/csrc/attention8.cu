@@ -26,8 +26,9 @@
 // The split. A unit of work is (sequence, group of query rows, KV head) with all the tiles
 // that the sequence is long. The device's resident blocks of threads share out the tiles of all
 // units, in order, to one tile: each finds its stretch from the lengths that it reads, whatever
-// they are, and goes through the units that it touches. A unit that several blocks have a part
-// of is put together by the last of them to arrive at a counter, part by part in order.
+// they are, and goes through the units that it touches. What several blocks have a part of, a
+// second kernel puts together, part by part in order: as a last block's work behind a counter
+// it took 5 us more of the first one's time (fence, counter, two rounds through L2 by one block).
 //
 // The weights of the rows (for eviction) need every query's final maximum and sum: the scores
 // are written down as they come, 4 bytes against 2 * head_dim / group read for them, and a
@@ -42,13 +43,23 @@
 namespace gufo {
 namespace {
 
-constexpr int kFewWarps = 4;                  // of a block of threads where there are many units
-// What a unit costs besides its tiles (queries, the join), and the least that a block gets, in tiles.
-constexpr int kUnitCost = 4;
-constexpr int kLeastCost = 4;
+constexpr int kMostUnitCost = 22;
+constexpr int kThreads = 128;
+constexpr int kWarps = 4;
 constexpr int kMostSms = 160;                 // whose blocks a call uses
+constexpr int kMostBlocks = 4 * kMostSms;     // of threads: four an SM at most
 constexpr float kProbScale = 32768.f;
 constexpr float kLog2e = 1.4426950408889634f;
+
+// A unit that several blocks have a part of: what the second kernel needs to know. One for every
+// unit, or, where they are more than the blocks, for the last one that each block begins.
+struct Cut {
+  int first;       // block
+  int parts;       // blocks with a part of it; 0: none is cut here
+  int rows;        // query rows
+  int token, head; // of its first row
+  int first_flat;  // that row's place among the sequence's tokens' heads of this KV head
+};
 
 struct AttendArgs {
   CacheView cache;
@@ -61,33 +72,36 @@ struct AttendArgs {
   const int* visible;
   int heads, group;
   float scale;             // times log2 e
-  int whole;               // query rows may be read four values at a time
-  unsigned* arrived;       // [blocks of threads]: of the unit that is cut behind a block's stretch
-  float* sums;             // [blocks][2: first, last unit][rows][head_dim]
+  int whole;               // rows of queries, gates and outputs may be taken four values at a time
+  Cut* cuts;               // [units or blocks]
+  int by_unit;
+  float* sums;             // [blocks][2: the unit it goes on with, the one it begins][rows][head_dim]
   float* stats;            // [blocks][2][rows][2]
   float* scores;           // [query rows][capacity]; null: no weights
   float* finals;           // [query rows][2]: maximum, 1 / sum
 };
 
-// NS: segments of 64 dimensions (1, 2, 4), warps of a group; RT: groups of eight query rows; W:
-// warps of a block of threads.
-template <int NS, int RT, int W>
+// NS: segments of 64 dimensions (1, 2, 4), warps of a group; RT: groups of eight query rows.
+// Small blocks of threads, several of which an SM holds: one's queries and join pass under
+// another's tiles (one block of 16 warps an SM: the verify batch 90 us, not 75; one long sequence
+// 60, not 64).
+template <int NS, int RT>
 struct Shape {
-  static constexpr int kThreads = 32 * W;
-  static constexpr int kTile = W * kCacheBlock;             // rows that a block of threads takes at a time
-  static constexpr int kGroups = W / NS;
+  static constexpr int kTile = NS * kCacheBlock;            // rows that a group takes at a time
+  static constexpr int kGroups = kWarps / NS;
+  // What a unit costs besides its tiles (queries, the join), in tiles: some 4 us, in which a
+  // block's share of the memory's rate brings 44 KB.
+  static constexpr int kUnitCost = kMostUnitCost / (NS * NS * RT) > 0 ? kMostUnitCost / (NS * NS * RT) : 1;
   static constexpr int kRowBytes = 64 * NS;
   static constexpr int kSlot = kCacheBlock * kRowBytes + 16;   // a block's keys or values, their scale
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
-  static constexpr int kRing = W * kSlots * kSlot;
+  static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
-  // Of threads that an SM holds: by registers (128, 168 or 255 a thread), or by shared memory.
-  static constexpr int kBlocks = W > kFewWarps ? 1 : RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
-  static constexpr int kParts = (8 * RT * kBlocks * kMostSms + 4 * kThreads) * 4;   // a unit's parts: factors, sums
-  static constexpr int kLarger = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kShared = kLarger > kParts ? kLarger : kParts;
+  // Of threads that an SM holds: by registers (RT == 4: 168 a thread or more), or by shared memory.
+  static constexpr int kBlocks = RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
+  static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
   static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4)
-  static constexpr int kWeights = NS == 1 ? 0 : 2 * W * RT * 32 * 16;   // the same of two tiles' weights
+  static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
 };
 
@@ -149,23 +163,32 @@ struct Task {
 };
 
 __device__ __forceinline__ int SeenBy(const AttendArgs& a, const BatchEntry& e, int position, int token) {
-  const int64_t seen = a.visible != nullptr ? a.visible[e.row + token] : static_cast<int64_t>(position) + token + 1;
+  const int64_t seen = a.visible != nullptr ? __ldcg(a.visible + e.row + token) : static_cast<int64_t>(position) + token + 1;
   return static_cast<int>(min(max(seen, static_cast<int64_t>(0)), static_cast<int64_t>(a.cache.capacity)));
 }
 
 // Tiles of each sequence in `tiles` (one at least: a row that sees nothing is an output too) and
 // the cost of the units of all sequences ahead of it in `ahead` ([sequences + 1]). (The sum of
-// all is an int: the caller has made sure.)
-template <int W>
-__device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int* tiles, int* ahead) {
+// all is an int: the caller has made sure.) Threads: 128 at least.
+struct Shares {
+  int tiles[kBatchSequences];
+  int ahead[kBatchSequences + 1];
+  int position[kBatchSequences];
+};
+__device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& batch, int tile_rows, int unit_cost, Shares& shares) {
+  int* const tiles = shares.tiles;
+  int* const ahead = shares.ahead;
   __shared__ int of_warp[kBatchSequences / 32];
   const int n = batch.sequences, i = threadIdx.x, warp = i >> 5, lane = i & 31;
+  if (i < n) {
+    shares.position[i] = __ldcg(batch.positions + batch.of[i].index);
+  }
   if (a.visible == nullptr) {
     if (i < n) {
-      tiles[i] = SeenBy(a, batch.of[i], batch.positions[batch.of[i].index], batch.of[i].tokens - 1);
+      tiles[i] = SeenBy(a, batch.of[i], shares.position[i], batch.of[i].tokens - 1);
     }
   } else {
-    for (int s = warp; s < n; s += W) {
+    for (int s = warp; s < n; s += blockDim.x / 32) {
       int most = 0;
       for (int token = lane; token < batch.of[s].tokens; token += 32) {
         most = max(most, SeenBy(a, batch.of[s], 0, token));
@@ -181,9 +204,9 @@ __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& b
   if (i < kBatchSequences) {
     int mine = 0;
     if (i < n) {
-      const int of = max(1, (tiles[i] + W * kCacheBlock - 1) / (W * kCacheBlock));
+      const int of = max(1, (tiles[i] + tile_rows - 1) / tile_rows);
       tiles[i] = of;
-      mine = (batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * (of + kUnitCost);
+      mine = (batch.first_item[i + 1] - batch.first_item[i]) * a.cache.kv_heads * (of + unit_cost);
     }
     sum = mine;
 #pragma unroll
@@ -208,51 +231,137 @@ __device__ __forceinline__ void ShareOut(const AttendArgs& a, const BatchArgs& b
   __syncthreads();
 }
 
+// The blocks' stretches of the whole cost: one more for the first `more` of them. A unit's own
+// cost comes ahead of its tiles: a block whose stretch ends within it has no part of the unit.
+struct Stretches {
+  int blocks, each, more;
+  __device__ __forceinline__ Stretches(int all, int least, int most) : blocks(min(most, max(all / least, 1))) {
+    each = all / blocks;
+    more = all - each * blocks;
+  }
+  __device__ __forceinline__ int start_of(int block) const { return each * block + min(block, more); }
+  __device__ __forceinline__ int owner_of(int at) const {     // the block whose stretch it is in
+    const int split = (each + 1) * more;
+    return at < split ? at / (each + 1) : more + (at - split) / each;
+  }
+};
+// The unit that `at` of the whole cost is of.
+struct Unit {
+  int sequence, tiles;
+  int start;      // of its tiles
+  int chunk, kh;
+  int number;     // of all units of the batch
+  __device__ __forceinline__ Unit(const BatchArgs& batch, const Shares& shares, int kv_heads, int unit_cost, int at) {
+    const int sequences = batch.sequences;
+    int low = 0, high = sequences - 1;
+    while (low < high) {
+      const int mid = (low + high + 1) / 2;
+      if (shares.ahead[mid] <= at) {
+        low = mid;
+      } else {
+        high = mid - 1;
+      }
+    }
+    sequence = low;
+    tiles = shares.tiles[low];
+    const int unit = (at - shares.ahead[low]) / (tiles + unit_cost);
+    start = shares.ahead[low] + unit * (tiles + unit_cost) + unit_cost;
+    chunk = unit / kv_heads;
+    kh = unit - chunk * kv_heads;
+    number = batch.first_item[low] * kv_heads + unit;
+  }
+};
+__device__ __forceinline__ Task TaskOf(const AttendArgs& a, const BatchArgs& batch, const Shares& shares, const Unit& unit, int rows) {
+  Task task;
+  task.e = batch.of[unit.sequence];
+  task.row0 = unit.chunk * rows;
+  task.rows = min(rows, task.e.tokens * a.group - task.row0);
+  task.position = shares.position[unit.sequence];
+  return task;
+}
+// Where a block's part of a unit starts, in rows: of the one that it goes on with, or begins.
+__device__ __forceinline__ size_t PartOf(int block, bool begins, int rows) { return (static_cast<size_t>(block) * 2 + (begins ? 1 : 0)) * rows; }
+// The call's query row of a task's row r: token and head.
+struct QueryRow {
+  int64_t token;
+  int head;
+  QueryRow() = default;
+  __device__ __forceinline__ QueryRow(const AttendArgs& a, const Task& task, int kh, int r) {
+    const int flat = task.row0 + r, t = flat / a.group;
+    token = static_cast<int64_t>(task.e.row) + t;
+    head = kh * a.group + flat - t * a.group;
+  }
+};
+// Four dimensions of a row of the output, gated; a row that saw nothing is zero.
+__device__ __forceinline__ void Finish(const AttendArgs& a, const QueryRow& q, int f, float4 v, float sum, bool sees) {
+  float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (a.gate != nullptr) {
+    const float* gate = a.gate + q.token * a.gate_token_stride + q.head * a.gate_head_stride + 4 * f;
+    if (a.whole) {
+      g = *reinterpret_cast<const float4*>(gate);
+    } else {
+      g = make_float4(gate[0], gate[1], gate[2], gate[3]);
+    }
+  }
+  const float by = 1.f / sum;
+  float4 o = make_float4(v.x * by, v.y * by, v.z * by, v.w * by);
+  if (a.gate != nullptr) {
+    o.x *= SigmoidDev(g.x), o.y *= SigmoidDev(g.y), o.z *= SigmoidDev(g.z), o.w *= SigmoidDev(g.w);
+  }
+  if (!sees) {
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float* out = a.out + q.token * a.out_token_stride + q.head * a.out_head_stride + 4 * f;
+  if (a.whole) {
+    *reinterpret_cast<float4*>(out) = o;
+  } else {
+    out[0] = o.x, out[1] = o.y, out[2] = o.z, out[3] = o.w;
+  }
+}
+// What the weights need of a row.
+__device__ __forceinline__ void Note(const AttendArgs& a, const QueryRow& q, float most, float sum) {
+  if (a.finals != nullptr) {
+    reinterpret_cast<float2*>(a.finals)[q.token * a.heads + q.head] = make_float2(most, 1.f / sum);
+  }
+}
+
 // Grid: resident blocks.
-template <typename Format, int NS, int RT, int W>
-__global__ void __launch_bounds__(32 * W, (Shape<NS, RT, W>::kBlocks))
+template <typename Format, int NS, int RT>
+__global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
-  using S = Shape<NS, RT, W>;
-  constexpr int kWarps = W, kThreads = S::kThreads, kTile = S::kTile;
+  using S = Shape<NS, RT>;
+  constexpr int kTile = S::kTile;
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores
   __shared__ int row_seen[8 * RT];
   __shared__ __align__(8) float block_top[2][kWarps][8 * RT];    // what a block's weights are taken against
-  __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT];
-  __shared__ float final_total[8 * RT];
-  __shared__ int tiles_of[kBatchSequences];
-  __shared__ int cost_ahead[kBatchSequences + 1];
-  __shared__ int is_last;
+  __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT], row_total[8 * RT];
+  __shared__ Shares shares;
   __shared__ __align__(16) uint4 nothing;        // a piece of zeros
-  __shared__ __align__(8) uint64_t bars[W][S::kSlots];
-  if (threadIdx.x < W * S::kSlots) {
+  __shared__ __align__(8) uint64_t bars[kWarps][S::kSlots];
+  if (threadIdx.x < kWarps * S::kSlots) {
     MbarInit(SharedAddress(&bars[0][0] + threadIdx.x), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x == 0) {
     nothing = make_uint4(0, 0, 0, 0);
   }
-  GridLaunchDependents();
+  // (The second kernel reads the inputs as soon as all blocks of this one have come so far.)
   GridDependencyWait();
+  GridLaunchDependents();
   const CacheView& c = a.cache;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / NS, member = warp % NS;
   const int g = lane >> 2, t = lane & 3;
-  ShareOut<W>(a, batch, tiles_of, cost_ahead);
-  const int all = cost_ahead[batch.sequences];
-  const int blocks = min(static_cast<int>(gridDim.x), max(all / kLeastCost, 1));
-  if (blockIdx.x >= blocks) {
+  ShareOut(a, batch, kTile, S::kUnitCost, shares);
+  const Stretches stretches(shares.ahead[batch.sequences], S::kGroups, gridDim.x);   // a tile a group at least
+  if (threadIdx.x == 0 && !a.by_unit) {
+    a.cuts[blockIdx.x].parts = 0;      // unless it begins a unit that others have parts of
+  }
+  if (blockIdx.x >= stretches.blocks) {
     return;
   }
-  // A block's stretch: one more for the first `more` of them. A unit's cost comes ahead of its
-  // tiles: a block whose stretch ends within it has no part of the unit.
-  const int each = all / blocks, more = all - each * blocks;
-  const auto start_of = [&](int block) { return each * block + min(block, more); };
-  const auto owner_of = [&](int at) {     // the block whose stretch it is in
-    const int split = (each + 1) * more;
-    return at < split ? at / (each + 1) : more + (at - split) / each;
-  };
-  const int begin = start_of(blockIdx.x), end = start_of(blockIdx.x + 1);
+  const int begin = stretches.start_of(blockIdx.x), end = stretches.start_of(blockIdx.x + 1);
 
   const auto ring_of = [&](int w) { return raw + w * (S::kSlots * S::kSlot); };
   uint8_t* const ring = ring_of(warp);
@@ -284,31 +393,15 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 
 #pragma unroll 1
   for (int from = begin; from < end;) {
-    // ---- the unit that this is of
-    int low = 0, high = batch.sequences - 1;
-    while (low < high) {
-      const int mid = (low + high + 1) / 2;
-      if (cost_ahead[mid] <= from) {
-        low = mid;
-      } else {
-        high = mid - 1;
-      }
-    }
-    const int tiles = tiles_of[low];
-    const int unit = (from - cost_ahead[low]) / (tiles + kUnitCost);
-    const int unit_start = cost_ahead[low] + unit * (tiles + kUnitCost) + kUnitCost;   // of its tiles
-    const int first_tile = max(from - unit_start, 0);
-    const int last_tile = min(end - unit_start, tiles);
-    from = unit_start + tiles;
+    const Unit unit(batch, shares, c.kv_heads, S::kUnitCost, from);
+    const int first_tile = max(from - unit.start, 0);
+    const int last_tile = min(end - unit.start, unit.tiles);
+    from = unit.start + unit.tiles;
     if (last_tile <= first_tile) {
       continue;
     }
-    const int chunk = unit / c.kv_heads, kh = unit - chunk * c.kv_heads;
-    Task task;
-    task.e = batch.of[low];
-    task.row0 = chunk * 8 * RT;
-    task.rows = min(8 * RT, task.e.tokens * a.group - task.row0);
-    task.position = batch.positions[task.e.index];
+    const int kh = unit.kh;
+    const Task task = TaskOf(a, batch, shares, unit, 8 * RT);
     if (threadIdx.x < 8 * RT) {
       const int r = min(static_cast<int>(threadIdx.x), task.rows - 1);
       row_seen[threadIdx.x] = SeenBy(a, task.e, task.position, (task.row0 + r) / a.group);
@@ -328,12 +421,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     // nobody sees is not copied)
     const uint8_t* const keys_from = BlocksOf(c, 0, of_head);
     const uint8_t* const values_from = BlocksOf(c, 1, of_head);
-    int next_tile = first_tile;
+    int next_tile = first_tile + group;
     bool next_values = false;
     auto load = [&]() {
       if (next_tile < end_tile) {
         if (lane == 0) {
-          const int block = next_tile * kWarps + warp;
+          const int block = next_tile * NS + member;
           const uint32_t bar = SharedAddress(&bars[warp][fill_slot]);
           if (block * kCacheBlock < length) {
             MbarArriveExpectTx(bar, block_bytes);
@@ -343,7 +436,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             MbarArrive(bar);
           }
         }
-        next_tile += next_values;
+        next_tile += next_values ? S::kGroups : 0;
         next_values = !next_values;
         fill_slot = fill_slot + 1 == S::kSlots ? 0 : fill_slot + 1;
       }
@@ -354,26 +447,34 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     }
 
     // ---- the queries: every fourth row to a warp, in the order of the B operands
-#pragma unroll 2
-    for (int r = warp; r < 8 * RT; r += kWarps) {
-      const bool there = r < task.rows;
-      const int flat = task.row0 + (there ? r : 0);
-      const int token = flat / a.group, head = kh * a.group + flat % a.group;
-      const float* row = a.queries + (static_cast<int64_t>(task.e.row) + token) * a.query_token_stride + head * a.query_head_stride;
-      constexpr int kTimes = (16 * NS + 31) / 32;
-      float4 x[kTimes];
-      uint32_t top = 0;
+    constexpr int kTimes = (16 * NS + 31) / 32;
+    constexpr int kEach = 8 * RT / kWarps;
+    float4 rows_in[kEach][kTimes];
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const bool there = warp + kWarps * n < task.rows;
+      const QueryRow q(a, task, kh, there ? warp + kWarps * n : 0);
+      const float* row = a.queries + q.token * a.query_token_stride + q.head * a.query_head_stride;
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
         const int f = lane + 32 * i;
-        x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        rows_in[n][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (there && 4 * f < c.head_dim) {
           if (a.whole) {
-            x[i] = *reinterpret_cast<const float4*>(row + 4 * f);
+            rows_in[n][i] = *reinterpret_cast<const float4*>(row + 4 * f);
           } else {
-            x[i] = make_float4(row[4 * f], row[4 * f + 1], row[4 * f + 2], row[4 * f + 3]);
+            rows_in[n][i] = make_float4(row[4 * f], row[4 * f + 1], row[4 * f + 2], row[4 * f + 3]);
           }
         }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const int r = warp + kWarps * n;
+      const float4(&x)[kTimes] = rows_in[n];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kTimes; ++i) {
         top = max(max(top, __float_as_uint(x[i].x) & 0x7FFFFFFFu), __float_as_uint(x[i].y) & 0x7FFFFFFFu);
         top = max(max(top, __float_as_uint(x[i].z) & 0x7FFFFFFFu), __float_as_uint(x[i].w) & 0x7FFFFFFFu);
       }
@@ -461,8 +562,10 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       constexpr int RA = decltype(groups)::value;
       int parity = 0;
 #pragma unroll 1
-      for (int tile = first_tile; tile < end_tile; ++tile) {
-        wait_for(warp);
+      for (int tile = first_tile + group; tile < end_tile; tile += S::kGroups) {
+        if ((tile * NS + member) * kCacheBlock < length) {
+          wait_for(warp);
+        }
         // Scores of this warp's block.
         const uint8_t* keys = ring + slot * S::kSlot;
         next_slot();
@@ -471,7 +574,14 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           const uint8_t* at = keys + key_place + 1024 * seg + more;
           return *reinterpret_cast<const uint4*>(4 * seg + t < pieces ? at : reinterpret_cast<const uint8_t*>(&nothing));
         };
-        if constexpr (Format::kWhole) {
+        // (A block behind the last row that is seen was not copied, and weighs nothing.)
+        const bool there = (tile * NS + member) * kCacheBlock < length;
+        if (!there) {
+#pragma unroll
+          for (int rt = 0; rt < RA; ++rt) {
+            s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
+          }
+        } else if constexpr (Format::kWhole) {
           int d[RA][3][4];      // by the queries' digits
 #pragma unroll
           for (int rt = 0; rt < RA; ++rt) {
@@ -538,7 +648,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           }
         }
         const float key_scale = *reinterpret_cast<const float*>(keys + codes_bytes);
-        const int r0 = (tile * kWarps + warp) * kCacheBlock + g;
+        const int r0 = (tile * NS + member) * kCacheBlock + g;
         const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
         uint4 p[RA];             // high pair of rows 0-7, of 8-15; low pairs
         float sum[RA][2];        // of this lane's weights
@@ -631,21 +741,25 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         // This warp's dimensions of the group's blocks.
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
+          const int block = tile * NS + b;
+          if (block * kCacheBlock >= length) {
+            break;
+          }
           wait_for(group * NS + b);
           uint8_t* values = ring_of(group * NS + b) + slot * S::kSlot;
           if constexpr (Format::kHasNan) {
             // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
-            // others, whose weight of 0 times NaN would: where some do not see all rows of a tile, such
-            // values are put into the sums by hand and taken out of the tile.
-            if (hides) {
+            // others, whose weight of 0 times NaN would: where some do not see all rows of a block, such
+            // values are put into the sums by hand and taken out of the block.
+            if ((block + 1) * kCacheBlock > least) {
               const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
               // This warp's pieces: 64 words each.
               uint32_t* const words = reinterpret_cast<uint32_t*>(values) + 256 * member;
               const int count = 64 * min(4, pieces - 4 * member);
               uint32_t found = 0;
-#pragma unroll 1
-              for (int i = lane; i < count; i += 32) {
-                found |= marks(words[i]);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                found |= lane + 32 * i < count ? marks(words[lane + 32 * i]) : 0;
               }
               if (__any_sync(0xFFFFFFFFu, found != 0)) {
 #pragma unroll
@@ -657,7 +771,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 #pragma unroll 1
                     for (int r = kCacheBlock - 1; r >= 0; --r) {
                       const uint8_t code = values[PieceAt(1, r, value_piece) + dim % 16];
-                      row = (code & 0x7F) == 0x7F ? (tile * kWarps + group * NS + b) * kCacheBlock + r : row;
+                      row = (code & 0x7F) == 0x7F ? block * kCacheBlock + r : row;
                     }
 #pragma unroll
                     for (int rt = 0; rt < RA; ++rt) {
@@ -677,10 +791,10 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             }
           }
           // (Read ahead of the values, which the products wait for: the slot is given back behind
-          // those. A block that was not copied adds nothing, whatever stands there.)
+          // those.)
           float by;
           asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(SharedAddress(values + codes_bytes)) : "memory");
-          by = (tile * kWarps + group * NS + b) * kCacheBlock < length ? by * (1.f / kProbScale) : 0.f;
+          by *= 1.f / kProbScale;
           float each[RA][2];
 #pragma unroll
           for (int rt = 0; rt < RA; ++rt) {
@@ -778,12 +892,11 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         }
       }
     }
-    __syncthreads();
-    // A row's maximum and sum, and the factor of a group's part.
-    const auto factor_of = [&](int r, int of, float most) {
-      return group_top[of][r] == most ? 1.f : exp2f(group_top[of][r] - most);
-    };
-    const auto row_stats = [&](int r) {
+    const bool alone = first_tile == 0 && last_tile == unit.tiles;
+    const size_t part = PartOf(blockIdx.x, first_tile == 0, 8 * RT);
+    if (threadIdx.x < 8 * RT) {
+      // A row's maximum and sum, and the factors of the groups' parts.
+      const int r = threadIdx.x;
       float most = -INFINITY;
 #pragma unroll
       for (int of = 0; of < S::kGroups; ++of) {
@@ -791,154 +904,144 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        sum += warp_total[w][r] * factor_of(r, w / NS, most);
-      }
-      return make_float2(most, sum);
-    };
-    const int fours = c.head_dim / 4;
-    // Four dimensions of a row of the output, gated; a row that saw nothing is zero.
-    auto finish = [&](int r, int f, float4 v, float sum, int sees) {
-      const int flat = task.row0 + r;
-      const int64_t token = static_cast<int64_t>(task.e.row) + flat / a.group;
-      const int head = kh * a.group + flat % a.group;
-      const float by = 1.f / sum;
-      float o[4] = {v.x * by, v.y * by, v.z * by, v.w * by};
-      if (a.gate != nullptr) {
-        const float* gate = a.gate + token * a.gate_token_stride + head * a.gate_head_stride + 4 * f;
+      for (int of = 0; of < S::kGroups; ++of) {
+        const float by = group_top[of][r] == most ? 1.f : exp2f(group_top[of][r] - most);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[i] *= SigmoidDev(gate[i]);
+        for (int w = 0; w < NS; ++w) {
+          sum += warp_total[of * NS + w][r] * by;
+        }
+        group_top[of][r] = by;      // from now on the part's factor
+      }
+      row_total[r] = sum;
+      if (r < task.rows) {
+        if (alone) {
+          Note(a, QueryRow(a, task, kh, r), most, sum);
+        } else {
+          // (A row that sees nothing is told by its sum, whatever its parts.)
+          reinterpret_cast<float2*>(a.stats)[part + r] = make_float2(most, row_seen[r] > 0 ? sum : -1.f);
         }
       }
-      float* out = a.out + token * a.out_token_stride + head * a.out_head_stride + 4 * f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        out[i] = sees > 0 ? o[i] : 0.f;
-      }
-    };
-    auto note = [&](int r, float most, float sum) {     // for the weights
-      if (a.finals != nullptr) {
-        const int flat = task.row0 + r;
-        const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
-        a.finals[2 * at] = most;
-        a.finals[2 * at + 1] = 1.f / sum;
-      }
-    };
-    const bool alone = first_tile == 0 && last_tile == tiles;
-    // A block's part of a unit that others have parts of too: of the one that it goes on with, or
-    // of the one that it begins.
-    const auto part_of = [&](int block, bool begins) { return (static_cast<size_t>(block) * 2 + (begins ? 1 : 0)) * 8 * RT; };
-    const size_t part = part_of(blockIdx.x, first_tile == 0);
+    }
+    __syncthreads();
+    const int fours = c.head_dim / 4;
+#pragma unroll 4
     for (int at = threadIdx.x; at < task.rows * fours; at += kThreads) {
-      const int r = at / fours, f = at % fours;
-      const float2 stats = row_stats(r);
+      const int r = at / fours, f = at - r * fours;
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int of = 0; of < S::kGroups; ++of) {
         const float4 v = *reinterpret_cast<const float4*>(join + (of * 8 * RT + r) * S::kRowBytes + 4 * f);
-        const float by = factor_of(r, of, stats.x);
+        const float by = group_top[of][r];
         sum.x = fmaf(v.x, by, sum.x), sum.y = fmaf(v.y, by, sum.y), sum.z = fmaf(v.z, by, sum.z), sum.w = fmaf(v.w, by, sum.w);
       }
       if (alone) {
-        finish(r, f, sum, stats.y, row_seen[r]);
+        Finish(a, QueryRow(a, task, kh, r), f, sum, row_total[r], row_seen[r] > 0);
       } else {
-        __stcg(reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim) + f, sum);
+        reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim)[f] = sum;
       }
     }
-    if (threadIdx.x < task.rows) {
-      const float2 stats = row_stats(threadIdx.x);
-      if (alone) {
-        note(threadIdx.x, stats.x, stats.y);
-      } else {
-        __stcg(reinterpret_cast<float2*>(a.stats) + part + threadIdx.x, stats);
-      }
-    }
-    if (alone) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rings are written by copies again
-      __syncthreads();
-      continue;
-    }
-    const int first_block = owner_of(unit_start), count = owner_of(unit_start + tiles - 1) - first_block + 1;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      is_last = atomicAdd(a.arrived + first_block, 1u) == static_cast<unsigned>(count - 1);
-    }
-    __syncthreads();
-    if (is_last) {
-      __threadfence();
-      if (threadIdx.x == 0) {
-        a.arrived[first_block] = 0;
-      }
-      // ---- the blocks' parts together: their factors in shared memory, then the sums
-      float* by = reinterpret_cast<float*>(raw);     // [row][count]
-      const auto part_at = [&](int i) { return part_of(first_block + i, i == 0); };
-      for (int r = warp; r < task.rows; r += kWarps) {
-        const float2* stats = reinterpret_cast<const float2*>(a.stats) + r;
-        float most = -INFINITY;
-        for (int i = lane; i < count; i += 32) {
-          most = fmaxf(most, __ldcg(stats + part_at(i)).x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-        }
-        float sum = 0.f;
-        for (int i = lane; i < count; i += 32) {
-          const float2 s = __ldcg(stats + part_at(i));
-          const float f = s.x == most ? 1.f : exp2f(s.x - most);
-          by[r * count + i] = f;
-          sum += s.y * f;
-        }
-        sum = WarpSum(sum);
-        if (lane == 0) {
-          final_total[r] = sum;
-          note(r, most, sum);
-        }
-      }
-      // Where there are more threads than outputs, several take a part of the parts each.
-      const int outputs = task.rows * fours;
-      const int takers = outputs >= kThreads ? 1 : min(kThreads / outputs, 8);
-      float4* partial = reinterpret_cast<float4*>(by + 8 * RT * S::kBlocks * kMostSms);    // [taker][output]
-      __syncthreads();
-      for (int at = threadIdx.x; at < outputs * takers; at += kThreads) {
-        const int taker = at / outputs, r = (at - taker * outputs) / fours, f = (at - taker * outputs) % fours;
-        const int i_first = count * taker / takers, i_end = count * (taker + 1) / takers;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = i_first; i0 < i_end; i0 += 8) {
-          float4 v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = i0 + i < i_end ? __ldcg(reinterpret_cast<const float4*>(a.sums + (part_at(i0 + i) + r) * c.head_dim) + f)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float f2 = i0 + i < i_end ? by[r * count + i0 + i] : 0.f;
-            sum.x = fmaf(v[i].x, f2, sum.x), sum.y = fmaf(v[i].y, f2, sum.y), sum.z = fmaf(v[i].z, f2, sum.z), sum.w = fmaf(v[i].w, f2, sum.w);
-          }
-        }
-        if (takers == 1) {
-          finish(r, f, sum, final_total[r], row_seen[r]);
-        } else {
-          partial[at] = sum;
-        }
-      }
-      if (takers > 1) {
-        __syncthreads();
-        for (int at = threadIdx.x; at < outputs; at += kThreads) {
-          float4 sum = partial[at];
-          for (int i = 1; i < takers; ++i) {
-            const float4 v = partial[i * outputs + at];
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-          }
-          finish(at / fours, at % fours, sum, final_total[at / fours], row_seen[at / fours]);
-        }
-      }
+    if (first_tile == 0 && threadIdx.x == 0 && (a.by_unit || !alone)) {
+      a.cuts[a.by_unit ? unit.number : static_cast<int>(blockIdx.x)] = {
+          static_cast<int>(blockIdx.x), alone ? 0 : stretches.owner_of(unit.start + unit.tiles - 1) - static_cast<int>(blockIdx.x) + 1,
+          task.rows, task.e.row, kh * a.group, task.row0};
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the rings are written by copies again
     __syncthreads();
+  }
+}
+
+// The units that several blocks have parts of: grid (cuts, rows of a unit). One block a query
+// row: the parts' factors, then their sums, groups of threads taking a part of the parts each.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads)
+JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
+  __shared__ float factor[kMostBlocks];
+  __shared__ float of_warp[kJoinThreads / 32][2];
+  __shared__ float4 partial[kJoinThreads];
+  GridLaunchDependents();
+  const CacheView& c = a.cache;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y;
+  GridDependencyWait();
+  const Cut cut = a.cuts[blockIdx.x];
+  const int first_block = cut.first, count = cut.parts;
+  if (r >= cut.rows || count == 0) {
+    return;
+  }
+  const auto part_at = [&](int i) { return PartOf(first_block + i, i == 0, rows) + r; };
+  const int fours = c.head_dim / 4;
+  const int takers = kJoinThreads / fours;
+  const int taker = threadIdx.x / fours, f = threadIdx.x - taker * fours;
+  const int i_first = count * taker / takers, i_end = taker < takers ? count * (taker + 1) / takers : 0;
+  // The first sums are on their way while the statistics are looked at.
+  constexpr int kAhead = 16;
+  float4 v[kAhead];
+  const auto get = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      v[i] = i0 + i < i_end ? __ldcg(reinterpret_cast<const float4*>(a.sums + part_at(i0 + i) * c.head_dim) + f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  get(i_first);
+  float most = -INFINITY;
+  for (int i = threadIdx.x; i < count; i += kJoinThreads) {
+    factor[i] = __ldcg(reinterpret_cast<const float2*>(a.stats) + part_at(i)).x;
+    most = fmaxf(most, factor[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  }
+  if (lane == 0) {
+    of_warp[warp][0] = most;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    most = fmaxf(most, of_warp[w][0]);
+  }
+  float total = 0.f;
+  for (int i = threadIdx.x; i < count; i += kJoinThreads) {
+    const float by = factor[i] == most ? 1.f : exp2f(factor[i] - most);
+    factor[i] = by;
+    total += __ldcg(reinterpret_cast<const float2*>(a.stats) + part_at(i)).y * by;
+  }
+  total = WarpSum(total);
+  if (lane == 0) {
+    of_warp[warp][1] = total;
+  }
+  __syncthreads();
+  total = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    total += of_warp[w][1];
+  }
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = i_first; i0 < i_end; i0 += kAhead) {
+    if (i0 > i_first) {
+      get(i0);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float by = i0 + i < i_end ? factor[i0 + i] : 0.f;
+      sum.x = fmaf(v[i].x, by, sum.x), sum.y = fmaf(v[i].y, by, sum.y), sum.z = fmaf(v[i].z, by, sum.z), sum.w = fmaf(v[i].w, by, sum.w);
+    }
+  }
+  partial[threadIdx.x] = sum;
+  __syncthreads();
+  QueryRow q;
+  q.token = cut.token + (cut.first_flat + r) / a.group;
+  q.head = cut.head + (cut.first_flat + r) % a.group;
+  const bool sees = !(total < 0.f);
+  if (taker == 0) {
+    for (int i = 1; i < takers; ++i) {
+      const float4 w = partial[i * fours + f];
+      sum.x += w.x, sum.y += w.y, sum.z += w.z, sum.w += w.w;
+    }
+    Finish(a, q, f, sum, total, sees);
+  }
+  if (threadIdx.x == 0) {
+    Note(a, q, most, total);
   }
 }
 
@@ -974,54 +1077,46 @@ WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batc
   c.weights[(static_cast<size_t>(e.slot) * c.kv_heads + kh) * c.capacity + row] += sum;
 }
 
-// Scratch of the blocks of threads that a device holds at once, four an SM at most: a counter
-// each; two units' rows times dimensions, 8 rt * 64 ns with rt, ns <= 4 (two blocks an SM then; one
-// half as large has three or four), and two statistics a row.
+// Scratch of the blocks of threads that a device holds at once, four an SM at most: two units'
+// rows times dimensions, 8 rt * 64 ns with rt, ns <= 4 (two blocks an SM then; one half as large
+// has three or four), and two statistics a row.
 int Sms(const gufo_cuda_ctx* ctx) { return ctx->sm_count < kMostSms ? ctx->sm_count : kMostSms; }
-size_t ArrivedBytes(int sms) { return (static_cast<size_t>(4 * sms) * sizeof(unsigned) + 255) / 256 * 256; }
 constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
 constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
-size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * (kPartialFloats + kStatsFloats) * sizeof(float); }
+size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * ((kPartialFloats + kStatsFloats) * sizeof(float) + 4 * 32); }
 
-template <typename Format, int NS, int RT, int W>
-int LaunchAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b) {
-  using S = Shape<NS, RT, W>;
+template <typename Format, int NS, int RT>
+int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t units, int rows) {
+  using S = Shape<NS, RT>;
+  const int blocks = Sms(ctx) * S::kBlocks;
+  a.by_unit = units <= blocks;
   static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
                 "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
   if (ctx->device >= 64 || !configured[ctx->device].load()) {
-    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     if (ctx->device < 64) {
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT, W>, dim3(Sms(ctx) * S::kBlocks), dim3(S::kThreads), S::kBytes,
-                                 ctx->stream, 1, a, b));
-  ctx->launches.fetch_add(1);
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(blocks), dim3(kThreads), S::kBytes, ctx->stream, 1, a, b));
+  GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel, dim3(a.by_unit ? static_cast<int>(units) : blocks, rows), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
+  ctx->launches.fetch_add(2);
   return GUFO_CUDA_OK;
 }
 
-// Few units: one block of as many warps as registers and shared memory hold, so that a unit has
-// few parts. Many: small blocks, several of which an SM holds, so that one's queries and join
-// pass under another's tiles.
-template <typename Format, int NS, int RT>
-int PickWarps(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units) {
-  constexpr int kMany = RT == 1 ? 16 : RT == 2 ? (NS == 1 ? 16 : 12) : NS == 1 ? 12 : 8;
-  return units < Sms(ctx) ? LaunchAttend<Format, NS, RT, kMany>(ctx, a, b) : LaunchAttend<Format, NS, RT, kFewWarps>(ctx, a, b);
-}
-
 template <typename Format>
-int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units, int ns, int rt) {
+int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units, int rows, int ns, int rt) {
   switch (ns * 8 + rt) {
-    case 8 + 1: return PickWarps<Format, 1, 1>(ctx, a, b, units);
-    case 8 + 2: return PickWarps<Format, 1, 2>(ctx, a, b, units);
-    case 8 + 4: return PickWarps<Format, 1, 4>(ctx, a, b, units);
-    case 16 + 1: return PickWarps<Format, 2, 1>(ctx, a, b, units);
-    case 16 + 2: return PickWarps<Format, 2, 2>(ctx, a, b, units);
-    case 16 + 4: return PickWarps<Format, 2, 4>(ctx, a, b, units);
-    case 32 + 1: return PickWarps<Format, 4, 1>(ctx, a, b, units);
-    case 32 + 2: return PickWarps<Format, 4, 2>(ctx, a, b, units);
-    default: return PickWarps<Format, 4, 4>(ctx, a, b, units);
+    case 8 + 1: return LaunchAttend<Format, 1, 1>(ctx, a, b, units, rows);
+    case 8 + 2: return LaunchAttend<Format, 1, 2>(ctx, a, b, units, rows);
+    case 8 + 4: return LaunchAttend<Format, 1, 4>(ctx, a, b, units, rows);
+    case 16 + 1: return LaunchAttend<Format, 2, 1>(ctx, a, b, units, rows);
+    case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b, units, rows);
+    case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b, units, rows);
+    case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b, units, rows);
+    case 32 + 2: return LaunchAttend<Format, 4, 2>(ctx, a, b, units, rows);
+    default: return LaunchAttend<Format, 4, 4>(ctx, a, b, units, rows);
   }
 }
 
@@ -1049,7 +1144,7 @@ int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle,
   if (accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / cache->c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend_scratch: too many query rows for one call");
   }
-  *bytes = gufo::ArrivedBytes(gufo::Sms(ctx)) + gufo::PartialBytes(gufo::Sms(ctx)) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
+  *bytes = gufo::PartialBytes(gufo::Sms(ctx)) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
   return GUFO_CUDA_OK;
 }
 
@@ -1082,7 +1177,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_attend: null pointer");
   }
   const size_t rows = static_cast<size_t>(p->heads) * tokens;
-  const size_t own = gufo::ArrivedBytes(gufo::Sms(ctx)) + gufo::PartialBytes(gufo::Sms(ctx));
+  const size_t own = gufo::PartialBytes(gufo::Sms(ctx));
   if (p->accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / c.capacity) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
   }
@@ -1105,10 +1200,11 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   a.heads = p->heads;
   a.group = p->heads / c.kv_heads;
   a.scale = (p->scale != 0.f ? p->scale : 1.0f / sqrtf(static_cast<float>(c.head_dim))) * gufo::kLog2e;
-  a.whole = reinterpret_cast<uintptr_t>(p->queries) % 16 == 0 && ((p->query_token_stride | p->query_head_stride) & 3) == 0;
+  a.whole = ((reinterpret_cast<uintptr_t>(p->queries) | reinterpret_cast<uintptr_t>(p->gate) | reinterpret_cast<uintptr_t>(p->out)) & 15) == 0 &&
+            ((p->query_token_stride | p->query_head_stride | p->gate_token_stride | p->gate_head_stride | p->out_token_stride |
+              p->out_head_stride) & 3) == 0;
   uint8_t* scratch = static_cast<uint8_t*>(p->scratch);
-  a.arrived = reinterpret_cast<unsigned*>(scratch);
-  a.sums = reinterpret_cast<float*>(scratch + gufo::ArrivedBytes(gufo::Sms(ctx)));
+  a.sums = reinterpret_cast<float*>(scratch);
   if (p->accumulate != 0) {
     a.finals = reinterpret_cast<float*>(scratch + own);
     a.scores = a.finals + 2 * rows;
@@ -1122,6 +1218,8 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   }
   const int64_t rows_each = static_cast<int64_t>(most) * a.group;
   a.stats = a.sums + static_cast<size_t>(gufo::Sms(ctx)) * gufo::kPartialFloats;
+  a.cuts = reinterpret_cast<gufo::Cut*>(a.stats + static_cast<size_t>(gufo::Sms(ctx)) * gufo::kStatsFloats);
+  static_assert(sizeof(gufo::Cut) <= 32, "the scratch has 32 bytes a block for it");
   const int rt = rows_each <= 8 ? 1 : rows_each <= 16 ? 2 : 4;
   if (tokens * a.group / (8 * rt) + batch->sequences > 65535) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
@@ -1132,11 +1230,12 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
       *batch, [&](int n) { return static_cast<int>((static_cast<int64_t>(n) * group + 8 * rt - 1) / (8 * rt)); },
       [&](const gufo::BatchArgs& b, int items) -> int {
         const int64_t units = static_cast<int64_t>(items) * c.kv_heads;
-        if (units * (c.capacity / (gufo::kFewWarps * gufo::kCacheBlock) + 1 + gufo::kUnitCost) > INT32_MAX) {
+        const int rows = rows_each < 8 * rt ? static_cast<int>(rows_each) : 8 * rt;
+        if (units * (c.capacity / gufo::kCacheBlock + 1 + gufo::kMostUnitCost) > INT32_MAX) {
           return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
         }
-        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, units, ns, rt)
-                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, units, ns, rt);
+        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, units, rows, ns, rt)
+                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, units, rows, ns, rt);
         if (run != GUFO_CUDA_OK || a.scores == nullptr) {
           return run;
         }
