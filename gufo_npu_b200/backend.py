@@ -76,18 +76,18 @@ def _ptr(buf) -> int:
     return buf.data_ptr()
 
 
-def check_rows(what: str, *tensors) -> None:
-    """fp32 device tensors [tokens, heads, head_dim] whose heads' values stand side by side."""
+def check_rows(what: str, device: int, *tensors) -> None:
+    """fp32 tensors [tokens, heads, head_dim] on the device whose heads' values stand side by side."""
     for t in tensors:
         if str(t.dtype) != "torch.float32" or t.dim() != 3 or not t.is_cuda or (t.shape[2] > 1 and t.stride(2) != 1) \
-                or t.device != tensors[0].device:
-            raise ValueError(f"{what}: rows are fp32 tensors [tokens, heads, head_dim] on one device, a head's values "
-                             "side by side")
+                or t.get_device() != device:
+            raise ValueError(f"{what}: rows are fp32 tensors [tokens, heads, head_dim] on the context's device, a head's "
+                             "values side by side")
 
 
-def check_ints(what: str, t) -> None:
-    if str(t.dtype) != "torch.int32" or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{what}: an int32 tensor on the device, its values side by side")
+def check_ints(what: str, device: int, t) -> None:
+    if str(t.dtype) != "torch.int32" or not t.is_cuda or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{what}: an int32 tensor on the context's device, its values side by side")
 
 
 def rope_params(rope_dim: int, theta: float, layout: str, scaling: str, factor: float, original_positions: float,
@@ -265,9 +265,9 @@ class Context:
     def rope_parts(self, parts: Sequence, rms_eps: float = 0.0) -> "C.Array":
         """[(x, out, norm weight or None)]: fp32 device tensors [tokens, heads, head_dim] (any token and head
         strides) as the array that rope_device takes; the caller keeps the tensors."""
-        arr = (_capi.RopeRows * len(parts))()
+        arr = (_capi.RopeRows * max(len(parts), 1))()
         for i, (x, out, norm) in enumerate(parts):
-            check_rows("rope", x, out)
+            check_rows("rope", self.device, x, out)
             if norm is not None and (norm.dtype != x.dtype or tuple(norm.shape) != (x.shape[2],) or not norm.is_contiguous()
                                      or norm.device != x.device):
                 raise ValueError("rope: a norm weight is an fp32 value for each of a head's, beside the rows")
@@ -280,11 +280,7 @@ class Context:
 
     def rope_device(self, rope: int, parts, positions) -> None:
         """Turns the rows of `parts` (rope_parts), token t by positions[t] (an int32 device tensor)."""
-        check_ints("rope", positions)
-        if positions.numel() > parts.tokens:
-            raise ValueError("rope: more positions than rows")
-        self._check(self.lib.gufo_cuda_rope_device(self.handle, rope, parts, len(parts),
-                                                   C.c_void_p(positions.data_ptr()), positions.numel()))
+        self._check(_capi.native.rope(self._address, self.device, rope, parts, parts.tokens, positions))
 
     # -- routed experts -------------------------------------------------------
     def route_device(self, router, stride: int, tokens: int, experts: int, k: int, chosen, weights,

@@ -11,14 +11,14 @@ import ctypes as C
 from typing import Optional, Sequence
 
 from . import _capi
-from .backend import Context, _DeviceArray, check_ints, check_rows
+from .backend import Context, _DeviceArray, check_ints
 
 
 class Batch:
     """Sequences of a call: slots and tokens as the library takes them, and the positions they start at."""
 
-    def __init__(self, positions, tokens: Optional[Sequence[int]], slots: Optional[Sequence[int]]):
-        check_ints("cache8", positions)
+    def __init__(self, device: int, positions, tokens: Optional[Sequence[int]], slots: Optional[Sequence[int]]):
+        check_ints("cache8", device, positions)
         n = positions.numel()
         for name, values in (("tokens", tokens), ("slots", slots)):
             if values is not None and len(values) != n:
@@ -38,9 +38,8 @@ class Scratch:
     may be in flight beside others."""
 
     def __init__(self, ctx: Context, nbytes: int):
-        self.ctx, self.bytes = ctx, nbytes
+        self.ctx, self.bytes, self.ptr = ctx, nbytes, 0
         self.ptr = ctx.malloc(nbytes)
-        ctx.memset_zero(self.ptr, nbytes)
 
     def close(self) -> None:
         if self.ptr and self.ctx.handle:
@@ -112,7 +111,7 @@ class CudaCache8:
     def batch(self, positions, tokens: Optional[Sequence[int]] = None, slots: Optional[Sequence[int]] = None) -> Batch:
         """Sequences of a call: `positions` (int32, device) rows held ahead of it, `tokens` rows each (one
         without), in `slots` (0, 1, ... without)."""
-        return Batch(positions, tokens, slots)
+        return Batch(self.ctx.device, positions, tokens, slots)
 
     def scratch(self, heads: int, tokens: int, accumulate: bool = False) -> Scratch:
         """Scratch of attend_device calls with up to `tokens` query tokens in all."""
@@ -121,61 +120,34 @@ class CudaCache8:
                                                                      int(accumulate), C.byref(nbytes)))
         return Scratch(self.ctx, nbytes.value)
 
-    def _check_kv(self, batch: Batch, *tensors) -> None:
-        check_rows("cache8", *tensors)
-        for t in tensors:
-            if tuple(t.shape) != (batch.rows, self.kv_heads, self.head_dim):
-                raise ValueError(f"cache8: rows [{batch.rows}, {self.kv_heads}, {self.head_dim}], not {list(t.shape)}")
-
     def append_device(self, batch: Batch, keys, values) -> None:
         """Writes the batch's rows, [rows, kv_heads, head_dim] each, at their positions."""
-        self._check_kv(batch, keys, values)
-        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_append_device(
-            self.ctx.handle, self.handle, C.byref(batch.args), C.c_void_p(keys.data_ptr()), keys.stride(0), keys.stride(1),
-            C.c_void_p(values.data_ptr()), values.stride(0), values.stride(1)))
+        ctx = self.ctx
+        ctx._check(_capi.native.cache8_append(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.kv_heads,
+                                              self.head_dim, keys, values))
 
     def rows_device(self, batch: Batch, keys, values) -> None:
         """What the rows of an append with this batch stand for, into contiguous [rows, kv_heads, head_dim]."""
-        self._check_kv(batch, keys, values)
-        if not (keys.is_contiguous() and values.is_contiguous()):
-            raise ValueError("cache8: rows are read into contiguous tensors")
-        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_rows_device(
-            self.ctx.handle, self.handle, C.byref(batch.args), C.c_void_p(keys.data_ptr()), C.c_void_p(values.data_ptr())))
+        ctx = self.ctx
+        ctx._check(_capi.native.cache8_rows(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.kv_heads,
+                                            self.head_dim, keys, values))
 
     def attend_device(self, batch: Batch, queries, out, scratch: Scratch, gate=None, scale: float = 0.0, visible=None,
                       accumulate: bool = False) -> None:
         """out = softmax(queries K^T scale) V [* sigmoid(gate)] for [rows, heads, head_dim] query rows. Token t of
         a sequence sees the rows up to position + t, or the first visible[...] (int32, a value per row of
         queries). `accumulate` adds what each cached row was given to `weights`."""
-        check_rows("cache8", queries, out, *([gate] if gate is not None else []))
-        heads = queries.shape[1]
-        for t in (queries, out, gate):
-            if t is not None and tuple(t.shape) != (batch.rows, heads, self.head_dim):
-                raise ValueError(f"cache8: query rows [{batch.rows}, {heads}, {self.head_dim}], not {list(t.shape)}")
-        if visible is not None:
-            check_ints("cache8", visible)
-            if visible.numel() != batch.rows:
-                raise ValueError(f"cache8: {batch.rows} query rows and {visible.numel()} numbers of rows they see")
-        args = _capi.Cache8AttendArgs(
-            heads, scale, queries.data_ptr(), queries.stride(0), queries.stride(1),
-            *((gate.data_ptr(), gate.stride(0), gate.stride(1)) if gate is not None else (None, 0, 0)),
-            out.data_ptr(), out.stride(0), out.stride(1), visible.data_ptr() if visible is not None else None,
-            int(accumulate), scratch.ptr, scratch.bytes)
-        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_attend_device(self.ctx.handle, self.handle, C.byref(batch.args),
-                                                                    C.byref(args)))
+        ctx = self.ctx
+        ctx._check(_capi.native.cache8_attend(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.head_dim,
+                                              queries, out, gate, visible, scale, accumulate, scratch.ptr, scratch.bytes))
 
     def evict_device(self, batch: Batch, budget: int, kept, first: int = 0, last: int = 0, held=None,
                      into: Optional["CudaCache8"] = None, into_slots: Optional[Sequence[int]] = None) -> None:
         """Brings the batch's sequences (their `positions` rows) down to `budget` rows: the first `first`, the
         last `last`, and the rest by weight; in place, or into another cache's slots. `kept` (int32
         [sequences, kv_heads, budget]) gets the rows that stayed, `held` (int32 [sequences]) how many."""
-        check_ints("cache8", kept)
         if tuple(kept.shape) != (batch.sequences, self.kv_heads, budget):
             raise ValueError(f"cache8: kept is [{batch.sequences}, {self.kv_heads}, {budget}], not {list(kept.shape)}")
-        if held is not None:
-            check_ints("cache8", held)
-            if held.numel() != batch.sequences:
-                raise ValueError("cache8: held has a value per sequence")
         slots = None
         if into_slots is not None:
             if len(into_slots) != batch.sequences:
@@ -183,6 +155,6 @@ class CudaCache8:
             slots = (C.c_int * batch.sequences)(*into_slots)
         if into is not None and into.ctx is not self.ctx:
             raise ValueError("cache8: both caches belong to one context")
-        self.ctx._check(self.ctx.lib.gufo_cuda_cache8_evict_device(
-            self.ctx.handle, self.handle, C.byref(batch.args), budget, first, last, C.c_void_p(kept.data_ptr()),
-            C.c_void_p(held.data_ptr()) if held is not None else None, into.handle if into is not None else 0, slots))
+        ctx = self.ctx
+        ctx._check(_capi.native.cache8_evict(ctx._address, ctx.device, self.handle, batch.args, batch.sequences, self.kv_heads,
+                                             budget, first, last, kept, held, into.handle if into is not None else 0, slots))

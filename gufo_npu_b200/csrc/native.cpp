@@ -32,6 +32,11 @@ struct Api {
   decltype(&gufo_cuda_route_device) route;
   decltype(&gufo_cuda_moe_ffn_device) moe_ffn;
   decltype(&gufo_cuda_moe_layer_device) moe_layer;
+  decltype(&gufo_cuda_rope_device) rope;
+  decltype(&gufo_cuda_cache8_append_device) cache8_append;
+  decltype(&gufo_cuda_cache8_rows_device) cache8_rows;
+  decltype(&gufo_cuda_cache8_attend_device) cache8_attend;
+  decltype(&gufo_cuda_cache8_evict_device) cache8_evict;
   decltype(&gufo_cuda_decoder_step) decoder_step;
   decltype(&gufo_cuda_decoder_step_tokens) decoder_step_tokens;
   decltype(&gufo_cuda_host_take) host_take;
@@ -432,6 +437,177 @@ PyObject* MoeLayer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+[[noreturn]] void Refuse(const char* why) {
+  PyErr_SetString(PyExc_ValueError, why);
+  throw Failed();
+}
+
+const at::Tensor& DeviceTensor(PyObject* o, int device) {
+  if (!THPVariable_Check(o)) {
+    PyErr_SetString(PyExc_TypeError, "gufo_cuda: a torch tensor is needed");
+    throw Failed();
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.get_device() != device) {
+    Refuse("gufo_cuda: tensors are on the context's device");
+  }
+  return t;
+}
+
+// fp32 rows [tokens][heads][head_dim], a head's values side by side.
+const at::Tensor& RowsOf(PyObject* o, int device, int64_t rows, int64_t heads, int64_t head_dim) {
+  const at::Tensor& t = DeviceTensor(o, device);
+  if (t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(0) != rows || t.size(1) != heads || t.size(2) != head_dim ||
+      (head_dim > 1 && t.stride(2) != 1)) {
+    PyErr_Format(PyExc_ValueError, "gufo_cuda: rows are fp32 [%lld, %lld, %lld], a head's values side by side", (long long)rows,
+                 (long long)heads, (long long)head_dim);
+    throw Failed();
+  }
+  return t;
+}
+
+int* IntsOf(PyObject* o, int device, int64_t count) {
+  const at::Tensor& t = DeviceTensor(o, device);
+  if (t.scalar_type() != at::kInt || !t.is_contiguous() || t.numel() != count) {
+    PyErr_Format(PyExc_ValueError, "gufo_cuda: %lld int32 values side by side", (long long)count);
+    throw Failed();
+  }
+  return static_cast<int*>(t.data_ptr());
+}
+
+// A ctypes structure, or array of them, used in place.
+template <typename T>
+struct InPlace {
+  explicit InPlace(PyObject* o) {
+    if (PyObject_GetBuffer(o, &view, PyBUF_SIMPLE) != 0) {
+      throw Failed();
+    }
+    if (view.len % sizeof(T) != 0 || view.len == 0) {
+      PyBuffer_Release(&view);
+      Refuse("gufo_cuda: a structure of another size");
+    }
+  }
+  ~InPlace() { PyBuffer_Release(&view); }
+  InPlace(const InPlace&) = delete;
+  InPlace& operator=(const InPlace&) = delete;
+  const T* data() const { return static_cast<const T*>(view.buf); }
+  int count() const { return static_cast<int>(view.len / sizeof(T)); }
+  Py_buffer view;
+};
+using BatchArgs = InPlace<gufo_cuda_cache8_batch>;
+
+// rope(ctx, device, rope, parts, rows, positions): positions for the first of `rows` rows
+PyObject* Rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded(n, 6, [&] {
+    gufo_cuda_ctx* ctx = Context(a[0]);
+    const long long rope = Int(a[2]);
+    const InPlace<gufo_cuda_rope_rows> parts(a[3]);
+    const at::Tensor& positions = DeviceTensor(a[5], SmallInt(a[1]));
+    if (positions.scalar_type() != at::kInt || !positions.is_contiguous() || positions.numel() > Int(a[4])) {
+      Refuse("rope: int32 positions side by side, no more than rows");
+    }
+    const int* at = static_cast<const int*>(positions.data_ptr());
+    const int tokens = static_cast<int>(positions.numel());
+    return Unlocked([&] { return api.rope(ctx, rope, parts.data(), parts.count(), at, tokens); });
+  });
+}
+
+// cache8_append(ctx, device, cache, batch, rows, kv_heads, head_dim, keys, values)
+PyObject* Cache8Append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded(n, 9, [&] {
+    gufo_cuda_ctx* ctx = Context(a[0]);
+    const int device = SmallInt(a[1]);
+    const long long cache = Int(a[2]);
+    const BatchArgs batch(a[3]);
+    const long long rows = Int(a[4]), heads = Int(a[5]), dim = Int(a[6]);
+    const at::Tensor &k = RowsOf(a[7], device, rows, heads, dim), &v = RowsOf(a[8], device, rows, heads, dim);
+    const float *keys = static_cast<const float*>(k.data_ptr()), *values = static_cast<const float*>(v.data_ptr());
+    const int64_t ks0 = k.stride(0), ks1 = k.stride(1), vs0 = v.stride(0), vs1 = v.stride(1);
+    return Unlocked([&] { return api.cache8_append(ctx, cache, batch.data(), keys, ks0, ks1, values, vs0, vs1); });
+  });
+}
+
+// cache8_rows(ctx, device, cache, batch, rows, kv_heads, head_dim, keys, values)
+PyObject* Cache8Rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded(n, 9, [&] {
+    gufo_cuda_ctx* ctx = Context(a[0]);
+    const int device = SmallInt(a[1]);
+    const long long cache = Int(a[2]);
+    const BatchArgs batch(a[3]);
+    const long long rows = Int(a[4]), heads = Int(a[5]), dim = Int(a[6]);
+    const at::Tensor &k = RowsOf(a[7], device, rows, heads, dim), &v = RowsOf(a[8], device, rows, heads, dim);
+    if (!k.is_contiguous() || !v.is_contiguous()) {
+      Refuse("cache8: rows are read into contiguous tensors");
+    }
+    float *keys = static_cast<float*>(k.data_ptr()), *values = static_cast<float*>(v.data_ptr());
+    return Unlocked([&] { return api.cache8_rows(ctx, cache, batch.data(), keys, values); });
+  });
+}
+
+// cache8_attend(ctx, device, cache, batch, rows, head_dim, queries, out, gate, visible, scale, accumulate, scratch,
+// scratch bytes); gate and visible may be None
+PyObject* Cache8Attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded(n, 14, [&] {
+    gufo_cuda_ctx* ctx = Context(a[0]);
+    const int device = SmallInt(a[1]);
+    const long long cache = Int(a[2]);
+    const BatchArgs batch(a[3]);
+    const long long rows = Int(a[4]), dim = Int(a[5]);
+    const at::Tensor& any = DeviceTensor(a[6], device);
+    if (any.dim() != 3) {
+      Refuse("cache8: query rows are [tokens, heads, head_dim]");
+    }
+    const int64_t heads = any.size(1);
+    gufo_cuda_cache8_attend_args args{};
+    args.heads = heads > INT32_MAX ? INT32_MAX : static_cast<int>(heads);
+    args.scale = Float(a[10]);
+    const at::Tensor& q = RowsOf(a[6], device, rows, heads, dim);
+    args.queries = static_cast<const float*>(q.data_ptr());
+    args.query_token_stride = q.stride(0);
+    args.query_head_stride = q.stride(1);
+    if (a[8] != Py_None) {
+      const at::Tensor& g = RowsOf(a[8], device, rows, heads, dim);
+      args.gate = static_cast<const float*>(g.data_ptr());
+      args.gate_token_stride = g.stride(0);
+      args.gate_head_stride = g.stride(1);
+    }
+    const at::Tensor& out = RowsOf(a[7], device, rows, heads, dim);
+    args.out = static_cast<float*>(out.data_ptr());
+    args.out_token_stride = out.stride(0);
+    args.out_head_stride = out.stride(1);
+    args.visible = a[9] != Py_None ? IntsOf(a[9], device, rows) : nullptr;
+    args.accumulate = SmallInt(a[11]);
+    args.scratch = Ptr<void>(a[12]);
+    args.scratch_bytes = static_cast<size_t>(Int(a[13]));
+    return Unlocked([&] { return api.cache8_attend(ctx, cache, batch.data(), &args); });
+  });
+}
+
+// cache8_evict(ctx, device, cache, batch, sequences, kv_heads, budget, first, last, kept, held, into, into_slots); held and
+// into_slots (a ctypes array) may be None
+PyObject* Cache8Evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return Guarded(n, 13, [&] {
+    gufo_cuda_ctx* ctx = Context(a[0]);
+    const int device = SmallInt(a[1]);
+    const long long cache = Int(a[2]);
+    const BatchArgs batch(a[3]);
+    const long long sequences = Int(a[4]), heads = Int(a[5]);
+    const int budget = SmallInt(a[6]), first = SmallInt(a[7]), last = SmallInt(a[8]);
+    int* kept = IntsOf(a[9], device, sequences * heads * budget);
+    int* held = a[10] != Py_None ? IntsOf(a[10], device, sequences) : nullptr;
+    const long long into = Int(a[11]);
+    std::unique_ptr<InPlace<int>> slots;
+    if (a[12] != Py_None) {
+      slots = std::make_unique<InPlace<int>>(a[12]);
+      if (slots->count() < sequences) {
+        Refuse("cache8: a slot for each sequence");
+      }
+    }
+    const int* into_slots = slots ? slots->data() : nullptr;
+    return Unlocked([&] { return api.cache8_evict(ctx, cache, batch.data(), budget, first, last, kept, held, into, into_slots); });
+  });
+}
+
 // decoder_step(decoder address, token, logits)
 PyObject* DecoderStep(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Guarded(n, 3, [&] {
@@ -525,6 +701,11 @@ PyObject* Bind(PyObject*, PyObject* handle) {
   find(&api.route, "gufo_cuda_route_device");
   find(&api.moe_ffn, "gufo_cuda_moe_ffn_device");
   find(&api.moe_layer, "gufo_cuda_moe_layer_device");
+  find(&api.rope, "gufo_cuda_rope_device");
+  find(&api.cache8_append, "gufo_cuda_cache8_append_device");
+  find(&api.cache8_rows, "gufo_cuda_cache8_rows_device");
+  find(&api.cache8_attend, "gufo_cuda_cache8_attend_device");
+  find(&api.cache8_evict, "gufo_cuda_cache8_evict_device");
   find(&api.decoder_step, "gufo_cuda_decoder_step");
   find(&api.decoder_step_tokens, "gufo_cuda_decoder_step_tokens");
   find(&api.host_take, "gufo_cuda_host_take");
@@ -546,6 +727,11 @@ PyMethodDef methods[] = {
     FAST("route", Route),
     FAST("moe_ffn", MoeFfn),
     FAST("moe_layer", MoeLayer),
+    FAST("rope", Rope),
+    FAST("cache8_append", Cache8Append),
+    FAST("cache8_rows", Cache8Rows),
+    FAST("cache8_attend", Cache8Attend),
+    FAST("cache8_evict", Cache8Evict),
     FAST("decoder_step", DecoderStep),
     FAST("decoder_step_tokens", DecoderStepTokens),
     FAST("host_buffer", NewHostBuffer),

@@ -541,9 +541,10 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
  * kv_heads. `out` overlaps none of the inputs.
  * accumulate != 0 (caches with weights): adds the softmax weights, summed over the sequence's
  * tokens and the query heads of a KV head, to the rows' weights.
- * scratch: gufo_cuda_cache8_attend_scratch bytes, 16-byte aligned, cleared once before its
- * first call (every call leaves its counters clear); calls that may be in flight together,
- * those of captured graphs among them, need one each. Works in stream captures. */
+ * scratch: gufo_cuda_cache8_attend_scratch bytes, 16-byte aligned, whatever they hold; calls that
+ * may be in flight together, those of captured graphs among them, need one each. Works in stream
+ * captures. Waits inside the kernel (for its own copies) are bounded: where one runs out, after
+ * about a second, the outputs it concerns are NaN. */
 typedef struct gufo_cuda_cache8_attend_args {
   int heads;
   float scale; /* 0: 1 / sqrt(head_dim) */

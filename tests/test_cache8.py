@@ -90,9 +90,9 @@ def test_null_contexts_refused(lib):
 
 def test_host_tensors_refused():
     with pytest.raises(ValueError):
-        Batch(torch.zeros(2, dtype=torch.int32), None, None)
+        Batch(0, torch.zeros(2, dtype=torch.int32), None, None)
     with pytest.raises(ValueError):
-        backend.check_rows("rows", torch.zeros(2, 1, 16))
+        backend.check_rows("rows", 0, torch.zeros(2, 1, 16))
     with pytest.raises(ValueError):
         CudaCache8(None, 1, 1, 16, 16, format="e5m2")
 
