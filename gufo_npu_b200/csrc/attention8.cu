@@ -43,7 +43,8 @@
 namespace gufo {
 namespace {
 
-constexpr int kMostUnitCost = 22;
+constexpr int kMostUnitCost = 32;
+constexpr int kShortCapacity = 384;
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kMostSms = 160;                 // whose blocks a call uses
@@ -75,6 +76,7 @@ struct AttendArgs {
   int whole;               // rows of queries, gates and outputs may be taken four values at a time
   Cut* cuts;               // [units or blocks]
   int by_unit;
+  int undivided;           // a block a unit
   float* sums;             // [blocks][2: the unit it goes on with, the one it begins][rows][head_dim]
   float* stats;            // [blocks][2][rows][2]
   float* scores;           // [query rows][capacity]; null: no weights
@@ -89,9 +91,9 @@ template <int NS, int RT>
 struct Shape {
   static constexpr int kTile = NS * kCacheBlock;            // rows that a group takes at a time
   static constexpr int kGroups = kWarps / NS;
-  // What a unit costs besides its tiles (queries, the join), in tiles: some 4 us, in which a
-  // block's share of the memory's rate brings 44 KB.
-  static constexpr int kUnitCost = kMostUnitCost / (NS * NS * RT) > 0 ? kMostUnitCost / (NS * NS * RT) : 1;
+  // What a unit costs besides its tiles (queries, the join): some 5 us, as much as so many tiles
+  // of a block that shares its SM with the others.
+  static constexpr int kUnitCost = kMostUnitCost / (NS * NS);
   static constexpr int kRowBytes = 64 * NS;
   static constexpr int kSlot = kCacheBlock * kRowBytes + 16;   // a block's keys or values, their scale
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
@@ -251,6 +253,7 @@ struct Unit {
   int start;      // of its tiles
   int chunk, kh;
   int number;     // of all units of the batch
+  Unit() = default;
   __device__ __forceinline__ Unit(const BatchArgs& batch, const Shares& shares, int kv_heads, int unit_cost, int at) {
     const int sequences = batch.sequences;
     int low = 0, high = sequences - 1;
@@ -271,12 +274,12 @@ struct Unit {
     number = batch.first_item[low] * kv_heads + unit;
   }
 };
-__device__ __forceinline__ Task TaskOf(const AttendArgs& a, const BatchArgs& batch, const Shares& shares, const Unit& unit, int rows) {
+__device__ __forceinline__ Task TaskOf(const AttendArgs& a, const BatchArgs& batch, int position, const Unit& unit, int rows) {
   Task task;
   task.e = batch.of[unit.sequence];
   task.row0 = unit.chunk * rows;
   task.rows = min(rows, task.e.tokens * a.group - task.row0);
-  task.position = shares.position[unit.sequence];
+  task.position = position;
   return task;
 }
 // Where a block's part of a unit starts, in rows: of the one that it goes on with, or begins.
@@ -353,15 +356,22 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = warp / NS, member = warp % NS;
   const int g = lane >> 2, t = lane & 3;
-  ShareOut(a, batch, kTile, S::kUnitCost, shares);
-  const Stretches stretches(shares.ahead[batch.sequences], S::kGroups, gridDim.x);   // a tile a group at least
-  if (threadIdx.x == 0 && !a.by_unit) {
-    a.cuts[blockIdx.x].parts = 0;      // unless it begins a unit that others have parts of
+  int begin = 0, end = 1, all = 1;
+  if (!a.undivided) {
+    ShareOut(a, batch, kTile, S::kUnitCost, shares);
+    all = shares.ahead[batch.sequences];
   }
-  if (blockIdx.x >= stretches.blocks) {
-    return;
+  const Stretches stretches(all, S::kGroups, gridDim.x);   // a tile a group at least
+  if (!a.undivided) {
+    if (threadIdx.x == 0 && !a.by_unit) {
+      a.cuts[blockIdx.x].parts = 0;      // unless it begins a unit that others have parts of
+    }
+    if (blockIdx.x >= stretches.blocks) {
+      return;
+    }
+    begin = stretches.start_of(blockIdx.x);
+    end = stretches.start_of(blockIdx.x + 1);
   }
-  const int begin = stretches.start_of(blockIdx.x), end = stretches.start_of(blockIdx.x + 1);
 
   const auto ring_of = [&](int w) { return raw + w * (S::kSlots * S::kSlot); };
   uint8_t* const ring = ring_of(warp);
@@ -393,15 +403,29 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 
 #pragma unroll 1
   for (int from = begin; from < end;) {
-    const Unit unit(batch, shares, c.kv_heads, S::kUnitCost, from);
-    const int first_tile = max(from - unit.start, 0);
-    const int last_tile = min(end - unit.start, unit.tiles);
-    from = unit.start + unit.tiles;
-    if (last_tile <= first_tile) {
-      continue;
+    Unit unit;
+    Task task;
+    int first_tile = 0, last_tile = INT_MAX;
+    if (a.undivided) {
+      const int item = blockIdx.x / c.kv_heads;
+      unit.sequence = SequenceOf(batch, item);
+      unit.kh = blockIdx.x - item * c.kv_heads;
+      unit.chunk = item - batch.first_item[unit.sequence];
+      unit.tiles = last_tile;
+      unit.start = unit.number = 0;
+      from = end;
+      task = TaskOf(a, batch, __ldcg(batch.positions + batch.of[unit.sequence].index), unit, 8 * RT);
+    } else {
+      unit = Unit(batch, shares, c.kv_heads, S::kUnitCost, from);
+      first_tile = max(from - unit.start, 0);
+      last_tile = min(end - unit.start, unit.tiles);
+      from = unit.start + unit.tiles;
+      if (last_tile <= first_tile) {
+        continue;
+      }
+      task = TaskOf(a, batch, shares.position[unit.sequence], unit, 8 * RT);
     }
     const int kh = unit.kh;
-    const Task task = TaskOf(a, batch, shares, unit, 8 * RT);
     if (threadIdx.x < 8 * RT) {
       const int r = min(static_cast<int>(threadIdx.x), task.rows - 1);
       row_seen[threadIdx.x] = SeenBy(a, task.e, task.position, (task.row0 + r) / a.group);
@@ -460,6 +484,9 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         const int f = lane + 32 * i;
         rows_in[n][i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (there && 4 * f < c.head_dim) {
+          if (a.gate != nullptr && f % 8 == 0) {      // (wanted at the end: from L2 then)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a.gate + q.token * a.gate_token_stride + q.head * a.gate_head_stride + 4 * f));
+          }
           if (a.whole) {
             rows_in[n][i] = *reinterpret_cast<const float4*>(row + 4 * f);
           } else {
@@ -940,7 +967,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim)[f] = sum;
       }
     }
-    if (first_tile == 0 && threadIdx.x == 0 && (a.by_unit || !alone)) {
+    if (first_tile == 0 && threadIdx.x == 0 && (a.by_unit || !alone) && !a.undivided) {
       a.cuts[a.by_unit ? unit.number : static_cast<int>(blockIdx.x)] = {
           static_cast<int>(blockIdx.x), alone ? 0 : stretches.owner_of(unit.start + unit.tiles - 1) - static_cast<int>(blockIdx.x) + 1,
           task.rows, task.e.row, kh * a.group, task.row0};
@@ -950,31 +977,35 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   }
 }
 
-// The units that several blocks have parts of: grid (cuts, rows of a unit). One block a query
-// row: the parts' factors, then their sums, groups of threads taking a part of the parts each.
+// The units that several blocks have parts of: grid (cuts, rows of a unit / R). R query rows a block:
+// the parts' factors, then their sums; groups of a row's threads take a part of the parts each. A row a
+// block where there are few (one long sequence has a hundred parts), four where there are many.
 constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads)
+template <int R>
+__global__ void __launch_bounds__(kJoinThreads, R == 1 ? 2 : 4)
 JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
-  __shared__ float factor[kMostBlocks];
-  __shared__ float of_warp[kJoinThreads / 32][2];
-  __shared__ float4 partial[kJoinThreads];
+  constexpr int kRowThreads = kJoinThreads / R, kRowWarps = kRowThreads / 32;
+  __shared__ float factor[R][kMostBlocks];
+  __shared__ float of_warp[R][kRowWarps][2];
+  __shared__ float4 partial[R][kRowThreads];
   GridLaunchDependents();
   const CacheView& c = a.cache;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.y;
+  const int at_row = threadIdx.x / kRowThreads, thread = threadIdx.x % kRowThreads, warp = thread >> 5, lane = thread & 31;
+  const int r = blockIdx.y * R + at_row;
   GridDependencyWait();
   const Cut cut = a.cuts[blockIdx.x];
   const int first_block = cut.first, count = cut.parts;
-  if (r >= cut.rows || count == 0) {
+  if (count == 0 || static_cast<int>(blockIdx.y) * R >= cut.rows) {
     return;
   }
+  const bool mine = r < cut.rows;      // (the others come along to the barriers)
   const auto part_at = [&](int i) { return PartOf(first_block + i, i == 0, rows) + r; };
   const int fours = c.head_dim / 4;
-  const int takers = kJoinThreads / fours;
-  const int taker = threadIdx.x / fours, f = threadIdx.x - taker * fours;
-  const int i_first = count * taker / takers, i_end = taker < takers ? count * (taker + 1) / takers : 0;
+  const int takers = kRowThreads / fours;
+  const int taker = thread / fours, f = thread - taker * fours;
+  const int i_first = count * taker / takers, i_end = mine && taker < takers ? count * (taker + 1) / takers : 0;
   // The first sums are on their way while the statistics are looked at.
-  constexpr int kAhead = 16;
+  constexpr int kAhead = R == 1 ? 16 : 8;
   float4 v[kAhead];
   const auto get = [&](int i0) {
 #pragma unroll
@@ -983,38 +1014,46 @@ JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
     }
   };
   get(i_first);
+  constexpr int kStats = (kMostBlocks + kRowThreads - 1) / kRowThreads;
+  float2 stats[kStats];
   float most = -INFINITY;
-  for (int i = threadIdx.x; i < count; i += kJoinThreads) {
-    factor[i] = __ldcg(reinterpret_cast<const float2*>(a.stats) + part_at(i)).x;
-    most = fmaxf(most, factor[i]);
+#pragma unroll
+  for (int n = 0; n < kStats; ++n) {
+    const int i = thread + n * kRowThreads;
+    stats[n] = mine && i < count ? __ldcg(reinterpret_cast<const float2*>(a.stats) + part_at(i)) : make_float2(-INFINITY, 0.f);
+    most = fmaxf(most, stats[n].x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
   }
   if (lane == 0) {
-    of_warp[warp][0] = most;
+    of_warp[at_row][warp][0] = most;
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    most = fmaxf(most, of_warp[w][0]);
+  for (int w = 0; w < kRowWarps; ++w) {
+    most = fmaxf(most, of_warp[at_row][w][0]);
   }
   float total = 0.f;
-  for (int i = threadIdx.x; i < count; i += kJoinThreads) {
-    const float by = factor[i] == most ? 1.f : exp2f(factor[i] - most);
-    factor[i] = by;
-    total += __ldcg(reinterpret_cast<const float2*>(a.stats) + part_at(i)).y * by;
+#pragma unroll
+  for (int n = 0; n < kStats; ++n) {
+    const int i = thread + n * kRowThreads;
+    const float by = stats[n].x == most ? 1.f : exp2f(stats[n].x - most);
+    if (i < count) {
+      factor[at_row][i] = by;
+    }
+    total += stats[n].y * by;
   }
   total = WarpSum(total);
   if (lane == 0) {
-    of_warp[warp][1] = total;
+    of_warp[at_row][warp][1] = total;
   }
   __syncthreads();
   total = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    total += of_warp[w][1];
+  for (int w = 0; w < kRowWarps; ++w) {
+    total += of_warp[at_row][w][1];
   }
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = i_first; i0 < i_end; i0 += kAhead) {
@@ -1023,24 +1062,26 @@ JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const float by = i0 + i < i_end ? factor[i0 + i] : 0.f;
+      const float by = i0 + i < i_end ? factor[at_row][i0 + i] : 0.f;
       sum.x = fmaf(v[i].x, by, sum.x), sum.y = fmaf(v[i].y, by, sum.y), sum.z = fmaf(v[i].z, by, sum.z), sum.w = fmaf(v[i].w, by, sum.w);
     }
   }
-  partial[threadIdx.x] = sum;
+  partial[at_row][thread] = sum;
   __syncthreads();
+  if (!mine) {
+    return;
+  }
   QueryRow q;
   q.token = cut.token + (cut.first_flat + r) / a.group;
   q.head = cut.head + (cut.first_flat + r) % a.group;
-  const bool sees = !(total < 0.f);
   if (taker == 0) {
     for (int i = 1; i < takers; ++i) {
-      const float4 w = partial[i * fours + f];
+      const float4 w = partial[at_row][i * fours + f];
       sum.x += w.x, sum.y += w.y, sum.z += w.z, sum.w += w.w;
     }
-    Finish(a, q, f, sum, total, sees);
+    Finish(a, q, f, sum, total, !(total < 0.f));
   }
-  if (threadIdx.x == 0) {
+  if (thread == 0) {
     Note(a, q, most, total);
   }
 }
@@ -1090,6 +1131,8 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
   using S = Shape<NS, RT>;
   const int blocks = Sms(ctx) * S::kBlocks;
   a.by_unit = units <= blocks;
+  // Short caches: a block a unit, and nothing to be shared out or joined.
+  a.undivided = a.cache.capacity <= kShortCapacity;
   static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
                 "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
@@ -1099,9 +1142,19 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(blocks), dim3(kThreads), S::kBytes, ctx->stream, 1, a, b));
-  GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel, dim3(a.by_unit ? static_cast<int>(units) : blocks, rows), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
-  ctx->launches.fetch_add(2);
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(a.undivided ? static_cast<int>(units) : blocks), dim3(kThreads), S::kBytes,
+                                 ctx->stream, 1, a, b));
+  ctx->launches.fetch_add(1);
+  if (a.undivided) {
+    return GUFO_CUDA_OK;
+  }
+  const int cuts = a.by_unit ? static_cast<int>(units) : blocks;
+  if (cuts * rows <= 1024) {
+    GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel<1>, dim3(cuts, rows), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
+  } else {
+    GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel<4>, dim3(cuts, (rows + 3) / 4), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
+  }
+  ctx->launches.fetch_add(1);
   return GUFO_CUDA_OK;
 }
 
