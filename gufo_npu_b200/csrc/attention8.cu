@@ -375,9 +375,9 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 
   const auto ring_of = [&](int w) { return raw + w * (S::kSlots * S::kSlot); };
   uint8_t* const ring = ring_of(warp);
-  const int codes_bytes = kCacheBlock * c.head_dim, block_bytes = BlockBytes(c.head_dim);
+  const int codes_bytes = CodeBytes(c.head_dim), block_bytes = BlockBytes(c.head_dim);
   const int pieces = c.head_dim / 16;
-  // This lane's places in a block: keys of row g (g + 8: 128 further), piece t of a segment
+  // This lane's places in a block: keys of row g (g + 8: 256 further), piece t of a segment
   // (a segment: 1024 further); values of rows 2 t and 2 t + 1 (+ 8), eight dimensions of this
   // warp's segment (past the last piece any: nobody asks for them).
   const int key_place = PieceAt(0, g, t);
@@ -619,7 +619,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           }
 #pragma unroll
           for (int seg = 0; seg < NS; ++seg) {
-            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 128);
+            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
 #pragma unroll
             for (int rt = 0; rt < RA; ++rt) {
 #pragma unroll
@@ -645,7 +645,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           }
 #pragma unroll
           for (int seg = 0; seg < NS; ++seg) {
-            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 128);
+            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
             const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
             uint32_t k[4][4];
 #pragma unroll
@@ -782,7 +782,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
               const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
               // This warp's pieces: 64 words each.
               uint32_t* const words = reinterpret_cast<uint32_t*>(values) + 256 * member;
-              const int count = 64 * min(4, pieces - 4 * member);
+              const int count = 64 * min(4, (pieces + 1) / 2 * 2 - 4 * member);
               uint32_t found = 0;
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -838,7 +838,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            v[i] = *reinterpret_cast<const uint2*>(values + (value_place ^ (16 * (i & 1))) + 128 * (i >> 1));
+            v[i] = *reinterpret_cast<const uint2*>(values + (value_place ^ (32 * (i & 1))) + 256 * (i >> 1));
           }
           uint32_t of[4][4];   // dimensions 2 m, 2 m + 1 of the eight: rows beside one another
 #pragma unroll

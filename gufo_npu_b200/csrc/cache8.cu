@@ -27,6 +27,7 @@ template <typename Format>
 __global__ void __launch_bounds__(kAppendThreads)
 AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ BatchArgs batch) {
   __shared__ float tops[2][4];
+  __shared__ __align__(16) uint8_t image[2][kCacheBlock * kCacheMaxDim];
   GridLaunchDependents();
   GridDependencyWait();
   const BatchEntry& e = batch.of[SequenceOf(batch, blockIdx.x)];
@@ -89,23 +90,47 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
     exponent = max(exponent, ExponentOf(was));
   }
   const float inverse = PowerOfTwo(-exponent);   // (exponent is -126 .. 120)
+  if (row0 >= start && row0 + kCacheBlock <= end) {
+    // A whole block: put together in shared memory and written sixteen bytes a thread. (The half
+    // that a last single piece leaves of its pair holds zeros.)
+    if (c.head_dim % 32 != 0 && lane < 16 && warp == 0) {
+      *reinterpret_cast<uint4*>(image[side] + PieceAt(side, lane, c.head_dim / 16)) = make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = row0 + 4 * warp + i;
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int n = 0; n < kTimes; ++n) {
-      const int f = lane + 32 * n;
-      if (f >= fours) {
-        continue;
+      for (int n = 0; n < kTimes; ++n) {
+        const int f = lane + 32 * n;
+        if (f < fours) {
+          const float4 v = x[i][n];
+          *(reinterpret_cast<uint32_t*>(image[side] + PieceAt(side, 4 * warp + i, f / 4)) + f % 4) =
+              Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+        }
       }
-      uint32_t* to = reinterpret_cast<uint32_t*>(codes + PieceAt(side, 4 * warp + i, f / 4)) + f % 4;
-      if (r >= start && r < end) {
-        const float4 v = x[i][n];
-        *to = Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
-      } else if (r < start && exponent > ExponentOf(was)) {
-        const float4 v = DecodeFour<Format>(*to);
-        const float down = was * inverse;   // (0 where the scales are more than 2^149 apart, as the codes are then)
-        *to = Format::Encode(v.x * down, v.y * down, v.z * down, v.w * down);
+    }
+    __syncthreads();
+    for (int at = threadIdx.x % 128 * 16; at < CodeBytes(c.head_dim); at += 128 * 16) {
+      *reinterpret_cast<uint4*>(codes + at) = *reinterpret_cast<const uint4*>(image[side] + at);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row0 + 4 * warp + i;
+#pragma unroll
+      for (int n = 0; n < kTimes; ++n) {
+        const int f = lane + 32 * n;
+        if (f >= fours) {
+          continue;
+        }
+        uint32_t* to = reinterpret_cast<uint32_t*>(codes + PieceAt(side, 4 * warp + i, f / 4)) + f % 4;
+        if (r >= start && r < end) {
+          const float4 v = x[i][n];
+          *to = Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+        } else if (r < start && exponent > ExponentOf(was)) {
+          const float4 v = DecodeFour<Format>(*to);
+          const float down = was * inverse;   // (0 where the scales are more than 2^149 apart, as the codes are then)
+          *to = Format::Encode(v.x * down, v.y * down, v.z * down, v.w * down);
+        }
       }
     }
   }
@@ -122,53 +147,63 @@ struct RowsArgs {
   float* out[2];
 };
 constexpr int kRowsThreads = 256;
-constexpr int kRowsEach = 8;    // groups of four values of a thread
 
-// Items: kRowsThreads * kRowsEach groups of four values of a sequence's rows. Grid: (items, 2).
+// Grid: (blocks that the batch touches, KV heads, 2). A block's rows are read a word of four codes a
+// lane, rows beside one another from the same sectors, and go out sixteen bytes a lane.
 template <typename Format>
 __global__ void __launch_bounds__(kRowsThreads)
 RowsKernel(const __grid_constant__ RowsArgs a, const __grid_constant__ BatchArgs batch) {
   GridLaunchDependents();
   GridDependencyWait();
-  const int side = blockIdx.y;
+  const int side = blockIdx.z, head = blockIdx.y;
   float* out = a.out[side];
   if (out == nullptr) {
     return;
   }
   const BatchEntry& e = batch.of[SequenceOf(batch, blockIdx.x)];
   const CacheView& c = a.cache;
-  const int position = batch.positions[e.index];
-  const unsigned fours = c.head_dim / 4, width = fours * c.kv_heads;   // of a row
-  const int64_t first = static_cast<int64_t>(blockIdx.x - batch.first_item[&e - batch.of]) * (kRowsThreads * kRowsEach);
-  const int token0 = static_cast<int>(first / width);
-  const unsigned in_row0 = static_cast<unsigned>(first - static_cast<int64_t>(token0) * width) + threadIdx.x;
-  float4* to = reinterpret_cast<float4*>(out) + static_cast<int64_t>(e.row) * width + first + threadIdx.x;
-  uint32_t word[kRowsEach];
-  float scale[kRowsEach];
-#pragma unroll
-  for (int i = 0; i < kRowsEach; ++i) {
-    const unsigned beyond = (in_row0 + i * kRowsThreads) / width, in_row = in_row0 + i * kRowsThreads - beyond * width;
-    const int64_t token = static_cast<int64_t>(token0) + beyond;
-    const int64_t r = position + token;
-    word[i] = 0;
-    scale[i] = 0.f;
-    if (token < e.tokens && r >= 0 && r < c.capacity) {
-      const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + in_row / fours;
-      const unsigned f = in_row % fours;
-      const uint8_t* block = BlocksOf(c, side, of_head) + (r / kCacheBlock) * BlockBytes(c.head_dim);
-      word[i] = *(reinterpret_cast<const uint32_t*>(block + PieceAt(side, r % kCacheBlock, f / 4)) + f % 4);
-      scale[i] = *ScaleOf(block, c.head_dim);
-    }
+  const int64_t position = batch.positions[e.index];
+  const int nth = blockIdx.x - batch.first_item[&e - batch.of];
+  // The first row of the block, counted from the slot's first (a block may lie outside).
+  const int64_t row0 = ((position >> 4) + nth) * kCacheBlock;
+  const int fours = c.head_dim / 4;
+  int lanes = 4;      // of a row: a power of two
+  while (lanes < fours) {
+    lanes *= 2;
   }
+  const int f = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = kRowsThreads / lanes;
+  if (f >= fours) {
+    return;
+  }
+  const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + head;
+  const bool inside = row0 >= 0 && row0 < c.capacity;
+  const uint8_t* block = BlocksOf(c, side, of_head) + static_cast<size_t>(inside ? row0 / kCacheBlock : 0) * BlockBytes(c.head_dim);
+  const float scale = inside ? *ScaleOf(block, c.head_dim) : 0.f;
+  const int64_t token0 = row0 - position;     // of the block's first row
+  float4* to = reinterpret_cast<float4*>(out + ((e.row + token0) * c.kv_heads + head) * c.head_dim) + f;
+  const int64_t stride = static_cast<int64_t>(c.kv_heads) * fours;
+  constexpr int kEach = 4;
+  for (int r0 = first; r0 < kCacheBlock; r0 += kEach * step) {
+    uint32_t word[kEach];
 #pragma unroll
-  for (int i = 0; i < kRowsEach; ++i) {
-    if (static_cast<int64_t>(token0) + (in_row0 + i * kRowsThreads) / width < e.tokens) {
-      float4 v = DecodeFour<Format>(word[i]);
-      v.x *= scale[i], v.y *= scale[i], v.z *= scale[i], v.w *= scale[i];
-      __stcs(to + i * kRowsThreads, v);
+    for (int i = 0; i < kEach; ++i) {
+      const int r = r0 + i * step;
+      word[i] = inside && r < kCacheBlock ? *(reinterpret_cast<const uint32_t*>(block + PieceAt(side, r, f / 4)) + f % 4) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int r = r0 + i * step;
+      if (r < kCacheBlock && token0 + r >= 0 && token0 + r < e.tokens) {
+        float4 v = DecodeFour<Format>(word[i]);
+        v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+        __stcs(to + r * stride, v);
+      }
     }
   }
 }
+
+// Blocks that `tokens` rows touch at most.
+int BlocksOfRows(int tokens) { return tokens > 0 ? (tokens - 1 + kCacheBlock - 1) / kCacheBlock + 1 : 0; }
 
 int CheckConfig(const gufo_cuda_cache8_config& c) {
   if (c.format != GUFO_CUDA_CACHE8_E4M3 && c.format != GUFO_CUDA_CACHE8_INT8) {
@@ -331,7 +366,7 @@ int gufo_cuda_cache8_append_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   const auto kernel = cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::AppendKernel<gufo::E4m3> : gufo::AppendKernel<gufo::Int8>;
   return gufo::ForEachRun(
-      *batch, [](int tokens) { return tokens > 0 ? (tokens - 1 + gufo::kCacheBlock - 1) / gufo::kCacheBlock + 1 : 0; },
+      *batch, gufo::BlocksOfRows,
       [&](const gufo::BatchArgs& b, int blocks) -> int {
         GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(blocks, cache->c.kv_heads), dim3(gufo::kAppendThreads), 0, ctx->stream,
                                              1, a, b));
@@ -358,18 +393,14 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, co
   if (((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15) != 0) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_rows: rows go to 16-byte boundaries");
   }
-  const int64_t width = static_cast<int64_t>(cache->c.kv_heads) * cache->c.head_dim / 4;
-  constexpr int64_t kItem = gufo::kRowsThreads * gufo::kRowsEach;
-  if (rows * width / kItem + batch->sequences > INT32_MAX) {
-    return Fail(GUFO_CUDA_TOO_LARGE, "cache8_rows: too many rows for one call");
-  }
   const gufo::RowsArgs a{gufo::ViewOf(*cache), {keys, values}};
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   const auto kernel = cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::RowsKernel<gufo::E4m3> : gufo::RowsKernel<gufo::Int8>;
   return gufo::ForEachRun(
-      *batch, [&](int tokens) { return static_cast<int>((tokens * width + kItem - 1) / kItem); },
-      [&](const gufo::BatchArgs& b, int items) -> int {
-        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(items, 2), dim3(gufo::kRowsThreads), 0, ctx->stream, 1, a, b));
+      *batch, gufo::BlocksOfRows,
+      [&](const gufo::BatchArgs& b, int blocks) -> int {
+        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(blocks, cache->c.kv_heads, 2), dim3(gufo::kRowsThreads), 0, ctx->stream,
+                                             1, a, b));
         ctx->launches.fetch_add(1);
         return GUFO_CUDA_OK;
       });

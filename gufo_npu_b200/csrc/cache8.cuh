@@ -26,11 +26,13 @@ struct BatchArgs {
   const int* positions;
 };
 
-// What a kernel sees of a cache. A block of 16 rows of a head is 16 * head_dim codes, then their
-// scale and 12 bytes of nothing: one contiguous copy. The codes stand piece by piece (16 values),
-// the 16 rows' bytes of a piece together, in an order of the rows that lets the attention's
-// lanes read them in fragments from different places of shared memory: for keys eight lanes read
-// four pieces of two rows, for values two pieces of every second row.
+// What a kernel sees of a cache. A block of 16 rows of a head is their codes, then their scale and
+// 12 bytes of nothing: one contiguous copy. The codes stand by pairs of pieces (32 values), the 16
+// rows' bytes of a pair together: a row's part of a pair is a sector, which is what a row that is
+// gathered or written by itself costs (pieces alone: half of what is fetched is of another row; 8192
+// rows scattered over 64 MB 24 us, not 17). The order of the rows within a pair lets the
+// attention's lanes read their fragments from different places of shared memory: for keys eight
+// lanes read four pieces of two rows, for values two pieces of every second row.
 struct CacheView {
   uint8_t* sides[2];
   float* weights;
@@ -39,20 +41,23 @@ struct CacheView {
 inline CacheView ViewOf(const Cache8& c) {
   return {{c.sides[0], c.sides[1]}, c.weights, c.c.kv_heads, c.c.head_dim, c.c.capacity};
 }
-__host__ __device__ inline int BlockBytes(int head_dim) { return kCacheBlock * head_dim + 16; }
+__host__ __device__ inline int CodeBytes(int head_dim) { return (head_dim + 31) / 32 * 32 * kCacheBlock; }
+__host__ __device__ inline int BlockBytes(int head_dim) { return CodeBytes(head_dim) + 16; }
 // The first block of a head of a slot, and of a side's block its scale.
 __device__ __forceinline__ uint8_t* BlocksOf(const CacheView& c, int side, size_t of_head) {
   return c.sides[side] + of_head * (c.capacity / kCacheBlock) * BlockBytes(c.head_dim);
 }
 __device__ __forceinline__ float* ScaleOf(uint8_t* block, int head_dim) {
-  return reinterpret_cast<float*>(block + kCacheBlock * head_dim);
+  return reinterpret_cast<float*>(block + CodeBytes(head_dim));
 }
 __device__ __forceinline__ const float* ScaleOf(const uint8_t* block, int head_dim) {
-  return reinterpret_cast<const float*>(block + kCacheBlock * head_dim);
+  return reinterpret_cast<const float*>(block + CodeBytes(head_dim));
 }
 // Where a piece of a row stands in its block.
 __device__ __forceinline__ int PieceAt(int side, int row, int piece) {
-  return (piece * kCacheBlock + (row ^ (side == 0 ? 2 * (piece & 3) : piece & 7))) * 16;
+  const int pair = piece >> 1;
+  const int at = side == 0 ? row ^ (2 * (pair & 1)) : row ^ (row >> 2 & 1);
+  return pair * 512 + at * 32 + (piece & 1) * 16;
 }
 
 // Calls launch(args) for every run of at most kBatchSequences sequences with work; items(tokens)

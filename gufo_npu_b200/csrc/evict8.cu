@@ -2,10 +2,10 @@
 //
 // Which rows stay. A block of threads per sequence and KV head finds the weight of the last row
 // that stays by radix selection over the weights' 32 bits (histograms of 11, 11 and 10 of them,
-// whole numbers, so that nothing depends on the order of the atomics), then walks the rows once
-// in their order, writes down the ones that stay and moves their weights. Bound by latency: four
-// walks over 4 bytes a row, which are in L2 behind the first, and a scan of the block a walk
-// of 4096 rows.
+// whole numbers, so that nothing depends on the order of the atomics), then goes through the rows
+// in their order, writes down the ones that stay and moves their weights. Bound by latency: up
+// to 16384 rows are read once and stay in registers, and behind the first histogram only the
+// rows of one bin are looked at.
 //
 // Moving them. A warp makes one block of 16 rows: it gathers them, takes their largest
 // magnitude, and rounds what had another scale. In place, the rows a block receives come from
@@ -40,42 +40,23 @@ __device__ __forceinline__ uint32_t KeyOf(float w) {
   return w != w ? 0u : (bits & 0x80000000u) != 0 ? ~bits : bits | 0x80000000u;
 }
 
-// Exclusive sum over the block in thread order, and the sum of all. `spare`: 33 words.
-__device__ __forceinline__ unsigned long long BlockScan(unsigned long long v, unsigned long long* spare, unsigned long long* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  unsigned long long sum = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long below = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-    sum += lane >= o ? below : 0;
-  }
-  __syncthreads();   // what the last call left has been read
-  if (lane == 31) {
-    spare[warp] = sum;
-  }
-  __syncthreads();
-  unsigned long long w = spare[lane];   // kSelectThreads / 32 warps
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long below = __shfl_up_sync(0xFFFFFFFFu, w, o);
-    w += lane >= o ? below : 0;
-  }
-  *total = __shfl_sync(0xFFFFFFFFu, w, 31);
-  const unsigned long long ahead = __shfl_sync(0xFFFFFFFFu, w, warp == 0 ? 0 : warp - 1);
-  return sum - v + (warp == 0 ? 0 : ahead);
-}
-
-// Grid: (KV heads, sequences).
+// Grid: (KV heads, sequences). Threads take four rows beside one another of each of C chunks of
+// 4096; up to 4096 * C rows stay in their registers from the first look to the last.
+template <int C>
 __global__ void __launch_bounds__(kSelectThreads)
 SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArgs batch) {
   __shared__ unsigned bins[kBins];
-  __shared__ unsigned long long spare[32];
-  __shared__ unsigned found[2];   // the bin, and how many more are wanted from it
+  __shared__ uint32_t listed[kBins];       // keys that share the first bits of the one that is looked for
+  __shared__ unsigned of_warp[C][32];
+  __shared__ unsigned found[3];            // the bin, how many more are wanted from it, how many it holds
+  __shared__ unsigned list_count;
+  constexpr int kChunk = 4 * kSelectThreads, kSpan = C * kChunk;
   GridLaunchDependents();
   GridDependencyWait();
   const BatchEntry& e = batch.of[blockIdx.y];
   const CacheView& c = a.cache;
   const int head = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = PositionOf(c, batch, e);
   const int budget = a.budget;
   int* kept = a.kept + (static_cast<size_t>(e.index) * c.kv_heads + head) * budget;
@@ -100,89 +81,185 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
   const int low = first, high = rows - last;        // the rows that compete
   int wanted = budget - first - last;               // of them; fewer than there are
 
-  // The key of the last row that stays: its bits from the top, 11, 11 and 10.
+  float4 w[C];
+  const bool one_span = rows <= kSpan;
+  const auto load = [&](int base) {
+#pragma unroll
+    for (int n = 0; n < C; ++n) {
+      const int i = base + n * kChunk + 4 * threadIdx.x;
+      w[n] = i < rows ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  const auto key_of = [&](int n, int j) { return KeyOf(j == 0 ? w[n].x : j == 1 ? w[n].y : j == 2 ? w[n].z : w[n].w); };
+  // Adds a key's bits to the bins. Many rows have the same weight, none: their lanes add up first.
+  const auto count = [&](uint32_t k, int shift, unsigned bits, bool counts) {
+    const bool none = counts && k == KeyOf(0.f);
+    const unsigned all = __ballot_sync(0xFFFFFFFFu, none);
+    if (none ? lane == __ffs(all) - 1 : counts) {
+      atomicAdd(&bins[k >> shift & bits], none ? __popc(all) : 1u);
+    }
+  };
+  load(0);
+  // The key of the last row that stays: its bits from the top, 11, 11 and 10. Behind the first
+  // look the keys that share its bits are listed, where they are few enough, and the rest is
+  // left alone.
   uint32_t key = 0, mask = 0;
+  bool list = false;
 #pragma unroll 1
   for (int pass = 0; pass < 3 && wanted > 0; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int width = pass == 2 ? 1024 : 2048;
+    const unsigned bits = pass == 2 ? 1023 : 2047;
     for (int i = threadIdx.x; i < kBins; i += kSelectThreads) {
       bins[i] = 0;
     }
+    if (threadIdx.x == 0) {
+      list_count = 0;
+    }
     __syncthreads();
-    for (int base = 0; base < rows; base += 4 * kSelectThreads) {
-      const int i = base + 4 * threadIdx.x;
-      const float4 w = i < rows ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float f[4] = {w.x, w.y, w.z, w.w};
+    if (list) {
+      const unsigned n = found[2];
+      for (unsigned i = threadIdx.x; i < (n + 31) / 32 * 32; i += kSelectThreads) {
+        const uint32_t k = i < n ? listed[i] : 0;
+        count(k, shift, bits, i < n && (k & mask) == key);
+      }
+    } else {
+      for (int base = 0; base < rows; base += kSpan) {
+        if (!one_span && (pass > 0 || base > 0)) {
+          load(base);
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t k = KeyOf(f[j]);
-        const bool counts = i + j >= low && i + j < high && (k & mask) == key;
-        // Many rows have the same weight, none: lanes with the same bin add up first.
-        const unsigned bin = counts ? (k >> shift) & (width - 1) : kBins;
-        const unsigned same = __match_any_sync(0xFFFFFFFFu, bin);
-        if (counts && (threadIdx.x & 31) == __ffs(same) - 1) {
-          atomicAdd(&bins[bin], __popc(same));
+        for (int n = 0; n < C; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = base + n * kChunk + 4 * threadIdx.x + j;
+            const uint32_t k = key_of(n, j);
+            count(k, shift, bits, i >= low && i < high && (k & mask) == key);
+          }
         }
       }
     }
     __syncthreads();
+    // The bin with the last wanted one, from the top: thread t has bins 2047 - 2 t and 2046 - 2 t.
     const unsigned top = bins[kBins - 1 - 2 * threadIdx.x], next = bins[kBins - 2 - 2 * threadIdx.x];
-    unsigned long long total;
-    const unsigned ahead = static_cast<unsigned>(BlockScan(top + next, spare, &total));
+    unsigned sum = top + next;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned below = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      sum += lane >= o ? below : 0;
+    }
+    if (lane == 31) {
+      of_warp[0][warp] = sum;
+    }
+    __syncthreads();
+    unsigned ahead = of_warp[0][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned below = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+      ahead += lane >= o ? below : 0;
+    }
+    ahead = __shfl_sync(0xFFFFFFFFu, ahead, warp == 0 ? 0 : warp - 1);
+    ahead = (warp == 0 ? 0 : ahead) + sum - top - next;
     const unsigned want = static_cast<unsigned>(wanted);
     if (ahead < want && want <= ahead + top) {
-      found[0] = kBins - 1 - 2 * threadIdx.x;
-      found[1] = want - ahead;
+      found[0] = kBins - 1 - 2 * threadIdx.x, found[1] = want - ahead;
+      if (!list) {
+        found[2] = top;
+      }
     } else if (ahead + top < want && want <= ahead + top + next) {
-      found[0] = kBins - 2 - 2 * threadIdx.x;
-      found[1] = want - ahead - top;
+      found[0] = kBins - 2 - 2 * threadIdx.x, found[1] = want - ahead - top;
+      if (!list) {
+        found[2] = next;
+      }
     }
     __syncthreads();
     key |= found[0] << shift;
-    mask |= static_cast<uint32_t>(width - 1) << shift;
+    mask |= bits << shift;
     wanted = static_cast<int>(found[1]);
+    if (!list && one_span && pass < 2 && found[2] <= kBins) {
+      list = true;
+#pragma unroll
+      for (int n = 0; n < C; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = n * kChunk + 4 * threadIdx.x + j;
+          const uint32_t k = key_of(n, j);
+          if (i >= low && i < high && (k & mask) == key) {
+            listed[atomicAdd(&list_count, 1u)] = k;
+          }
+        }
+      }
+    }
     __syncthreads();
   }
 
-  // The rows above the key stay, the ends, and the first `wanted` rows with that very key.
-  unsigned long long before = 0;   // rows that stay anyway | rows with the key << 32
+  // The rows above the key stay, the ends, and the first `wanted` rows with that very key. Rows that
+  // stay anyway and rows with the key are counted together, 16 bits each (a chunk has 4096).
+  unsigned before = 0, ties_before = 0;
 #pragma unroll 1
-  for (int base = 0; base < rows; base += 4 * kSelectThreads) {
-    const int i = base + 4 * threadIdx.x;
-    const float4 w = i < rows ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    const float f[4] = {w.x, w.y, w.z, w.w};
-    bool stays[4], ties[4];
-    unsigned long long mine = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t k = KeyOf(f[j]);
-      const bool competes = i + j >= low && i + j < high && mask != 0;
-      stays[j] = i + j < rows && (i + j < low || i + j >= high || (competes && k > key));
-      ties[j] = competes && k == key;
-      mine += (stays[j] ? 1ull : 0ull) + (ties[j] ? 1ull << 32 : 0ull);
+  for (int base = 0; base < rows; base += kSpan) {
+    if (!one_span) {
+      load(base);
     }
-    unsigned long long total;
-    unsigned long long at = before + BlockScan(mine, spare, &total);   // (a barrier: the weights have been read)
-    before += total;
+    unsigned marks[C], sums[C];      // a thread's rows: stays 1 << j, ties 16 << j; counts up to this thread
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned equal = static_cast<unsigned>(at >> 32);
-      const unsigned place = static_cast<unsigned>(at) + min(equal, static_cast<unsigned>(wanted));
-      if (stays[j] || (ties[j] && equal < static_cast<unsigned>(wanted))) {
-        kept[place] = i + j;
-        if (to != nullptr) {
-          to[place] = f[j];
-        }
+    for (int n = 0; n < C; ++n) {
+      marks[n] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = base + n * kChunk + 4 * threadIdx.x + j;
+        const uint32_t k = key_of(n, j);
+        const bool competes = i >= low && i < high && mask != 0;
+        marks[n] |= i < rows && (i < low || i >= high || (competes && k > key)) ? 1u << j : 0u;
+        marks[n] |= competes && k == key ? 16u << j : 0u;
       }
-      at += (stays[j] ? 1ull : 0ull) + (ties[j] ? 1ull << 32 : 0ull);
+      sums[n] = __popc(marks[n] & 15u) | __popc(marks[n] & 0xF0u) << 16;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned below = __shfl_up_sync(0xFFFFFFFFu, sums[n], o);
+        sums[n] += lane >= o ? below : 0;
+      }
+      if (lane == 31) {
+        of_warp[n][warp] = sums[n];
+      }
     }
+    __syncthreads();     // (the weights have been read, too)
+#pragma unroll
+    for (int n = 0; n < C; ++n) {
+      unsigned ahead = of_warp[n][lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned below = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+        ahead += lane >= o ? below : 0;
+      }
+      const unsigned chunk = __shfl_sync(0xFFFFFFFFu, ahead, 31);
+      ahead = __shfl_sync(0xFFFFFFFFu, ahead, warp == 0 ? 0 : warp - 1);
+      const unsigned up_to = (warp == 0 ? 0 : ahead) + sums[n];
+      unsigned stays = before + (up_to & 0xFFFFu) - __popc(marks[n] & 15u);
+      unsigned ties = ties_before + (up_to >> 16) - __popc(marks[n] & 0xF0u);
+      const float f[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool stay = marks[n] >> j & 1u, tie = marks[n] >> (4 + j) & 1u;
+        if (stay || (tie && ties < static_cast<unsigned>(wanted))) {
+          const unsigned place = stays + min(ties, static_cast<unsigned>(wanted));
+          kept[place] = base + n * kChunk + 4 * threadIdx.x + j;
+          if (to != nullptr) {
+            to[place] = f[j];
+          }
+        }
+        stays += stay;
+        ties += tie;
+      }
+      before += chunk & 0xFFFFu;
+      ties_before += chunk >> 16;
+    }
+    __syncthreads();     // before the counts' next use
   }
 }
 
 // Grid: (groups of kMoveWarps blocks, 2 * KV heads, sequences); in place the first is a cluster.
 template <typename Format, bool kInPlace>
-__global__ void __launch_bounds__(kMoveThreads, 3)
+__global__ void __launch_bounds__(kMoveThreads, kInPlace ? 3 : 2)
 MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArgs batch) {
   constexpr int kTimes = kCacheBlock * kCacheMaxDim / 16 / 32;   // 16-byte pieces of a block, a lane's
   GridLaunchDependents();
@@ -211,8 +288,8 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
     if (moves) {
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        // (Sixteen lanes gather a piece of all rows: what they write is together.)
-        const int r = lane & 15, piece = (lane >> 4) + 2 * i;
+        // (Two lanes a row's part of a pair of pieces, the rows of a pair together.)
+        const int r = lane >> 1, piece = (lane & 1) + 2 * i;
         const int row_of = __shfl_sync(0xFFFFFFFFu, mine, r);
         word[i] = make_uint4(0, 0, 0, 0);
         if (piece < pieces && row_of >= 0) {
@@ -222,7 +299,7 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
       }
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        const float scale = __shfl_sync(0xFFFFFFFFu, was, lane & 15);
+        const float scale = __shfl_sync(0xFFFFFFFFu, was, lane >> 1);
         __half2 most = __float2half2_rn(0.f);
         const uint32_t w[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
 #pragma unroll
@@ -247,7 +324,7 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
       const float now = PowerOfTwo(exponent), inverse = PowerOfTwo(-exponent);
 #pragma unroll
       for (int i = 0; i < kTimes; ++i) {
-        const int r = lane & 15, piece = (lane >> 4) + 2 * i;
+        const int r = lane >> 1, piece = (lane & 1) + 2 * i;
         const float scale = __shfl_sync(0xFFFFFFFFu, was, r);
         const int there = __shfl_sync(0xFFFFFFFFu, mine, r);
         if (piece >= pieces || there < 0) {
@@ -352,7 +429,8 @@ extern "C" int gufo_cuda_cache8_evict_device(gufo_cuda_ctx* ctx, gufo_cuda_cache
         for (int i = 0; i < b.sequences; ++i) {
           a.into_slots[i] = in_place || into_slots == nullptr ? b.of[i].slot : into_slots[b.of[i].index];
         }
-        GUFO_CUDA_TRY(gufo::LaunchOverlapped(gufo::SelectKernel, dim3(cache->c.kv_heads, b.sequences), dim3(gufo::kSelectThreads),
+        const auto select = cache->c.capacity <= 4 * gufo::kSelectThreads ? gufo::SelectKernel<1> : gufo::SelectKernel<4>;
+        GUFO_CUDA_TRY(gufo::LaunchOverlapped(select, dim3(cache->c.kv_heads, b.sequences), dim3(gufo::kSelectThreads),
                                              0, ctx->stream, 1, a, b));
         ctx->launches.fetch_add(1);
         return cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::LaunchMove<gufo::E4m3>(ctx, a, b, in_place)

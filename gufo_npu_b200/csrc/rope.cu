@@ -101,69 +101,97 @@ RopeKernel(const __grid_constant__ RopeArgs a, bool interleaved) {
   }
   const float* in = r.in + token * r.in_token_stride + head0 * r.in_head_stride;
   float* out = r.out + token * r.out_token_stride + head0 * r.out_head_stride;
-  // (Every lane of a warp goes round as often as the longest group of it, for the shuffles.)
+  // Several heads' rows are on their way at once. (Every lane of a warp goes round as often as the
+  // longest group of it, for the shuffles.)
+  constexpr int U = N * V <= 4 ? 4 : 2;
   const int rounds = __reduce_max_sync(0xFFFFFFFFu, heads);
-  for (int h = 0; h < rounds; ++h, in += r.in_head_stride, out += r.out_head_stride) {
-    float x[N][V], y[N][V];
-    float sq = 0.f;
+  for (int h0 = 0; h0 < rounds; h0 += U) {
+    float x[U][N][V], y[U][N][V];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int pair = at(n);
-      const bool mine = h < heads && pair < pairs;
-      if constexpr (V == 4) {
-        float4 first = make_float4(0.f, 0.f, 0.f, 0.f), second = first;
-        const bool split = apart && pair < half;
-        if (mine) {
-          const float* from = in + (split ? pair : 2 * pair);
-          first = __ldcs(reinterpret_cast<const float4*>(from));
-          second = __ldcs(reinterpret_cast<const float4*>(from + (split ? half : 4)));
+    for (int u = 0; u < U; ++u) {
+      const float* row = in + (h0 + u) * r.in_head_stride;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int pair = at(n);
+        const bool mine = h0 + u < heads && pair < pairs;
+        if constexpr (V == 4) {
+          float4 first = make_float4(0.f, 0.f, 0.f, 0.f), second = first;
+          const bool split = apart && pair < half;
+          if (mine) {
+            const float* from = row + (split ? pair : 2 * pair);
+            first = __ldcs(reinterpret_cast<const float4*>(from));
+            second = __ldcs(reinterpret_cast<const float4*>(from + (split ? half : 4)));
+          }
+          const float f[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            x[u][n][v] = split ? f[v] : f[2 * v];
+            y[u][n][v] = split ? f[4 + v] : f[2 * v + 1];
+          }
+        } else {
+          x[u][n][0] = mine ? __ldcs(row + index(pair, 0, false)) : 0.f;
+          y[u][n][0] = mine ? __ldcs(row + index(pair, 0, true)) : 0.f;
         }
-        const float f[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
+      }
+    }
+    float inv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      inv[u] = 1.f;
+    }
+    if (__any_sync(0xFFFFFFFFu, norm)) {
+      float sq[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sq[u] = 0.f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            sq[u] = fmaf(x[u][n][v], x[u][n][v], sq[u]);
+            sq[u] = fmaf(y[u][n][v], y[u][n][v], sq[u]);
+          }
+        }
+      }
+      for (int o = a.lanes / 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          sq[u] += __shfl_xor_sync(0xFFFFFFFFu, sq[u], o);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        inv[u] = norm ? 1.0f / sqrtf(sq[u] / static_cast<float>(r.head_dim) + r.rms_eps) : 1.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float* row = out + (h0 + u) * r.out_head_stride;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int pair = at(n);
+        if (h0 + u >= heads || pair >= pairs) {
+          continue;
+        }
+        const bool turns = pair < half;   // the others are passed on as they are, NaN and infinities too
+        float f[V], g[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          x[n][v] = split ? f[v] : f[2 * v];
-          y[n][v] = split ? f[4 + v] : f[2 * v + 1];
+          const float p = x[u][n][v] * inv[u] * wa[n][v], w = y[u][n][v] * inv[u] * wb[n][v];
+          f[v] = turns ? fmaf(p, cs[n][v], -(w * sn[n][v])) : p;
+          g[v] = turns ? fmaf(p, sn[n][v], w * cs[n][v]) : w;
         }
-      } else {
-        x[n][0] = mine ? __ldcs(in + index(pair, 0, false)) : 0.f;
-        y[n][0] = mine ? __ldcs(in + index(pair, 0, true)) : 0.f;
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        sq = fmaf(x[n][v], x[n][v], sq);
-        sq = fmaf(y[n][v], y[n][v], sq);
-      }
-    }
-    float inv = 1.f;
-    if (__any_sync(0xFFFFFFFFu, norm)) {
-      for (int o = a.lanes / 2; o > 0; o >>= 1) {
-        sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o);
-      }
-      inv = norm ? 1.0f / sqrtf(sq / static_cast<float>(r.head_dim) + r.rms_eps) : 1.f;
-    }
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int pair = at(n);
-      if (h >= heads || pair >= pairs) {
-        continue;
-      }
-      const bool turns = pair < half;   // the others are passed on as they are, NaN and infinities too
-      float f[V], g[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float u = x[n][v] * inv * wa[n][v], w = y[n][v] * inv * wb[n][v];
-        f[v] = turns ? fmaf(u, cs[n][v], -(w * sn[n][v])) : u;
-        g[v] = turns ? fmaf(u, sn[n][v], w * cs[n][v]) : w;
-      }
-      if constexpr (V == 4) {
-        const bool split = apart && turns;
-        float* to = out + (split ? pair : 2 * pair);
-        *reinterpret_cast<float4*>(to) = split ? make_float4(f[0], f[1], f[2], f[3]) : make_float4(f[0], g[0], f[1], g[1]);
-        *reinterpret_cast<float4*>(to + (split ? half : 4)) =
-            split ? make_float4(g[0], g[1], g[2], g[3]) : make_float4(f[2], g[2], f[3], g[3]);
-      } else {
-        out[index(pair, 0, false)] = f[0];
-        out[index(pair, 0, true)] = g[0];
+        if constexpr (V == 4) {
+          const bool split = apart && turns;
+          float* to = row + (split ? pair : 2 * pair);
+          const float4 first = split ? make_float4(f[0], f[1], f[2], f[3]) : make_float4(f[0], g[0], f[1], g[1]);
+          const float4 second = split ? make_float4(g[0], g[1], g[2], g[3]) : make_float4(f[2], g[2], f[3], g[3]);
+          *reinterpret_cast<float4*>(to) = first;
+          *reinterpret_cast<float4*>(to + (split ? half : 4)) = second;
+        } else {
+          row[index(pair, 0, false)] = f[0];
+          row[index(pair, 0, true)] = g[0];
+        }
       }
     }
   }
