@@ -13,7 +13,8 @@ namespace gufo {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr float kLargest = 0x1p127f;   // magnitudes from here on saturate: what a code stands for is finite then
+constexpr float kLargest = 0x1p127f;
+constexpr uint32_t kLargestBits = 0x7F000000u;
 
 struct AppendArgs {
   CacheView cache;
@@ -26,7 +27,7 @@ struct AppendArgs {
 template <typename Format>
 __global__ void __launch_bounds__(kAppendThreads)
 AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ BatchArgs batch) {
-  __shared__ float tops[2][4];
+  __shared__ uint32_t tops[2][4];
   __shared__ __align__(16) uint8_t image[2][kCacheBlock * kCacheMaxDim];
   GridLaunchDependents();
   GridDependencyWait();
@@ -49,7 +50,7 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
 
   // This warp's new rows: r = row0 + 4 warp + i where start <= r < end.
   float4 x[4][kTimes];
-  float top = 0.f;
+  uint32_t bits = 0;     // of the largest magnitude: as whole numbers they order alike, NaN above all
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = row0 + 4 * warp + i;
@@ -64,28 +65,49 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
         } else {
           x[i][n] = make_float4(__ldcs(from + 4 * f), __ldcs(from + 4 * f + 1), __ldcs(from + 4 * f + 2), __ldcs(from + 4 * f + 3));
         }
-        const auto hold = [&](float& v) {
-          v = v != v ? v : fminf(fmaxf(v, -kLargest), kLargest);
-          top = fmaxf(top, fabsf(v));   // (passes NaN by)
-        };
-        hold(x[i][n].x), hold(x[i][n].y), hold(x[i][n].z), hold(x[i][n].w);
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int n = 0; n < kTimes; ++n) {
+      const auto magnitude = [](float v) { return __float_as_uint(v) & 0x7FFFFFFFu; };
+      bits = max(bits, max(max(magnitude(x[i][n].x), magnitude(x[i][n].y)), max(magnitude(x[i][n].z), magnitude(x[i][n].w))));
     }
   }
   const bool joins = row0 < start;   // rows that stay are in the block
   uint8_t* codes = BlocksOf(c, side, of_head) + static_cast<size_t>(block) * BlockBytes(c.head_dim);
   float* scale_at = ScaleOf(codes, c.head_dim);
   const float was = joins ? *scale_at : 0.f;
+  const auto most_of_side = [&](uint32_t mine) {
+    mine = __reduce_max_sync(0xFFFFFFFFu, mine);
+    if (lane == 0) {
+      tops[side][warp] = mine;
+    }
+    __syncthreads();
+    return max(max(tops[side][0], tops[side][1]), max(tops[side][2], tops[side][3]));
+  };
+  bits = most_of_side(bits);
+  if (__syncthreads_or(bits >= kLargestBits)) {
+    // Magnitudes from there on saturate: what a code stands for is finite. NaN stays, and counts for nothing.
+    uint32_t finite = 0;
+    const auto hold = [&](float& v) {
+      if (v == v) {
+        v = fminf(fmaxf(v, -kLargest), kLargest);
+        finite = max(finite, __float_as_uint(v) & 0x7FFFFFFFu);
+      }
+    };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int n = 0; n < kTimes; ++n) {
+        hold(x[i][n].x), hold(x[i][n].y), hold(x[i][n].z), hold(x[i][n].w);
+      }
+    }
+    bits = most_of_side(finite);
   }
-  if (lane == 0) {
-    tops[side][warp] = top;
-  }
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[side][0], tops[side][1]), fmaxf(tops[side][2], tops[side][3]));
-  int exponent = ScaleExponentOf<Format>(top);
+  int exponent = ScaleExponentOf<Format>(__uint_as_float(bits));
   if (joins) {
     exponent = max(exponent, ExponentOf(was));
   }
@@ -102,9 +124,7 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
       for (int n = 0; n < kTimes; ++n) {
         const int f = lane + 32 * n;
         if (f < fours) {
-          const float4 v = x[i][n];
-          *(reinterpret_cast<uint32_t*>(image[side] + PieceAt(side, 4 * warp + i, f / 4)) + f % 4) =
-              Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+          *(reinterpret_cast<uint32_t*>(image[side] + PieceAt(side, 4 * warp + i, f / 4)) + f % 4) = Format::Encode(x[i][n], inverse);
         }
       }
     }
@@ -124,12 +144,10 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
         }
         uint32_t* to = reinterpret_cast<uint32_t*>(codes + PieceAt(side, 4 * warp + i, f / 4)) + f % 4;
         if (r >= start && r < end) {
-          const float4 v = x[i][n];
-          *to = Format::Encode(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse);
+          *to = Format::Encode(x[i][n], inverse);
         } else if (r < start && exponent > ExponentOf(was)) {
-          const float4 v = DecodeFour<Format>(*to);
-          const float down = was * inverse;   // (0 where the scales are more than 2^149 apart, as the codes are then)
-          *to = Format::Encode(v.x * down, v.y * down, v.z * down, v.w * down);
+          // (was * inverse is 0 where the scales are more than 2^149 apart, as the codes are then.)
+          *to = Format::Encode(DecodeFour<Format>(*to), was * inverse);
         }
       }
     }
@@ -145,17 +163,18 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
 struct RowsArgs {
   CacheView cache;
   float* out[2];
+  int each;       // heads a block of threads
 };
 constexpr int kRowsThreads = 256;
 
-// Grid: (blocks that the batch touches, KV heads, 2). A block's rows are read a word of four codes a
+// Grid: (blocks that the batch touches, KV heads / each, 2). A block's rows are read a word of four codes a
 // lane, rows beside one another from the same sectors, and go out sixteen bytes a lane.
 template <typename Format>
 __global__ void __launch_bounds__(kRowsThreads)
 RowsKernel(const __grid_constant__ RowsArgs a, const __grid_constant__ BatchArgs batch) {
   GridLaunchDependents();
   GridDependencyWait();
-  const int side = blockIdx.z, head = blockIdx.y;
+  const int side = blockIdx.z;
   float* out = a.out[side];
   if (out == nullptr) {
     return;
@@ -167,36 +186,43 @@ RowsKernel(const __grid_constant__ RowsArgs a, const __grid_constant__ BatchArgs
   // The first row of the block, counted from the slot's first (a block may lie outside).
   const int64_t row0 = ((position >> 4) + nth) * kCacheBlock;
   const int fours = c.head_dim / 4;
-  int lanes = 4;      // of a row: a power of two
-  while (lanes < fours) {
-    lanes *= 2;
+  int shift = 2;      // 2^shift lanes a row
+  while (1 << shift < fours) {
+    ++shift;
   }
-  const int f = threadIdx.x & (lanes - 1), first = threadIdx.x / lanes, step = kRowsThreads / lanes;
-  if (f >= fours) {
-    return;
-  }
-  const size_t of_head = static_cast<size_t>(e.slot) * c.kv_heads + head;
+  const int f = threadIdx.x & ((1 << shift) - 1);
   const bool inside = row0 >= 0 && row0 < c.capacity;
-  const uint8_t* block = BlocksOf(c, side, of_head) + static_cast<size_t>(inside ? row0 / kCacheBlock : 0) * BlockBytes(c.head_dim);
-  const float scale = inside ? *ScaleOf(block, c.head_dim) : 0.f;
   const int64_t token0 = row0 - position;     // of the block's first row
-  float4* to = reinterpret_cast<float4*>(out + ((e.row + token0) * c.kv_heads + head) * c.head_dim) + f;
   const int64_t stride = static_cast<int64_t>(c.kv_heads) * fours;
+  const int head0 = blockIdx.y * a.each;
+  const int all = min(a.each, c.kv_heads - head0) * kCacheBlock;    // rows of the heads, one head's after another's
+  const size_t first_head = static_cast<size_t>(e.slot) * c.kv_heads + head0;
+  const size_t of_head = static_cast<size_t>(c.capacity / kCacheBlock) * BlockBytes(c.head_dim);
+  const uint8_t* block = c.sides[side] + first_head * of_head + static_cast<size_t>(inside ? row0 / kCacheBlock : 0) * BlockBytes(c.head_dim);
+  float4* to = reinterpret_cast<float4*>(out + ((e.row + token0) * c.kv_heads + head0) * c.head_dim) + f;
   constexpr int kEach = 4;
-  for (int r0 = first; r0 < kCacheBlock; r0 += kEach * step) {
+  const int step = kRowsThreads >> shift;
+  for (int n0 = threadIdx.x >> shift; n0 < all; n0 += kEach * step) {
     uint32_t word[kEach];
+    float scale[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int r = r0 + i * step;
-      word[i] = inside && r < kCacheBlock ? *(reinterpret_cast<const uint32_t*>(block + PieceAt(side, r, f / 4)) + f % 4) : 0;
+      const int n = n0 + i * step, r = n % kCacheBlock;
+      word[i] = 0;
+      scale[i] = 0.f;
+      if (inside && n < all && f < fours) {
+        const uint8_t* from = block + (n / kCacheBlock) * of_head;
+        word[i] = *(reinterpret_cast<const uint32_t*>(from + PieceAt(side, r, f / 4)) + f % 4);
+        scale[i] = *ScaleOf(from, c.head_dim);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int r = r0 + i * step;
-      if (r < kCacheBlock && token0 + r >= 0 && token0 + r < e.tokens) {
+      const int n = n0 + i * step, r = n % kCacheBlock;
+      if (n < all && f < fours && token0 + r >= 0 && token0 + r < e.tokens) {
         float4 v = DecodeFour<Format>(word[i]);
-        v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
-        __stcs(to + r * stride, v);
+        v.x *= scale[i], v.y *= scale[i], v.z *= scale[i], v.w *= scale[i];
+        __stcs(to + r * stride + (n / kCacheBlock) * fours, v);
       }
     }
   }
@@ -393,14 +419,19 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, co
   if (((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 15) != 0) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "cache8_rows: rows go to 16-byte boundaries");
   }
-  const gufo::RowsArgs a{gufo::ViewOf(*cache), {keys, values}};
+  gufo::RowsArgs a{gufo::ViewOf(*cache), {keys, values}, 1};
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   const auto kernel = cache->c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::RowsKernel<gufo::E4m3> : gufo::RowsKernel<gufo::Int8>;
   return gufo::ForEachRun(
       *batch, gufo::BlocksOfRows,
       [&](const gufo::BatchArgs& b, int blocks) -> int {
-        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(blocks, cache->c.kv_heads, 2), dim3(gufo::kRowsThreads), 0, ctx->stream,
-                                             1, a, b));
+        // Heads a block of threads: 1024 values of a row where that leaves the device full, as what a block costs
+        // by itself is as much as four groups of values a thread (2048 rows of 8 heads of 128, 8 sequences: 54 us
+        // with a head a block).
+        const int wide = 1024 / cache->c.head_dim < cache->c.kv_heads ? 1024 / cache->c.head_dim : cache->c.kv_heads;
+        a.each = static_cast<int64_t>(blocks) * cache->c.kv_heads * 2 / wide >= 4 * ctx->sm_count ? wide : 1;
+        GUFO_CUDA_TRY(gufo::LaunchOverlapped(kernel, dim3(blocks, (cache->c.kv_heads + a.each - 1) / a.each, 2),
+                                             dim3(gufo::kRowsThreads), 0, ctx->stream, 1, a, b));
         ctx->launches.fetch_add(1);
         return GUFO_CUDA_OK;
       });

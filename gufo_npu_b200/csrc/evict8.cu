@@ -334,8 +334,7 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
         if (scale != now) {
           const float by = scale * inverse;
           const auto again = [&](uint32_t w) {
-            const float4 v = DecodeFour<Format>(w);
-            return Format::Encode(v.x * by, v.y * by, v.z * by, v.w * by);
+            return Format::Encode(DecodeFour<Format>(w), by);
           };
           out = make_uint4(again(out.x), again(out.y), again(out.z), again(out.w));
         }
