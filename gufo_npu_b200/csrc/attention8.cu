@@ -349,7 +349,6 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   if (threadIdx.x == 0) {
     nothing = make_uint4(0, 0, 0, 0);
   }
-  // (The second kernel reads the inputs as soon as all blocks of this one have come so far.)
   GridDependencyWait();
   GridLaunchDependents();
   const CacheView& c = a.cache;
@@ -980,9 +979,11 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 // The units that several blocks have parts of: grid (cuts, rows of a unit / R). R query rows a block:
 // the parts' factors, then their sums; groups of a row's threads take a part of the parts each. A row a
 // block where there are few (one long sequence has a hundred parts), four where there are many.
+// (Two blocks an SM, not four: they come while the first kernel's last blocks run, and take shared
+// memory and issue slots from what follows: the verify batch 84 us with four, 70 with two.)
 constexpr int kJoinThreads = 256;
 template <int R>
-__global__ void __launch_bounds__(kJoinThreads, R == 1 ? 2 : 4)
+__global__ void __launch_bounds__(kJoinThreads, 2)
 JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
   constexpr int kRowThreads = kJoinThreads / R, kRowWarps = kRowThreads / 32;
   __shared__ float factor[R][kMostBlocks];
