@@ -34,7 +34,6 @@
 // are written down as they come, 4 bytes against 2 * head_dim / group read for them, and a
 // second kernel turns them into weights and adds those up, one thread a row, in order.
 #include <climits>
-#include <type_traits>
 
 #include "cache8.cuh"
 #include "decode_device.cuh"
@@ -43,7 +42,7 @@
 namespace gufo {
 namespace {
 
-constexpr int kMostUnitCost = 32;
+constexpr int kMostUnitRows = 256;
 constexpr int kShortCapacity = 384;
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
@@ -91,16 +90,19 @@ template <int NS, int RT>
 struct Shape {
   static constexpr int kTile = NS * kCacheBlock;            // rows that a group takes at a time
   static constexpr int kGroups = kWarps / NS;
-  // What a unit costs besides its tiles (queries, the join): some 5 us, as much as so many tiles
-  // of a block that shares its SM with the others.
-  static constexpr int kUnitCost = kMostUnitCost / (NS * NS);
+  // What a unit costs besides its tiles (queries, the join), in tiles: as much as so many rows of the
+  // cache. (The verify batch, heads of 256: 68, 64 and 67 us with 64, 128 and 256 rows; heads of 128:
+  // 50, 46, 48; 100 sequences, heads of 64: 77, 60, 52.)
+  static constexpr int kUnitCost = (NS == 1 ? kMostUnitRows : 128) / kTile;
   static constexpr int kRowBytes = 64 * NS;
   static constexpr int kSlot = kCacheBlock * kRowBytes + 16;   // a block's keys or values, their scale
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
-  // Of threads that an SM holds: by registers (RT == 4: 168 a thread or more), or by shared memory.
-  static constexpr int kBlocks = RT == 4 ? (NS == 4 ? 2 : 3) : NS == 4 ? 3 : 4;
+  // Of threads that an SM holds: as many as keep their sums in registers. (32 sequences of some 2000
+  // rows, heads of 128: 16 query rows 66 us with four, 48 with three; 32 query rows 129 with three,
+  // 95 with two. Heads of 256, 16 query rows: 70 with three, 79 with two.)
+  static constexpr int kBlocks = RT == 4 ? 2 : NS == 4 || RT == 2 ? 3 : 4;
   static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
   static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4)
   static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
@@ -583,302 +585,292 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         acc[rt][m][0] = acc[rt][m][1] = acc[rt][m][2] = acc[rt][m][3] = 0.f;
       }
     }
-    // RA: groups of eight rows that there are.
-    const auto go = [&](auto groups) {
-      constexpr int RA = decltype(groups)::value;
-      int parity = 0;
+    // (All groups of eight rows, also where the sequence has fewer: a second loop for those is code that
+    // the SM fetches in vain; a ragged batch of one to four tokens took 70 us with it and 64 without,
+    // one to eight tokens 157 and 131.)
+    int parity = 0;
 #pragma unroll 1
-      for (int tile = first_tile + group; tile < end_tile; tile += S::kGroups) {
-        if ((tile * NS + member) * kCacheBlock < length) {
-          wait_for(warp);
+    for (int tile = first_tile + group; tile < end_tile; tile += S::kGroups) {
+      if ((tile * NS + member) * kCacheBlock < length) {
+        wait_for(warp);
+      }
+      // Scores of this warp's block.
+      const uint8_t* keys = ring + slot * S::kSlot;
+      next_slot();
+      float s[RT][4];
+      const auto key_words = [&](int seg, int more) {
+        const uint8_t* at = keys + key_place + 1024 * seg + more;
+        return *reinterpret_cast<const uint4*>(4 * seg + t < pieces ? at : reinterpret_cast<const uint8_t*>(&nothing));
+      };
+      // (A block behind the last row that is seen was not copied, and weighs nothing.)
+      const bool there = (tile * NS + member) * kCacheBlock < length;
+      if (!there) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
         }
-        // Scores of this warp's block.
-        const uint8_t* keys = ring + slot * S::kSlot;
-        next_slot();
-        float s[RA][4];
-        const auto key_words = [&](int seg, int more) {
-          const uint8_t* at = keys + key_place + 1024 * seg + more;
-          return *reinterpret_cast<const uint4*>(4 * seg + t < pieces ? at : reinterpret_cast<const uint8_t*>(&nothing));
-        };
-        // (A block behind the last row that is seen was not copied, and weighs nothing.)
-        const bool there = (tile * NS + member) * kCacheBlock < length;
-        if (!there) {
+      } else if constexpr (Format::kWhole) {
+        int d[RT][3][4];      // by the queries' digits
 #pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
-            s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int l = 0; l < 3; ++l) {
+            d[rt][l][0] = d[rt][l][1] = d[rt][l][2] = d[rt][l][3] = 0;
           }
-        } else if constexpr (Format::kWhole) {
-          int d[RA][3][4];      // by the queries' digits
+        }
 #pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
+        for (int seg = 0; seg < NS; ++seg) {
+          const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
             for (int l = 0; l < 3; ++l) {
-              d[rt][l][0] = d[rt][l][1] = d[rt][l][2] = d[rt][l][3] = 0;
-            }
-          }
-#pragma unroll
-          for (int seg = 0; seg < NS; ++seg) {
-            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
-#pragma unroll
-            for (int rt = 0; rt < RA; ++rt) {
-#pragma unroll
-              for (int l = 0; l < 3; ++l) {
-                const uint4 q = query[((rt * NS + seg) * 3 + l) * 32 + lane];
-                MmaWhole(d[rt][l], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
-                MmaWhole(d[rt][l], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
-              }
-            }
-          }
-          // (A digit's sum is at most 256 * 128 * 127: two of them fit an int, the lowest a float.)
-#pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
-            }
-          }
-        } else {
-#pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
-            s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
-          }
-#pragma unroll
-          for (int seg = 0; seg < NS; ++seg) {
-            const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
-            const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-            uint32_t k[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              Format::Decode(w0[j], k[j][0], k[j][2]);
-              Format::Decode(w1[j], k[j][1], k[j][3]);
-            }
-            // Four products at a time, low halves first: an instruction's result is not waited for.
-#pragma unroll
-            for (int rt = 0; rt < RA; ++rt) {
-              uint4 q[4];
-              float d[4][4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                q[j] = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
-                MmaFirst(d[j], k[j], q[j].z, q[j].w);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                MmaMore(d[j], k[j], q[j].x, q[j].y);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                s[rt][i] += (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]);
-              }
+              const uint4 q = query[((rt * NS + seg) * 3 + l) * 32 + lane];
+              MmaWhole(d[rt][l], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
+              MmaWhole(d[rt][l], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
             }
           }
         }
-        const float key_scale = *reinterpret_cast<const float*>(keys + codes_bytes);
-        const int r0 = (tile * NS + member) * kCacheBlock + g;
-        const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
-        uint4 p[RA];             // high pair of rows 0-7, of 8-15; low pairs
-        float sum[RA][2];        // of this lane's weights
-        float own[RA][2];        // what they are taken against
+        // (A digit's sum is at most 256 * 128 * 127: two of them fit an int, the lowest a float.)
 #pragma unroll
-        for (int rt = 0; rt < RA; ++rt) {
+        for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[rt][i] *= factor[rt][i & 1] * key_scale;
-          }
-          if (a.scores != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * rt + 2 * t + (i & 1), row = r0 + 8 * (i >> 1);
-              if (r < task.rows && row < length) {
-                const int flat = task.row0 + r;
-                const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
-                __stcg(a.scores + at * c.capacity + row, s[rt][i]);
-              }
-            }
-          }
-          if (hides) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              s[rt][i] = r0 + 8 * (i >> 1) < seen[rt][i & 1] ? s[rt][i] : -INFINITY;
-            }
-          }
-          float m0 = fmaxf(fmaxf(s[rt][0], s[rt][2]), top[rt][0]), m1 = fmaxf(fmaxf(s[rt][1], s[rt][3]), top[rt][1]);
-          if (__any_sync(0xFFFFFFFFu, m0 > top[rt][0] || m1 > top[rt][1])) {
-#pragma unroll
-            for (int o = 4; o <= 16; o <<= 1) {
-              m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
-              m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
-            }
-          }
-          own[rt][0] = m0, own[rt][1] = m1;
-          if constexpr (NS > 1) {
-            if (g == 0) {
-              *reinterpret_cast<float2*>(&block_top[parity][warp][8 * rt + 2 * t]) = make_float2(m0, m1);
-            }
-          }
-          const float t0 = m0 == -INFINITY ? 0.f : m0, t1 = m1 == -INFINITY ? 0.f : m1;
-          const float e0 = exp2f(s[rt][0] - t0), e1 = exp2f(s[rt][1] - t1), e2 = exp2f(s[rt][2] - t0), e3 = exp2f(s[rt][3] - t1);
-          sum[rt][0] = e0 + e2;
-          sum[rt][1] = e1 + e3;
-          const float x[4] = {e0 * kProbScale, e1 * kProbScale, e2 * kProbScale, e3 * kProbScale};
-          __half high[4], low[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            high[i] = __float2half_rn(x[i]);
-            low[i] = __float2half_rn(x[i] - __half2float(high[i]));
-          }
-          p[rt] = make_uint4(Transpose(PackHalves(high[0], high[1])), Transpose(PackHalves(high[2], high[3])),
-                             Transpose(PackHalves(low[0], low[1])), Transpose(PackHalves(low[2], low[3])));
-          if constexpr (NS > 1) {
-            shared_p[((parity * kWarps + warp) * RT + rt) * 32 + lane] = p[rt];
+            s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
           }
         }
-        Meet<NS>(group);       // the weights are there; the last tile's values and this one's keys are done with
-        load();
-        load();
-        // Where a block has raised the maximum: the sums to it.
-        bool raised = false;
+      } else {
 #pragma unroll
-        for (int rt = 0; rt < RA; ++rt) {
-          float n0 = own[rt][0], n1 = own[rt][1];
-          if constexpr (NS > 1) {
-#pragma unroll
-            for (int b = 0; b < NS; ++b) {
-              const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
-              n0 = fmaxf(n0, of.x), n1 = fmaxf(n1, of.y);
-            }
-          }
-          if (__any_sync(0xFFFFFFFFu, n0 > top[rt][0] || n1 > top[rt][1])) {
-            raised = true;
-            const float keep0 = n0 == top[rt][0] ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == top[rt][1] ? 1.f : exp2f(top[rt][1] - n1);
-            top[rt][0] = n0, top[rt][1] = n1;
-            const float mine0 = own[rt][0] == n0 ? 1.f : exp2f(own[rt][0] - n0), mine1 = own[rt][1] == n1 ? 1.f : exp2f(own[rt][1] - n1);
-            total[rt][0] = total[rt][0] * keep0 + sum[rt][0] * mine0;
-            total[rt][1] = total[rt][1] * keep1 + sum[rt][1] * mine1;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
-            }
-          } else {
-            total[rt][0] += sum[rt][0];
-            total[rt][1] += sum[rt][1];
-          }
+        for (int rt = 0; rt < RT; ++rt) {
+          s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
         }
-        // This warp's dimensions of the group's blocks.
 #pragma unroll
-        for (int b = 0; b < NS; ++b) {
-          const int block = tile * NS + b;
-          if (block * kCacheBlock >= length) {
-            break;
+        for (int seg = 0; seg < NS; ++seg) {
+          const uint4 k0 = key_words(seg, 0), k1 = key_words(seg, 256);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          uint32_t k[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            Format::Decode(w0[j], k[j][0], k[j][2]);
+            Format::Decode(w1[j], k[j][1], k[j][3]);
           }
-          wait_for(group * NS + b);
-          uint8_t* values = ring_of(group * NS + b) + slot * S::kSlot;
-          if constexpr (Format::kHasNan) {
-            // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
-            // others, whose weight of 0 times NaN would: where some do not see all rows of a block, such
-            // values are put into the sums by hand and taken out of the block.
-            if ((block + 1) * kCacheBlock > least) {
-              const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
-              // This warp's pieces: 64 words each.
-              uint32_t* const words = reinterpret_cast<uint32_t*>(values) + 256 * member;
-              const int count = 64 * min(4, (pieces + 1) / 2 * 2 - 4 * member);
-              uint32_t found = 0;
+          // Four products at a time, low halves first: an instruction's result is not waited for.
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                found |= lane + 32 * i < count ? marks(words[lane + 32 * i]) : 0;
-              }
-              if (__any_sync(0xFFFFFFFFu, found != 0)) {
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-#pragma unroll
-                  for (int half = 0; half < 2; ++half) {
-                    const int dim = 8 * g + 2 * m + half;
-                    int row = INT_MAX;      // the first with NaN
-#pragma unroll 1
-                    for (int r = kCacheBlock - 1; r >= 0; --r) {
-                      const uint8_t code = values[PieceAt(1, r, value_piece) + dim % 16];
-                      row = (code & 0x7F) == 0x7F ? block * kCacheBlock + r : row;
-                    }
-#pragma unroll
-                    for (int rt = 0; rt < RA; ++rt) {
-                      acc[rt][m][2 * half] = row < seen[rt][0] ? NAN : acc[rt][m][2 * half];
-                      acc[rt][m][2 * half + 1] = row < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
-                    }
-                  }
-                }
-                __syncwarp();
-#pragma unroll 1
-                for (int i = lane; i < count; i += 32) {
-                  words[i] &= ~((marks(words[i]) >> 7) * 255u);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // ahead of the slot's next copy
-                __syncwarp();
-              }
-            }
-          }
-          // (Read ahead of the values, which the products wait for: the slot is given back behind
-          // those.)
-          float by;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(SharedAddress(values + codes_bytes)) : "memory");
-          by *= 1.f / kProbScale;
-          float each[RA][2];
-#pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
-            each[rt][0] = each[rt][1] = by;
-            if constexpr (NS > 1) {
-              p[rt] = shared_p[((parity * kWarps + group * NS + b) * RT + rt) * 32 + lane];
-              if (raised) {
-                const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
-                each[rt][0] *= of.x == top[rt][0] ? 1.f : exp2f(of.x - top[rt][0]);
-                each[rt][1] *= of.y == top[rt][1] ? 1.f : exp2f(of.y - top[rt][1]);
-              }
-            }
-          }
-          uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = *reinterpret_cast<const uint2*>(values + (value_place ^ (32 * (i & 1))) + 256 * (i >> 1));
-          }
-          uint32_t of[4][4];   // dimensions 2 m, 2 m + 1 of the eight: rows beside one another
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const uint32_t w0 = m < 2 ? v[0].x : v[0].y, w1 = m < 2 ? v[1].x : v[1].y;
-            const uint32_t w2 = m < 2 ? v[2].x : v[2].y, w3 = m < 2 ? v[3].x : v[3].y;
-            Format::Decode(__byte_perm(w0, w1, m & 1 ? 0x7362 : 0x5140), of[m][0], of[m][1]);
-            Format::Decode(__byte_perm(w2, w3, m & 1 ? 0x7362 : 0x5140), of[m][2], of[m][3]);
-          }
-#pragma unroll
-          for (int rt = 0; rt < RA; ++rt) {
+          for (int rt = 0; rt < RT; ++rt) {
+            uint4 q[4];
             float d[4][4];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              MmaFirst(d[m], of[m], p[rt].z, p[rt].w);
+            for (int j = 0; j < 4; ++j) {
+              q[j] = query[(rt * 4 * NS + seg * 4 + j) * 32 + lane];
+              MmaFirst(d[j], k[j], q[j].z, q[j].w);
             }
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              MmaMore(d[m], of[m], p[rt].x, p[rt].y);
+            for (int j = 0; j < 4; ++j) {
+              MmaMore(d[j], k[j], q[j].x, q[j].y);
             }
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                acc[rt][m][i] = fmaf(d[m][i], each[rt][i & 1], acc[rt][m][i]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              s[rt][i] += (d[0][i] + d[1][i]) + (d[2][i] + d[3][i]);
             }
           }
         }
-        next_slot();
-        parity ^= 1;
       }
-    };
-    if constexpr (RT == 1) {
-      go(std::integral_constant<int, 1>());
-    } else if (task.rows <= 8) {
-      go(std::integral_constant<int, 1>());
-    } else if (RT == 2 || task.rows <= 16) {
-      go(std::integral_constant<int, 2>());
-    } else {
-      go(std::integral_constant<int, RT>());
+      const float key_scale = *reinterpret_cast<const float*>(keys + codes_bytes);
+      const int r0 = (tile * NS + member) * kCacheBlock + g;
+      const bool hides = (tile + 1) * kTile > least;     // some rows from some queries
+      uint4 p[RT];             // high pair of rows 0-7, of 8-15; low pairs
+      float sum[RT][2];        // of this lane's weights
+      float own[RT][2];        // what they are taken against
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[rt][i] *= factor[rt][i & 1] * key_scale;
+        }
+        if (a.scores != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * rt + 2 * t + (i & 1), row = r0 + 8 * (i >> 1);
+            if (r < task.rows && row < length) {
+              const int flat = task.row0 + r;
+              const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
+              __stcg(a.scores + at * c.capacity + row, s[rt][i]);
+            }
+          }
+        }
+        if (hides) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[rt][i] = r0 + 8 * (i >> 1) < seen[rt][i & 1] ? s[rt][i] : -INFINITY;
+          }
+        }
+        float m0 = fmaxf(fmaxf(s[rt][0], s[rt][2]), top[rt][0]), m1 = fmaxf(fmaxf(s[rt][1], s[rt][3]), top[rt][1]);
+        if (__any_sync(0xFFFFFFFFu, m0 > top[rt][0] || m1 > top[rt][1])) {
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1) {
+            m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, o));
+            m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, o));
+          }
+        }
+        own[rt][0] = m0, own[rt][1] = m1;
+        if constexpr (NS > 1) {
+          if (g == 0) {
+            *reinterpret_cast<float2*>(&block_top[parity][warp][8 * rt + 2 * t]) = make_float2(m0, m1);
+          }
+        }
+        const float t0 = m0 == -INFINITY ? 0.f : m0, t1 = m1 == -INFINITY ? 0.f : m1;
+        const float e0 = exp2f(s[rt][0] - t0), e1 = exp2f(s[rt][1] - t1), e2 = exp2f(s[rt][2] - t0), e3 = exp2f(s[rt][3] - t1);
+        sum[rt][0] = e0 + e2;
+        sum[rt][1] = e1 + e3;
+        const float x[4] = {e0 * kProbScale, e1 * kProbScale, e2 * kProbScale, e3 * kProbScale};
+        __half high[4], low[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          high[i] = __float2half_rn(x[i]);
+          low[i] = __float2half_rn(x[i] - __half2float(high[i]));
+        }
+        p[rt] = make_uint4(Transpose(PackHalves(high[0], high[1])), Transpose(PackHalves(high[2], high[3])),
+                           Transpose(PackHalves(low[0], low[1])), Transpose(PackHalves(low[2], low[3])));
+        if constexpr (NS > 1) {
+          shared_p[((parity * kWarps + warp) * RT + rt) * 32 + lane] = p[rt];
+        }
+      }
+      Meet<NS>(group);       // the weights are there; the last tile's values and this one's keys are done with
+      load();
+      load();
+      // Where a block has raised the maximum: the sums to it.
+      bool raised = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float n0 = own[rt][0], n1 = own[rt][1];
+        if constexpr (NS > 1) {
+#pragma unroll
+          for (int b = 0; b < NS; ++b) {
+            const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
+            n0 = fmaxf(n0, of.x), n1 = fmaxf(n1, of.y);
+          }
+        }
+        if (__any_sync(0xFFFFFFFFu, n0 > top[rt][0] || n1 > top[rt][1])) {
+          raised = true;
+          const float keep0 = n0 == top[rt][0] ? 1.f : exp2f(top[rt][0] - n0), keep1 = n1 == top[rt][1] ? 1.f : exp2f(top[rt][1] - n1);
+          top[rt][0] = n0, top[rt][1] = n1;
+          const float mine0 = own[rt][0] == n0 ? 1.f : exp2f(own[rt][0] - n0), mine1 = own[rt][1] == n1 ? 1.f : exp2f(own[rt][1] - n1);
+          total[rt][0] = total[rt][0] * keep0 + sum[rt][0] * mine0;
+          total[rt][1] = total[rt][1] * keep1 + sum[rt][1] * mine1;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            acc[rt][m][0] *= keep0, acc[rt][m][1] *= keep1, acc[rt][m][2] *= keep0, acc[rt][m][3] *= keep1;
+          }
+        } else {
+          total[rt][0] += sum[rt][0];
+          total[rt][1] += sum[rt][1];
+        }
+      }
+      // This warp's dimensions of the group's blocks.
+#pragma unroll
+      for (int b = 0; b < NS; ++b) {
+        const int block = tile * NS + b;
+        if (block * kCacheBlock >= length) {
+          break;
+        }
+        wait_for(group * NS + b);
+        uint8_t* values = ring_of(group * NS + b) + slot * S::kSlot;
+        if constexpr (Format::kHasNan) {
+          // A value that is NaN makes NaN of the sums of the queries that see its row, and of no
+          // others, whose weight of 0 times NaN would: where some do not see all rows of a block, such
+          // values are put into the sums by hand and taken out of the block.
+          if ((block + 1) * kCacheBlock > least) {
+            const auto marks = [](uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; };   // of 0x7F, 0xFF
+            // This warp's pieces: 64 words each.
+            uint32_t* const words = reinterpret_cast<uint32_t*>(values) + 256 * member;
+            const int count = 64 * min(4, (pieces + 1) / 2 * 2 - 4 * member);
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              found |= lane + 32 * i < count ? marks(words[lane + 32 * i]) : 0;
+            }
+            if (__any_sync(0xFFFFFFFFu, found != 0)) {
+#pragma unroll
+              for (int m = 0; m < 4; ++m) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const int dim = 8 * g + 2 * m + half;
+                  int row = INT_MAX;      // the first with NaN
+#pragma unroll 1
+                  for (int r = kCacheBlock - 1; r >= 0; --r) {
+                    const uint8_t code = values[PieceAt(1, r, value_piece) + dim % 16];
+                    row = (code & 0x7F) == 0x7F ? block * kCacheBlock + r : row;
+                  }
+#pragma unroll
+                  for (int rt = 0; rt < RT; ++rt) {
+                    acc[rt][m][2 * half] = row < seen[rt][0] ? NAN : acc[rt][m][2 * half];
+                    acc[rt][m][2 * half + 1] = row < seen[rt][1] ? NAN : acc[rt][m][2 * half + 1];
+                  }
+                }
+              }
+              __syncwarp();
+#pragma unroll 1
+              for (int i = lane; i < count; i += 32) {
+                words[i] &= ~((marks(words[i]) >> 7) * 255u);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // ahead of the slot's next copy
+              __syncwarp();
+            }
+          }
+        }
+        // (Read ahead of the values, which the products wait for: the slot is given back behind
+        // those.)
+        float by;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(SharedAddress(values + codes_bytes)) : "memory");
+        by *= 1.f / kProbScale;
+        float each[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          each[rt][0] = each[rt][1] = by;
+          if constexpr (NS > 1) {
+            p[rt] = shared_p[((parity * kWarps + group * NS + b) * RT + rt) * 32 + lane];
+            if (raised) {
+              const float2 of = *reinterpret_cast<const float2*>(&block_top[parity][group * NS + b][8 * rt + 2 * t]);
+              each[rt][0] *= of.x == top[rt][0] ? 1.f : exp2f(of.x - top[rt][0]);
+              each[rt][1] *= of.y == top[rt][1] ? 1.f : exp2f(of.y - top[rt][1]);
+            }
+          }
+        }
+        uint2 v[4];     // this lane's eight dimensions of rows 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = *reinterpret_cast<const uint2*>(values + (value_place ^ (32 * (i & 1))) + 256 * (i >> 1));
+        }
+        uint32_t of[4][4];   // dimensions 2 m, 2 m + 1 of the eight: rows beside one another
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t w0 = m < 2 ? v[0].x : v[0].y, w1 = m < 2 ? v[1].x : v[1].y;
+          const uint32_t w2 = m < 2 ? v[2].x : v[2].y, w3 = m < 2 ? v[3].x : v[3].y;
+          Format::Decode(__byte_perm(w0, w1, m & 1 ? 0x7362 : 0x5140), of[m][0], of[m][1]);
+          Format::Decode(__byte_perm(w2, w3, m & 1 ? 0x7362 : 0x5140), of[m][2], of[m][3]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float d[4][4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            MmaFirst(d[m], of[m], p[rt].z, p[rt].w);
+          }
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            MmaMore(d[m], of[m], p[rt].x, p[rt].y);
+          }
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              acc[rt][m][i] = fmaf(d[m][i], each[rt][i & 1], acc[rt][m][i]);
+            }
+          }
+        }
+      }
+      next_slot();
+      parity ^= 1;
     }
     if (late) {
 #pragma unroll
@@ -1285,7 +1277,7 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
       [&](const gufo::BatchArgs& b, int items) -> int {
         const int64_t units = static_cast<int64_t>(items) * c.kv_heads;
         const int rows = rows_each < 8 * rt ? static_cast<int>(rows_each) : 8 * rt;
-        if (units * (c.capacity / gufo::kCacheBlock + 1 + gufo::kMostUnitCost) > INT32_MAX) {
+        if (units * (c.capacity / gufo::kCacheBlock + 1 + gufo::kMostUnitRows / gufo::kCacheBlock) > INT32_MAX) {
           return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
         }
         const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, units, rows, ns, rt)
