@@ -19,6 +19,7 @@ class Batch:
 
     def __init__(self, device: int, positions, tokens: Optional[Sequence[int]], slots: Optional[Sequence[int]]):
         check_ints("cache8", device, positions)
+        self.device = device
         n = positions.numel()
         for name, values in (("tokens", tokens), ("slots", slots)):
             if values is not None and len(values) != n:
@@ -113,6 +114,11 @@ class CudaCache8:
         without), in `slots` (0, 1, ... without)."""
         return Batch(self.ctx.device, positions, tokens, slots)
 
+    def _ctx_of(self, batch: Batch) -> Context:
+        if batch.device != self.ctx.device:
+            raise ValueError("cache8: the batch is another device's")
+        return self.ctx
+
     def scratch(self, heads: int, tokens: int, accumulate: bool = False) -> Scratch:
         """Scratch of attend_device calls with up to `tokens` query tokens in all."""
         nbytes = C.c_size_t()
@@ -122,13 +128,13 @@ class CudaCache8:
 
     def append_device(self, batch: Batch, keys, values) -> None:
         """Writes the batch's rows, [rows, kv_heads, head_dim] each, at their positions."""
-        ctx = self.ctx
+        ctx = self._ctx_of(batch)
         ctx._check(_capi.native.cache8_append(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.kv_heads,
                                               self.head_dim, keys, values))
 
     def rows_device(self, batch: Batch, keys, values) -> None:
         """What the rows of an append with this batch stand for, into contiguous [rows, kv_heads, head_dim]."""
-        ctx = self.ctx
+        ctx = self._ctx_of(batch)
         ctx._check(_capi.native.cache8_rows(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.kv_heads,
                                             self.head_dim, keys, values))
 
@@ -137,7 +143,9 @@ class CudaCache8:
         """out = softmax(queries K^T scale) V [* sigmoid(gate)] for [rows, heads, head_dim] query rows. Token t of
         a sequence sees the rows up to position + t, or the first visible[...] (int32, a value per row of
         queries). `accumulate` adds what each cached row was given to `weights`."""
-        ctx = self.ctx
+        ctx = self._ctx_of(batch)
+        if scratch.ctx.device != ctx.device:
+            raise ValueError("cache8: the scratch is another device's")
         ctx._check(_capi.native.cache8_attend(ctx._address, ctx.device, self.handle, batch.args, batch.rows, self.head_dim,
                                               queries, out, gate, visible, scale, accumulate, scratch.ptr, scratch.bytes))
 
@@ -155,6 +163,6 @@ class CudaCache8:
             slots = (C.c_int * batch.sequences)(*into_slots)
         if into is not None and into.ctx is not self.ctx:
             raise ValueError("cache8: both caches belong to one context")
-        ctx = self.ctx
+        ctx = self._ctx_of(batch)
         ctx._check(_capi.native.cache8_evict(ctx._address, ctx.device, self.handle, batch.args, batch.sequences, self.kv_heads,
                                              budget, first, last, kept, held, into.handle if into is not None else 0, slots))

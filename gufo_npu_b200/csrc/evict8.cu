@@ -11,7 +11,7 @@
 // magnitude, and rounds what had another scale. In place, the rows a block receives come from
 // its own place or behind it, so blocks written in order overwrite nothing that is still wanted:
 // a cluster of thread blocks does the next 64 blocks of a head at a time, all read before any
-// is written. Blocks whose rows stay where they are are not touched. Into another cache there
+// is written. Blocks that stay as they are are not touched. Into another cache there
 // is no order to keep, and every block is a warp of its own.
 #include <cooperative_groups.h>
 
@@ -276,12 +276,14 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
   const int bytes = BlockBytes(c.head_dim);
   const int pieces = c.head_dim / 16;   // of a row
   const int blocks = (a.budget + kCacheBlock - 1) / kCacheBlock;
+  // In place the last block may keep its first rows where they are, and lose others.
+  const bool loses = kInPlace && a.budget % kCacheBlock != 0 && batch.positions[e.index] > a.budget;
   for (int first = blockIdx.x * kMoveWarps; first - static_cast<int>(blockIdx.x * kMoveWarps) < blocks;
        first += gridDim.x * kMoveWarps) {   // (in place every block of the cluster goes round as often)
     const int block = first + warp;
     const int row = block * kCacheBlock + lane;
     const int mine = block < blocks && lane < kCacheBlock && row < a.budget ? kept[row] : -1;
-    const bool moves = __any_sync(0xFFFFFFFFu, mine >= 0 && (!kInPlace || mine != row));
+    const bool moves = __any_sync(0xFFFFFFFFu, mine >= 0 && (!kInPlace || mine != row)) || (loses && block == blocks - 1);
     const float was = moves && mine >= 0 ? *ScaleOf(from + static_cast<size_t>(mine / kCacheBlock) * bytes, c.head_dim) : 0.f;
     uint4 word[kTimes];
     float top = 0.f;
@@ -332,7 +334,7 @@ MoveKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchArg
         }
         uint4 out = word[i];
         if (scale != now) {
-          const float by = scale * inverse;
+          const float by = fminf(scale * inverse, 0x1p127f);   // (beyond: of zeros beside much smaller rows, or alone)
           const auto again = [&](uint32_t w) {
             return Format::Encode(DecodeFour<Format>(w), by);
           };

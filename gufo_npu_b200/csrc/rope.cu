@@ -213,14 +213,14 @@ int CheckRope(const gufo_cuda_rope_params* p) {
   if (p->scaling != GUFO_CUDA_ROPE_UNSCALED && p->scaling != GUFO_CUDA_ROPE_LINEAR && !by_parts) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "rope: unknown scaling");
   }
-  if (p->scaling != GUFO_CUDA_ROPE_UNSCALED && (!(p->factor > 0.0) || !std::isfinite(p->factor))) {
+  if (p->scaling != GUFO_CUDA_ROPE_UNSCALED && (!(p->factor > 0.0) || !std::isfinite(p->factor) || !std::isfinite(1.0 / p->factor))) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "rope: the scaling's factor is above 0");
   }
   if (by_parts && (!(p->original_positions > 0.0) || !std::isfinite(p->original_positions) || !(p->slow_turns > 0.0) ||
                    !(p->fast_turns > p->slow_turns) || !std::isfinite(p->fast_turns))) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "rope: by parts takes original_positions > 0 and fast_turns > slow_turns > 0");
   }
-  if (!std::isfinite(p->magnitude)) {
+  if (!std::isfinite(static_cast<float>(p->magnitude))) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "rope: the magnitude is finite");
   }
   return GUFO_CUDA_OK;

@@ -438,7 +438,7 @@ typedef struct gufo_cuda_rope_params {
   int layout;
   int scaling;
   double theta;               /* > 1 */
-  double factor;              /* LINEAR, BY_PARTS: > 0 */
+  double factor;              /* LINEAR, BY_PARTS: > 0, as is its reciprocal */
   double original_positions;  /* BY_PARTS: > 0 */
   double fast_turns, slow_turns; /* BY_PARTS: fast > slow > 0 */
   double magnitude; /* factor of the rotated values; 0: 1, BY_PARTS 0.1 ln(factor) + 1 (at least 1) */
@@ -537,7 +537,8 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
  *   out = softmax(q K^T * scale) V  [* sigmoid(gate)]
  * Token t of a sequence sees rows 0 .. positions[i] + t (the rows of an append with the same
  * batch included), or the first visible[...] rows where `visible` is given; a token that
- * sees no row gets zeros. fp32 on the device, strides in floats; heads is a multiple of
+ * sees no row gets zeros. Sums of exp(score - largest score) times values are fp32: of values
+ * near its largest they are infinite. fp32 on the device, strides in floats; heads is a multiple of
  * kv_heads. `out` overlaps none of the inputs.
  * accumulate != 0 (caches with weights): adds the softmax weights, summed over the sequence's
  * tokens and the query heads of a KV head, to the rows' weights.
@@ -570,11 +571,11 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
  * (batch->tokens is not read): for each KV head the first `first` rows stay, the last `last`
  * ones, and of the rows between those of largest weight (of equal ones the lowest row; NaN
  * counts as least), as far as the budget goes in this order. They move together, in their old
- * order, to rows 0 .. budget - 1 with their weights; blocks get the scale of what they hold
- * now. What stands in the rows behind them counts for nothing then. kept (device int32 [batch sequences][kv_heads]
- * [budget]) receives the rows that stayed, -1 behind them where a sequence held fewer than
- * budget, held (device int32 [batch sequences], may be NULL) the rows it holds now,
- * min(positions[i], budget); held may not be positions. Queries keep the positions their
+ * order, to rows 0 .. budget - 1 with their weights; a block whose rows change gets the scale
+ * of what it holds now. What stands in the rows behind them counts for nothing then. kept
+ * (device int32 [batch sequences][kv_heads][budget]) receives the rows that stayed, -1 behind
+ * them where a sequence held fewer than budget, held (device int32 [batch sequences], may be
+ * NULL) the rows it holds now, min(positions[i], budget); held may not be positions. Queries keep the positions their
  * keys were turned by: rotary positions do not go back with the rows.
  * into != 0: the rows go to slots into_slots (host; NULL: the same slots) of that cache
  * instead, which has the same kv_heads, head_dim and format and room for budget rows, and

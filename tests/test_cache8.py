@@ -49,7 +49,8 @@ def test_frequencies(lib, rope_dim, theta, scaling, more):
 @pytest.mark.parametrize("kw, status", [
     ({"rope_dim": 0}, 2), ({"rope_dim": 3}, 2), ({"rope_dim": 514}, 2), ({"rope_dim": -2}, 2), ({"theta": 1.0}, 1),
     ({"theta": float("nan")}, 1), ({"theta": float("inf")}, 1), ({"scaling": "linear", "factor": 0.0}, 1),
-    ({"scaling": "linear", "factor": -1.0}, 1), ({"scaling": "by_parts", "original_positions": 0.0}, 1),
+    ({"scaling": "linear", "factor": -1.0}, 1), ({"scaling": "linear", "factor": 1e-310}, 1), ({"magnitude": 1e300}, 1),
+    ({"scaling": "by_parts", "original_positions": 0.0}, 1),
     ({"scaling": "by_parts", "original_positions": 100.0, "fast_turns": 1.0, "slow_turns": 1.0}, 1),
     ({"scaling": "by_parts", "original_positions": 100.0, "slow_turns": 0.0}, 1), ({"magnitude": float("nan")}, 1)])
 def test_frequencies_refused(lib, kw, status):

@@ -156,6 +156,28 @@ def test_append_takes_rows_as_they_lie(ctx):
             np.testing.assert_array_equal(got[side, h], p.ref.values(side, 0, h, 23)[3:])
 
 
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("head_dim, kv_heads", [(16, 8), (48, 5), (112, 3), (64, 32), (128, 16)])
+def test_rows_of_many_heads(ctx, form, head_dim, kv_heads):
+    """Ragged appends and reads of many heads: whole blocks written together, rows read from inside a block."""
+    p = Pair(ctx, 3, kv_heads, head_dim, 96, form)
+    tokens = [90, 37, 16]
+    n = sum(tokens)
+    p.append([5, 0, 40], tokens, draw(1, n, kv_heads, head_dim), draw(2, n, kv_heads, head_dim), [1, 2, 0])
+    first, count, slots = [3, 20, 41], [60, 17, 14], [1, 2, 0]
+    total = sum(count)
+    out = torch.full((2, total, kv_heads, head_dim), float("nan"), device=DEV)
+    torch.cuda.synchronize()
+    p.gpu.rows_device(p.gpu.batch(ints(*first), count, slots), out[0], out[1])
+    ctx.synchronize()
+    got, at = out.cpu().numpy(), 0
+    for f, c, s in zip(first, count, slots):
+        for side in range(2):
+            for h in range(kv_heads):
+                np.testing.assert_array_equal(got[side, at:at + c, h], p.ref.values(side, s, h, f + c)[f:])
+        at += c
+
+
 def test_rows_outside_are_zeros(ctx):
     p = Pair(ctx, 2, 1, 16, 32, "e4m3")
     p.fill([32, 32])
@@ -280,6 +302,74 @@ def test_attend_over_long_contexts(ctx, form, heads, kv_heads, head_dim, length,
     # The same again, to the bit: sums are taken in one order, and the scratch is as it was.
     for _ in range(3):
         np.testing.assert_array_equal(attend(p, [length - tokens], [tokens], q, scratch=scratch), out)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("heads, kv_heads, head_dim, most", [
+    (4, 4, 64, 1), (4, 2, 48, 8), (12, 1, 64, 8), (32, 8, 128, 1), (8, 2, 112, 4), (6, 1, 128, 8), (8, 2, 256, 1), (8, 2, 256, 4),
+    (9, 3, 192, 8), (40, 2, 256, 2)])
+def test_attend_shares_ragged_sequences_out(ctx, form, heads, kv_heads, head_dim, most):
+    """Sequences of one row to a thousand, whose tiles many blocks take parts of: every group of query rows, ragged."""
+    lengths = [9, 15, 1033, 700, 64, 65, 1, 400, 1040]
+    tokens = [min(n, most) for n in (1, 2, 8, 3, 4, 8, 1, 5, 2)]
+    p = Pair(ctx, 9, kv_heads, head_dim, 1040, form)
+    p.fill(lengths)
+    rows = sum(tokens)
+    q, gate = (draw(5, rows, heads, head_dim) * 1.5).to(DEV), draw(6, rows, heads, head_dim).to(DEV)
+    slots = [(4 * i) % 9 for i in range(9)]
+    positions = [lengths[s] - t if lengths[s] >= t else 0 for s, t in zip(slots, tokens)]
+    out = attend(p, positions, tokens, q, gate, slots=slots)
+    check_attend(p, positions, tokens, q, out, gate, slots=slots)
+    # The tokens in any order, some that see nothing, and their weights.
+    seen = [(331 * i * i) % 1041 if i % 4 else 0 for i in range(rows)]
+    p.gpu.weights.zero_()
+    out = attend(p, positions, tokens, q, slots=slots, visible=seen, accumulate=True)
+    given = check_attend(p, positions, tokens, q, out, slots=slots, visible=seen)
+    got = p.gpu.weights.cpu().numpy()
+    for slot in range(9):
+        # (as in test_attend_adds_up_weights, for each of up to 8 tokens' 20 heads)
+        np.testing.assert_allclose(got[slot], given.get(slot, np.zeros((kv_heads, 1040))), rtol=2.0 ** -23, atol=3e-5 * 8)
+
+
+@pytest.mark.parametrize("form, sequences, heads, kv_heads, head_dim, most", [
+    ("int8", 130, 10, 5, 64, 3), ("e4m3", 70, 56, 14, 128, 4), ("e4m3", 33, 32, 16, 256, 3)])
+def test_attend_with_more_units_than_blocks(ctx, form, sequences, heads, kv_heads, head_dim, most):
+    """Blocks that go through several sequences' heads, and share the last of them with the next block."""
+    capacity = 400
+    p = Pair(ctx, sequences, kv_heads, head_dim, capacity, form, weights=False)
+    lengths = [most + (i * 149) % (capacity + 1 - most) for i in range(sequences)]
+    # One content for all slots (the reference holds one): a sequence is told by its length and its queries.
+    one = R.Cache(1, kv_heads, head_dim, capacity, form)
+    k, v = draw(1, capacity, kv_heads, head_dim), draw(2, capacity, kv_heads, head_dim)
+    one.append(0, 0, (k.numpy(), v.numpy()))
+    kd, vd = k.to(DEV), v.to(DEV)
+    torch.cuda.synchronize()
+    for slot in range(sequences):
+        p.gpu.append_device(p.gpu.batch(ints(0), [capacity], [slot]), kd, vd)
+    p.ctx.synchronize()
+    p.ref = one
+    tokens = [1 + i % most for i in range(sequences)]
+    rows = sum(tokens)
+    q = (draw(5, rows, heads, head_dim) * 1.5).to(DEV)
+    positions = [n - t for n, t in zip(lengths, tokens)]
+    out = attend(p, positions, tokens, q)
+    check_attend(p, positions, tokens, q, out, slots=[0] * sequences)
+
+
+def test_scratch_is_anybodys(ctx):
+    """One scratch, full of NaN, for calls of different shapes one behind another."""
+    p = Pair(ctx, 4, 2, 128, 1024, "e4m3")
+    p.fill([1000, 30, 500, 1024])
+    q = draw(5, 16, 8, 128).to(DEV)
+    scratch = p.gpu.scratch(8, 16, accumulate=True)
+    nan = np.full(scratch.bytes // 4, np.nan, dtype=np.float32)
+    for tokens in ([1, 1, 1, 1], [4, 4, 4, 4], [0, 0, 0, 1], [1, 8, 2, 0]):
+        ctx.upload(scratch.ptr, nan)
+        n = sum(tokens)
+        for accumulate in (False, True, False):
+            positions = [a - b for a, b in zip((1000, 30, 500, 1024), tokens)]
+            out = attend(p, positions, tokens, q[:n], accumulate=accumulate, scratch=scratch)
+            check_attend(p, positions, tokens, q[:n], out)
 
 
 def test_attend_with_peaked_and_flat_scores(ctx):
@@ -517,6 +607,21 @@ def test_evict_in_place_over_many_blocks(ctx, form):
     p.same(1, 16)
 
 
+@pytest.mark.parametrize("other", [False, True])
+def test_evict_of_many_rows(ctx, other):
+    """More rows than a thread holds weights of at a time, with and without ties."""
+    rows, budget = [20000, 4097, 16385], 6001
+    p = Pair(ctx, 3, 1, 16, 20000, "int8")
+    p.fill(rows)
+    for ties in (False, True):
+        set_weights(p, 5, ties)
+        into = Pair(ctx, 3, 1, 16, 6016, "int8") if other else None
+        check_evict(p, rows, budget, 4, 100, evict(p, rows, budget, 4, 100, into=into, into_slots=[2, 1, 0] if other else None),
+                    into=into, into_slots=[2, 1, 0] if other else None)
+        rows = rows if other else [min(n, budget) for n in rows]
+        budget -= 3000
+
+
 def test_evict_goes_by_any_weight(ctx):
     """Negative weights, zeros of both signs, infinities, NaN last; the positions left alone."""
     p = Pair(ctx, 1, 1, 16, 64, "e4m3")
@@ -550,6 +655,52 @@ def test_evict_tightens_scales(ctx):
     y = draw(2, 1, 1, 16) * 0.5
     p.append([39], [1], y, y)
     p.same(0, 40)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("other", [False, True])
+def test_evict_of_zeros_from_under_a_large_scale(ctx, form, other):
+    """Zeros that shared a scale with large rows, by themselves and beside the smallest numbers: zeros they stay."""
+    p = Pair(ctx, 1, 1, 32, 96, form)
+    x = torch.zeros(96, 1, 32)
+    x[0:16:2] = draw(1, 8, 1, 32) * 2.0 ** 100        # rows 1, 3, ...: zeros under their scale
+    x[16:32] = draw(2, 16, 1, 32)
+    x[16:32:4] = 0.0
+    x[32:48] = 1e-40 * torch.arange(32)
+    x[64:80] = draw(3, 16, 1, 32) * 2.0 ** -100
+    x[80:96] = float("inf")
+    x[81:96:3] = 0.0
+    p.append([0], [96], x, -x)
+    for rows in (list(range(1, 16, 2)) + [16, 20, 24, 28] + list(range(32, 37)), list(range(1, 16, 2)) + list(range(64, 74)),
+                 [81, 84, 87], [16, 81]):
+        w = torch.zeros(1, 1, 96)
+        w[0, 0, rows] = 1.0
+        q = Pair(ctx, 1, 1, 32, 96, form)
+        q.append([0], [96], x, -x)
+        q.gpu.weights.copy_(w)
+        torch.cuda.synchronize()
+        q.ref.weights[:] = w.numpy()
+        into = Pair(ctx, 1, 1, 32, 96, form) if other else None
+        check_evict(q, [96], len(rows), 0, 0, evict(q, [96], len(rows), 0, 0, into=into), into=into)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("other", [False, True])
+def test_evict_tightens_the_last_block(ctx, form, other):
+    """The last block keeps its first rows in their places and loses a large one: what comes after it is held as finely as beside
+    those rows alone, in place as in another cache."""
+    p = Pair(ctx, 1, 1, 16, 48, form)
+    x = draw(1, 40, 1, 16)
+    x[38] *= 1000.0
+    p.append([0], [40], x, x)
+    p.gpu.weights.copy_(torch.arange(48, 0, -1).float().view(1, 1, 48))
+    torch.cuda.synchronize()
+    p.ref.weights[:] = p.gpu.weights.cpu().numpy()
+    into = Pair(ctx, 1, 1, 16, 48, form) if other else None
+    check_evict(p, [40], 37, 0, 0, evict(p, [40], 37, 0, 0, into=into), into=into)
+    y = draw(2, 4, 1, 16)
+    (into or p).append([37], [4], y, y)
+    (into or p).same(0, 41)
 
 
 # ---- as they are used together ----------------------------------------------------------
@@ -685,6 +836,15 @@ def test_refusals(ctx):
         gpu.evict_device(b, 8, kept, held=ints(0))
     with pytest.raises(ValueError):
         gpu.batch(at, tokens=[1])
+    # Batches and scratch of another device (as they would be: there may be one device only).
+    elsewhere = gpu.batch(at)
+    elsewhere.device = 1
+    foreign = type("Scratch", (), {"ctx": type("Context", (), {"device": 1}), "ptr": scratch.ptr, "bytes": scratch.bytes})
+    for call, *args in ((gpu.append_device, elsewhere, k, k), (gpu.rows_device, elsewhere, k, k),
+                        (gpu.attend_device, elsewhere, out, out, scratch), (gpu.attend_device, b, out, out, foreign),
+                        (gpu.evict_device, elsewhere, 8, kept)):
+        with pytest.raises(ValueError):
+            call(*args)
     for args in ((0, 1, 64, 64), (4097, 1, 64, 64), (1, 0, 64, 64), (1, 1, 8, 64), (1, 1, 72, 64), (1, 1, 272, 64), (1, 1, 64, 0),
                  (1, 1, 64, 24), (1, 1, 64, 1 << 29)):
         with pytest.raises(GufoCudaError) as e:
