@@ -508,10 +508,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
       top = __reduce_max_sync(0xFFFFFFFFu, top);
       if constexpr (Format::kWhole) {
-        // Whole numbers of 23 bits (the largest 2^21 .. 2^22) as three signed bytes, base 256:
-        // rounded to half of 2^-21 of the largest. A row that is not finite: any, its factor is NaN.
-        const int e = min(max(static_cast<int>(top >> 23), 23), 250);
-        const float up = PowerOfTwo(148 - e);
+        // Whole numbers of 24 bits, the largest as near to three signed bytes' most (base 256: 127 * 65793) as a
+        // power of two takes it: rounded to half of 2^-23 of the largest, of 2^-22 where its fraction is above
+        // 1.992. A row that is not finite: any, its factor is NaN.
+        const int e = min(max(static_cast<int>(top >> 23), 23), 254);
+        const int by = (top & 0x7FFFFFu) <= 0x7EFEFEu ? 149 - e : 148 - e;
+        const float up = PowerOfTwo(by);
 #pragma unroll
         for (int i = 0; i < kTimes; ++i) {
           const int f = lane + 32 * i;     // dimensions 64 seg + 16 c + 4 j ..
@@ -537,11 +539,11 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           }
         }
         if (lane == 0) {
-          row_factor[r] = top < 0x7F800000u ? a.scale * PowerOfTwo(e - 148) : NAN;
+          row_factor[r] = top < 0x7F800000u ? a.scale * PowerOfTwo(-by) : NAN;
         }
       } else {
         // The largest to 2^14 .. 2^15. (Products with codes of up to 448 and their sums stay in fp32's range.)
-        const int e = min(max(static_cast<int>(top >> 23), 16), 250);
+        const int e = min(max(static_cast<int>(top >> 23), 16), 254);
         const float up = PowerOfTwo(141 - e);
 #pragma unroll
         for (int i = 0; i < kTimes; ++i) {

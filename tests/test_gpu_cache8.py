@@ -385,6 +385,20 @@ def test_attend_with_peaked_and_flat_scores(ctx):
         check_attend(p, [3999, 3999], [1, 1], tiny, attend(p, [3999, 3999], [1, 1], tiny, scale=0.125 / size), scale=0.125 / size)
 
 
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("largest", [2.0 ** -130, 2.0 ** -100, 1.99, 1.9922, 1.99225, 1.9999, 2.0 ** 123.5, 2.0 ** 124.5, 2.0 ** 127, 3.4e38])
+def test_attend_with_queries_of_any_size(ctx, form, largest):
+    """Largest values on both sides of where the queries' scaling changes, to the ends of fp32; the scale makes up for it."""
+    p = Pair(ctx, 1, 1, 64, 512, form)
+    k, v = draw(1, 400, 1, 64) * 2.0 ** -60, draw(2, 400, 1, 64)
+    p.append([0], [400], k, v)
+    q = draw(5, 2, 4, 64)
+    q = (q.double() / q.abs().amax(-1, keepdim=True) * largest).float().to(DEV)
+    scale = float(np.float32(min(2.0 ** 62 / largest, 2.0 ** 126)))
+    out = attend(p, [398], [2], q, scale=scale)
+    check_attend(p, [398], [2], q, out, scale=scale)
+
+
 def test_attend_hides_what_is_not_seen(ctx):
     """Rows behind the ones a token sees hold NaN, and change nothing; tokens that see nothing get zeros."""
     p = Pair(ctx, 3, 2, 64, 64, "e4m3")
