@@ -330,8 +330,9 @@ __device__ __forceinline__ void Note(const AttendArgs& a, const QueryRow& q, flo
   }
 }
 
-// Grid: resident blocks.
-template <typename Format, int NS, int RT>
+// Grid: resident blocks. W: the scores are written down. (Apart, as what the loop has to fetch counts: with
+// the stores behind a test in it a verify batch that writes none took 97 us, not 63.)
+template <typename Format, int NS, int RT, bool W>
 __global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
   using S = Shape<NS, RT>;
@@ -339,6 +340,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores
   __shared__ int row_seen[8 * RT];
+  __shared__ float* row_scores[W ? 8 * RT : 1];      // where a query row's scores are written
   __shared__ __align__(8) float block_top[2][kWarps][8 * RT];    // what a block's weights are taken against
   __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT], row_total[8 * RT];
   __shared__ Shares shares;
@@ -430,6 +432,10 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     if (threadIdx.x < 8 * RT) {
       const int r = min(static_cast<int>(threadIdx.x), task.rows - 1);
       row_seen[threadIdx.x] = SeenBy(a, task.e, task.position, (task.row0 + r) / a.group);
+      if constexpr (W) {
+        const QueryRow q(a, task, kh, r);
+        row_scores[threadIdx.x] = a.scores + (q.token * a.heads + q.head) * c.capacity;
+      }
     }
     __syncthreads();
     int length = 0, least = INT_MAX;
@@ -689,14 +695,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         for (int i = 0; i < 4; ++i) {
           s[rt][i] *= factor[rt][i & 1] * key_scale;
         }
-        if (a.scores != nullptr) {
+        if constexpr (W) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 8 * rt + 2 * t + (i & 1), row = r0 + 8 * (i >> 1);
             if (r < task.rows && row < length) {
-              const int flat = task.row0 + r;
-              const int64_t at = (static_cast<int64_t>(task.e.row) + flat / a.group) * a.heads + kh * a.group + flat % a.group;
-              __stcg(a.scores + at * c.capacity + row, s[rt][i]);
+              __stcg(row_scores[r] + row, s[rt][i]);
             }
           }
         }
@@ -1121,7 +1125,7 @@ constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
 constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
 size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * ((kPartialFloats + kStatsFloats) * sizeof(float) + 4 * 32); }
 
-template <typename Format, int NS, int RT>
+template <typename Format, int NS, int RT, bool W>
 int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t units, int rows) {
   using S = Shape<NS, RT>;
   const int blocks = Sms(ctx) * S::kBlocks;
@@ -1132,12 +1136,12 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
                 "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
   if (ctx->device >= 64 || !configured[ctx->device].load()) {
-    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     if (ctx->device < 64) {
       configured[ctx->device].store(true);
     }
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT>, dim3(a.undivided ? static_cast<int>(units) : blocks), dim3(kThreads), S::kBytes,
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT, W>, dim3(a.undivided ? static_cast<int>(units) : blocks), dim3(kThreads), S::kBytes,
                                  ctx->stream, 1, a, b));
   ctx->launches.fetch_add(1);
   if (a.undivided) {
@@ -1153,18 +1157,18 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
   return GUFO_CUDA_OK;
 }
 
-template <typename Format>
+template <typename Format, bool W>
 int PickAttend(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int64_t units, int rows, int ns, int rt) {
   switch (ns * 8 + rt) {
-    case 8 + 1: return LaunchAttend<Format, 1, 1>(ctx, a, b, units, rows);
-    case 8 + 2: return LaunchAttend<Format, 1, 2>(ctx, a, b, units, rows);
-    case 8 + 4: return LaunchAttend<Format, 1, 4>(ctx, a, b, units, rows);
-    case 16 + 1: return LaunchAttend<Format, 2, 1>(ctx, a, b, units, rows);
-    case 16 + 2: return LaunchAttend<Format, 2, 2>(ctx, a, b, units, rows);
-    case 16 + 4: return LaunchAttend<Format, 2, 4>(ctx, a, b, units, rows);
-    case 32 + 1: return LaunchAttend<Format, 4, 1>(ctx, a, b, units, rows);
-    case 32 + 2: return LaunchAttend<Format, 4, 2>(ctx, a, b, units, rows);
-    default: return LaunchAttend<Format, 4, 4>(ctx, a, b, units, rows);
+    case 8 + 1: return LaunchAttend<Format, 1, 1, W>(ctx, a, b, units, rows);
+    case 8 + 2: return LaunchAttend<Format, 1, 2, W>(ctx, a, b, units, rows);
+    case 8 + 4: return LaunchAttend<Format, 1, 4, W>(ctx, a, b, units, rows);
+    case 16 + 1: return LaunchAttend<Format, 2, 1, W>(ctx, a, b, units, rows);
+    case 16 + 2: return LaunchAttend<Format, 2, 2, W>(ctx, a, b, units, rows);
+    case 16 + 4: return LaunchAttend<Format, 2, 4, W>(ctx, a, b, units, rows);
+    case 32 + 1: return LaunchAttend<Format, 4, 1, W>(ctx, a, b, units, rows);
+    case 32 + 2: return LaunchAttend<Format, 4, 2, W>(ctx, a, b, units, rows);
+    default: return LaunchAttend<Format, 4, 4, W>(ctx, a, b, units, rows);
   }
 }
 
@@ -1282,8 +1286,11 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
         if (units * (c.capacity / gufo::kCacheBlock + 1 + gufo::kMostUnitRows / gufo::kCacheBlock) > INT32_MAX) {
           return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
         }
-        const int run = c.format == GUFO_CUDA_CACHE8_E4M3 ? gufo::PickAttend<gufo::E4m3>(ctx, a, b, units, rows, ns, rt)
-                                                          : gufo::PickAttend<gufo::Int8>(ctx, a, b, units, rows, ns, rt);
+        const bool e4m3 = c.format == GUFO_CUDA_CACHE8_E4M3;
+        const int run = a.scores != nullptr ? (e4m3 ? gufo::PickAttend<gufo::E4m3, true>(ctx, a, b, units, rows, ns, rt)
+                                                    : gufo::PickAttend<gufo::Int8, true>(ctx, a, b, units, rows, ns, rt))
+                                            : (e4m3 ? gufo::PickAttend<gufo::E4m3, false>(ctx, a, b, units, rows, ns, rt)
+                                                    : gufo::PickAttend<gufo::Int8, false>(ctx, a, b, units, rows, ns, rt));
         if (run != GUFO_CUDA_OK || a.scores == nullptr) {
           return run;
         }
