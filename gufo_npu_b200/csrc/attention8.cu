@@ -2,7 +2,11 @@
 //
 // What bounds it. The cache is read once, two bytes a row and dimension of a KV head: far into
 // the contexts that is all the time there is, if loads are never waited for and the arithmetic
-// stays hidden under them. Short contexts are bound by latency.
+// stays hidden under them: one int8 sequence of 131000 rows of 4 heads of 256 63 us, 4.3 TB/s, of
+// which the loop alone takes 4.6; half of all cycles issue, and three warps a scheduler do not cover
+// more of what instructions wait for one another. Short contexts are bound by latency (500 rows
+// 10.5 us, two launches), ragged batches by both (verify batch of 32 sequences 63 us: 23, and 3.4
+// TB/s behind them).
 //
 // The arithmetic. A group of one, two or four warps (64 dimensions each) goes through tiles of
 // as many blocks of the cache (16 rows, one scale for the keys, one for the values), streamed
@@ -33,6 +37,7 @@
 // The weights of the rows (for eviction) need every query's final maximum and sum: the scores
 // are written down as they come, 4 bytes against 2 * head_dim / group read for them, and a
 // second kernel turns them into weights and adds those up, one thread a row, in order.
+#include <algorithm>
 #include <climits>
 
 #include "cache8.cuh"
@@ -43,7 +48,6 @@ namespace gufo {
 namespace {
 
 constexpr int kMostUnitRows = 256;
-constexpr int kShortCapacity = 384;
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kMostSms = 160;                 // whose blocks a call uses
@@ -975,8 +979,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 }
 
 // The units that several blocks have parts of: grid (cuts, rows of a unit / R). R query rows a block:
-// the parts' factors, then their sums; groups of a row's threads take a part of the parts each. A row a
-// block where there are few (one long sequence has a hundred parts), four where there are many.
+// the parts' factors, then their sums; groups of a row's threads take a part of the parts each.
 // (Two blocks an SM, not four: they come while the first kernel's last blocks run, and take shared
 // memory and issue slots from what follows: the verify batch 84 us with four, 70 with two.)
 constexpr int kJoinThreads = 256;
@@ -1085,7 +1088,8 @@ JoinKernel(const __grid_constant__ AttendArgs a, int rows) {
   }
 }
 
-// Weights of the rows: grid (groups of kWeightsThreads rows, KV heads, sequences).
+// Weights of the rows: grid (groups of kWeightsThreads rows, KV heads, sequences). Bound by latency (16
+// sequences of some 2000 rows, 8 KV heads of 4 query heads, 5 MB of scores: 8.5 us cold by itself).
 constexpr int kWeightsThreads = 128;
 __global__ void __launch_bounds__(kWeightsThreads)
 WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
@@ -1130,8 +1134,12 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
   using S = Shape<NS, RT>;
   const int blocks = Sms(ctx) * S::kBlocks;
   a.by_unit = units <= blocks;
-  // Short caches: a block a unit, and nothing to be shared out or joined.
-  a.undivided = a.cache.capacity <= kShortCapacity;
+  // Short caches: a block a unit, and nothing to be shared out or joined, where the longest unit takes no
+  // longer than that: 384 rows (4 heads of 64 of 64 sequences of up to 333 rows: 9.8 us, 14.2 shared out; one
+  // sequence of 500 rows, 2 heads of 256: 20.5, 10.9), more where there are units for two blocks in five at
+  // least (64 sequences, 500 rows: 11.9, 15.2; 100 sequences, 1000 rows: 21.4, 22.9; 200 sequences, 2000 rows:
+  // 66, 63; heads of 256, 128 sequences of 4, 500 rows: 27.9, 29.7; 1000 rows: 44.5, 40.9).
+  a.undivided = a.cache.capacity <= (units * 5 >= blocks * 2 ? (NS == 4 ? 512 : 1024) : 384);
   static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
                 "a block's parts fit the scratch");
   static std::atomic<bool> configured[64];
@@ -1148,7 +1156,9 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
     return GUFO_CUDA_OK;
   }
   const int cuts = a.by_unit ? static_cast<int>(units) : blocks;
-  if (cuts * rows <= 1024) {
+  // Units of many parts: a block a row. (One sequence of 131000 rows, 111 parts: 63 us, 86 with four rows a
+  // block; the verify batch of 8 sequences, 14 parts: 33, 38; of 32, 3: 73, 63.)
+  if (std::min<int64_t>(blocks / units, a.cache.capacity / S::kTile) > 8) {
     GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel<1>, dim3(cuts, rows), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
   } else {
     GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel<4>, dim3(cuts, (rows + 3) / 4), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));

@@ -30,7 +30,7 @@ struct BatchArgs {
 // 12 bytes of nothing: one contiguous copy. The codes stand by pairs of pieces (32 values), the 16
 // rows' bytes of a pair together: a row's part of a pair is a sector, which is what a row that is
 // gathered or written by itself costs (pieces alone: half of what is fetched is of another row; 8192
-// rows scattered over 64 MB 24 us, not 17). The order of the rows within a pair lets the
+// rows scattered over 64 MB 24 us, not 16). The order of the rows within a pair lets the
 // attention's lanes read their fragments from different places of shared memory: for keys eight
 // lanes read four pieces of two rows, for values two pieces of every second row.
 struct CacheView {

@@ -331,11 +331,11 @@ def test_attend_shares_ragged_sequences_out(ctx, form, heads, kv_heads, head_dim
         np.testing.assert_allclose(got[slot], given.get(slot, np.zeros((kv_heads, 1040))), rtol=2.0 ** -23, atol=3e-5 * 8)
 
 
+@pytest.mark.parametrize("capacity", [400, 1040])
 @pytest.mark.parametrize("form, sequences, heads, kv_heads, head_dim, most", [
     ("int8", 130, 10, 5, 64, 3), ("e4m3", 70, 56, 14, 128, 4), ("e4m3", 33, 32, 16, 256, 3)])
-def test_attend_with_more_units_than_blocks(ctx, form, sequences, heads, kv_heads, head_dim, most):
-    """Blocks that go through several sequences' heads, and share the last of them with the next block."""
-    capacity = 400
+def test_attend_with_more_units_than_blocks(ctx, form, sequences, heads, kv_heads, head_dim, most, capacity):
+    """Blocks that go through several sequences' heads, and share the last of them with the next block; or a block for each."""
     p = Pair(ctx, sequences, kv_heads, head_dim, capacity, form, weights=False)
     lengths = [most + (i * 149) % (capacity + 1 - most) for i in range(sequences)]
     # One content for all slots (the reference holds one): a sequence is told by its length and its queries.
