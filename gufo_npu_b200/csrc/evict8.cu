@@ -101,6 +101,9 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
     }
   };
   load(0);
+  if (threadIdx.x == 0) {
+    list_count = 0;
+  }
   // The key of the last row that stays: its bits from the top, 11, 11 and 10. Behind the first
   // look the keys that share its bits are listed, where they are few enough, and the rest is
   // left alone.
@@ -113,12 +116,9 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
     for (int i = threadIdx.x; i < kBins; i += kSelectThreads) {
       bins[i] = 0;
     }
-    if (threadIdx.x == 0) {
-      list_count = 0;
-    }
     __syncthreads();
     if (list) {
-      const unsigned n = found[2];
+      const unsigned n = list_count;
       for (unsigned i = threadIdx.x; i < (n + 31) / 32 * 32; i += kSelectThreads) {
         const uint32_t k = i < n ? listed[i] : 0;
         count(k, shift, bits, i < n && (k & mask) == key);
@@ -162,20 +162,17 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
     ahead = (warp == 0 ? 0 : ahead) + sum - top - next;
     const unsigned want = static_cast<unsigned>(wanted);
     if (ahead < want && want <= ahead + top) {
-      found[0] = kBins - 1 - 2 * threadIdx.x, found[1] = want - ahead;
-      if (!list) {
-        found[2] = top;
-      }
+      found[0] = kBins - 1 - 2 * threadIdx.x, found[1] = want - ahead, found[2] = top;
     } else if (ahead + top < want && want <= ahead + top + next) {
-      found[0] = kBins - 2 - 2 * threadIdx.x, found[1] = want - ahead - top;
-      if (!list) {
-        found[2] = next;
-      }
+      found[0] = kBins - 2 - 2 * threadIdx.x, found[1] = want - ahead - top, found[2] = next;
     }
     __syncthreads();
     key |= found[0] << shift;
     mask |= bits << shift;
     wanted = static_cast<int>(found[1]);
+    if (found[1] == found[2]) {
+      break;      // all of the bin stay, whatever their other bits
+    }
     if (!list && one_span && pass < 2 && found[2] <= kBins) {
       list = true;
 #pragma unroll
@@ -193,7 +190,7 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
     __syncthreads();
   }
 
-  // The rows above the key stay, the ends, and the first `wanted` rows with that very key. Rows that
+  // The rows above the key stay, the ends, and the first `wanted` rows with the key's bits. Rows that
   // stay anyway and rows with the key are counted together, 16 bits each (a chunk has 4096).
   unsigned before = 0, ties_before = 0;
 #pragma unroll 1
@@ -210,8 +207,8 @@ SelectKernel(const __grid_constant__ EvictArgs a, const __grid_constant__ BatchA
         const int i = base + n * kChunk + 4 * threadIdx.x + j;
         const uint32_t k = key_of(n, j);
         const bool competes = i >= low && i < high && mask != 0;
-        marks[n] |= i < rows && (i < low || i >= high || (competes && k > key)) ? 1u << j : 0u;
-        marks[n] |= competes && k == key ? 16u << j : 0u;
+        marks[n] |= i < rows && (i < low || i >= high || (competes && (k & mask) > key)) ? 1u << j : 0u;
+        marks[n] |= competes && (k & mask) == key ? 16u << j : 0u;
       }
       sums[n] = __popc(marks[n] & 15u) | __popc(marks[n] & 0xF0u) << 16;
 #pragma unroll
