@@ -320,7 +320,10 @@ int gufo_cuda_cache8_create(gufo_cuda_ctx* ctx, const gufo_cuda_cache8_config* c
   uint8_t* data = nullptr;
   const size_t bytes = 2 * side + weights;
   GUFO_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&data), bytes));
-  const cudaError_t e = cudaMemsetAsync(data, 0, bytes, ctx->stream);
+  cudaError_t e = cudaMemsetAsync(data, 0, bytes, ctx->stream);
+  if (e == cudaSuccess) {
+    e = cudaStreamSynchronize(ctx->stream);   // (the next call may be on another stream)
+  }
   if (e != cudaSuccess) {
     cudaFree(data);
     return gufo::CudaFail(e, "cache8_create");

@@ -454,8 +454,8 @@ int gufo_cuda_rope_free(gufo_cuda_ctx* ctx, gufo_cuda_rope rope);
 
 /* Rows that turn: `heads` heads of `head_dim` values (even, rope_dim .. 512) for each
  * token, strides in floats. With norm_weight ([head_dim], device) a head's row goes
- * through RMSNorm first. `out` may be `in` with the same strides; otherwise the two
- * do not overlap. Values behind rope_dim are passed on (normed where asked). */
+ * through RMSNorm first. `out` may be `in` with the same strides; otherwise no part's
+ * `out` overlaps any part's rows. Values behind rope_dim are passed on (normed where asked). */
 typedef struct gufo_cuda_rope_rows {
   const float* in;
   int64_t in_token_stride, in_head_stride;

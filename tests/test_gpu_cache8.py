@@ -540,6 +540,26 @@ def test_calls_on_two_streams_and_in_graphs(ctx):
         part[0].close()
 
 
+def test_a_new_cache_is_used_on_another_stream():
+    """A cache made on a stream that is busy, and written on another: nothing clears it afterwards."""
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    c = Context(0, busy.cuda_stream)
+    with torch.cuda.stream(busy):
+        x = torch.ones(4096, 4096, device=DEV)
+        for _ in range(50):
+            x = x @ x * 2.0 ** -12
+    p = Pair(c, 1, 1, 16, 32, "e4m3")
+    c.set_stream(other.cuda_stream)
+    k = draw(1, 20, 1, 16)
+    kd = k.to(DEV)
+    other.wait_stream(torch.cuda.current_stream())
+    p.gpu.append_device(p.gpu.batch(ints(0), [20]), kd, kd)
+    torch.cuda.synchronize()
+    p.ref.append(0, 0, (k.numpy(), k.numpy()))
+    p.same(0, 20)
+    c.close()
+
+
 # ---- eviction ---------------------------------------------------------------------------
 
 
