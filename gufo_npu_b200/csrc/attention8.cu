@@ -5,7 +5,7 @@
 // stays hidden under them: one int8 sequence of 131000 rows of 4 heads of 256 63 us, 4.3 TB/s, of
 // which the loop alone takes 4.6; half of all cycles issue, and three warps a scheduler do not cover
 // more of what instructions wait for one another. Short contexts are bound by latency (500 rows
-// 10.5 us, two launches), ragged batches by both (verify batch of 32 sequences 63 us: 23, and 3.4
+// 7 us), ragged batches by both (verify batch of 32 sequences 63 us: 23, and 3.4
 // TB/s behind them).
 //
 // The arithmetic. A group of one, two or four warps (64 dimensions each) goes through tiles of
@@ -33,12 +33,17 @@
 // they are, and goes through the units that it touches. What several blocks have a part of, a
 // second kernel puts together, part by part in order: as a last block's work behind a counter
 // it took 5 us more of the first one's time (fence, counter, two rounds through L2 by one block).
+// Where the cache is short, a unit has a block or a cluster of blocks instead, which join in
+// distributed shared memory.
 //
 // The weights of the rows (for eviction) need every query's final maximum and sum: the scores
 // are written down as they come, 4 bytes against 2 * head_dim / group read for them, and a
 // second kernel turns them into weights and adds those up, one thread a row, in order.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "cache8.cuh"
 #include "decode_device.cuh"
@@ -48,6 +53,7 @@ namespace gufo {
 namespace {
 
 constexpr int kMostUnitRows = 256;
+constexpr int kRanks = 8;
 constexpr int kThreads = 128;
 constexpr int kWarps = 4;
 constexpr int kMostSms = 160;                 // whose blocks a call uses
@@ -79,7 +85,7 @@ struct AttendArgs {
   int whole;               // rows of queries, gates and outputs may be taken four values at a time
   Cut* cuts;               // [units or blocks]
   int by_unit;
-  int undivided;           // a block a unit
+  int ranks;               // blocks of a unit that is not shared out: 1, or a cluster's kRanks
   float* sums;             // [blocks][2: the unit it goes on with, the one it begins][rows][head_dim]
   float* stats;            // [blocks][2][rows][2]
   float* scores;           // [query rows][capacity]; null: no weights
@@ -111,6 +117,7 @@ struct Shape {
   static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4)
   static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
+  static_assert(kBlocks * (kBytes + 1024 + 2880) <= 228 * 1024 || RT == 4, "kBlocks fit an SM with what else is in shared memory");
 };
 
 // Waits until a copy that this kernel asked for has landed; false, once, where it has not after
@@ -334,20 +341,22 @@ __device__ __forceinline__ void Note(const AttendArgs& a, const QueryRow& q, flo
   }
 }
 
-// Grid: resident blocks. W: the scores are written down. (Apart, as what the loop has to fetch counts: with
+// D: tiles are shared out, grid: resident blocks; otherwise grid: units times ranks. W: the scores are written
+// down. (Apart, as what the loop has to fetch counts: with
 // the stores behind a test in it a verify batch that writes none took 97 us, not 63.)
-template <typename Format, int NS, int RT, bool W>
+template <typename Format, int NS, int RT, bool W, bool D>
 __global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
   using S = Shape<NS, RT>;
   constexpr int kTile = S::kTile;
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ float row_factor[8 * RT];       // of a query row's scores
+  __shared__ float row_factor[8 * RT];       // of a query row's scores; then their weights' sum
   __shared__ int row_seen[8 * RT];
+  __shared__ float2 row_stats[D ? 1 : 8 * RT];       // a cluster's blocks': maximum and sum
   __shared__ float* row_scores[W ? 8 * RT : 1];      // where a query row's scores are written
   __shared__ __align__(8) float block_top[2][kWarps][8 * RT];    // what a block's weights are taken against
-  __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT], row_total[8 * RT];
-  __shared__ Shares shares;
+  __shared__ float group_top[S::kGroups][8 * RT], warp_total[kWarps][8 * RT];
+  __shared__ std::conditional_t<D, Shares, int> shares;
   __shared__ __align__(16) uint4 nothing;        // a piece of zeros
   __shared__ __align__(8) uint64_t bars[kWarps][S::kSlots];
   if (threadIdx.x < kWarps * S::kSlots) {
@@ -364,12 +373,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   const int group = warp / NS, member = warp % NS;
   const int g = lane >> 2, t = lane & 3;
   int begin = 0, end = 1, all = 1;
-  if (!a.undivided) {
+  if constexpr (D) {
     ShareOut(a, batch, kTile, S::kUnitCost, shares);
     all = shares.ahead[batch.sequences];
   }
   const Stretches stretches(all, S::kGroups, gridDim.x);   // a tile a group at least
-  if (!a.undivided) {
+  if constexpr (D) {
     if (threadIdx.x == 0 && !a.by_unit) {
       a.cuts[blockIdx.x].parts = 0;      // unless it begins a unit that others have parts of
     }
@@ -413,10 +422,10 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     Unit unit;
     Task task;
     int first_tile = 0, last_tile = INT_MAX;
-    if (a.undivided) {
-      const int item = blockIdx.x / c.kv_heads;
+    if constexpr (!D) {
+      const int number = blockIdx.x / a.ranks, item = number / c.kv_heads;
       unit.sequence = SequenceOf(batch, item);
-      unit.kh = blockIdx.x - item * c.kv_heads;
+      unit.kh = number - item * c.kv_heads;
       unit.chunk = item - batch.first_item[unit.sequence];
       unit.tiles = last_tile;
       unit.start = unit.number = 0;
@@ -449,7 +458,13 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       least = min(least, row_seen[r]);
     }
     // (These rows may see less than the sequence's last ones.)
-    const int end_tile = min(last_tile, (length + kTile - 1) / kTile);
+    const int all_tiles = (length + kTile - 1) / kTile;
+    const int rank = D || a.ranks == 1 ? 0 : blockIdx.x % kRanks;
+    if (!D && a.ranks > 1) {
+      first_tile = all_tiles * rank / kRanks;
+      last_tile = all_tiles * (rank + 1) / kRanks;
+    }
+    const int end_tile = min(last_tile, all_tiles);
     const size_t of_head = static_cast<size_t>(task.e.slot) * c.kv_heads + kh;
 
     // ---- the ring: a warp copies its block of every tile, keys and values in turn (a block that
@@ -920,7 +935,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         }
       }
     }
-    const bool alone = first_tile == 0 && last_tile == unit.tiles;
+    const bool alone = D ? first_tile == 0 && last_tile == unit.tiles : a.ranks == 1;
     const size_t part = PartOf(blockIdx.x, first_tile == 0, 8 * RT);
     if (threadIdx.x < 8 * RT) {
       // A row's maximum and sum, and the factors of the groups' parts.
@@ -940,11 +955,14 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         }
         group_top[of][r] = by;      // from now on the part's factor
       }
-      row_total[r] = sum;
+      row_factor[r] = sum;
+      if constexpr (!D) {
+        row_stats[r] = make_float2(most, sum);
+      }
       if (r < task.rows) {
         if (alone) {
           Note(a, QueryRow(a, task, kh, r), most, sum);
-        } else {
+        } else if (D) {
           // (A row that sees nothing is told by its sum, whatever its parts.)
           reinterpret_cast<float2*>(a.stats)[part + r] = make_float2(most, row_seen[r] > 0 ? sum : -1.f);
         }
@@ -963,12 +981,56 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
         sum.x = fmaf(v.x, by, sum.x), sum.y = fmaf(v.y, by, sum.y), sum.z = fmaf(v.z, by, sum.z), sum.w = fmaf(v.w, by, sum.w);
       }
       if (alone) {
-        Finish(a, QueryRow(a, task, kh, r), f, sum, row_total[r], row_seen[r] > 0);
+        Finish(a, QueryRow(a, task, kh, r), f, sum, row_factor[r], row_seen[r] > 0);
+      } else if (!D) {
+        *reinterpret_cast<float4*>(join + r * S::kRowBytes + 4 * f) = sum;
       } else {
         reinterpret_cast<float4*>(a.sums + (part + r) * c.head_dim)[f] = sum;
       }
     }
-    if (first_tile == 0 && threadIdx.x == 0 && (a.by_unit || !alone) && !a.undivided) {
+    if (!D && a.ranks > 1) {
+      // The cluster's blocks put their parts together, each an eighth of the outputs.
+      const auto cluster = cooperative_groups::this_cluster();
+      cluster.sync();
+      const auto parts_of = [&](int r, float (&by)[kRanks], float& most, float& total) {
+        float2 stats[kRanks];
+        most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kRanks; ++i) {
+          stats[i] = cluster.map_shared_rank(row_stats, i)[r];
+          most = fmaxf(most, stats[i].x);
+        }
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRanks; ++i) {
+          by[i] = stats[i].x == most ? 1.f : exp2f(stats[i].x - most);
+          total = fmaf(stats[i].y, by[i], total);
+        }
+      };
+      for (int at = rank * kThreads + threadIdx.x; at < task.rows * fours; at += kRanks * kThreads) {
+        const int r = at / fours, f = at - r * fours;
+        float4 v[kRanks];
+#pragma unroll
+        for (int i = 0; i < kRanks; ++i) {
+          v[i] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(join, i) + r * S::kRowBytes + 4 * f);
+        }
+        float by[kRanks], most, total;
+        parts_of(r, by, most, total);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kRanks; ++i) {
+          sum.x = fmaf(v[i].x, by[i], sum.x), sum.y = fmaf(v[i].y, by[i], sum.y);
+          sum.z = fmaf(v[i].z, by[i], sum.z), sum.w = fmaf(v[i].w, by[i], sum.w);
+        }
+        const QueryRow q(a, task, kh, r);
+        Finish(a, q, f, sum, total, row_seen[r] > 0);
+        if (f == 0) {
+          Note(a, q, most, total);
+        }
+      }
+      cluster.sync();      // (the others have read this block's part)
+    }
+    if (D && first_tile == 0 && threadIdx.x == 0 && (a.by_unit || !alone)) {
       a.cuts[a.by_unit ? unit.number : static_cast<int>(blockIdx.x)] = {
           static_cast<int>(blockIdx.x), alone ? 0 : stretches.owner_of(unit.start + unit.tiles - 1) - static_cast<int>(blockIdx.x) + 1,
           task.rows, task.e.row, kh * a.group, task.row0};
@@ -1129,31 +1191,47 @@ constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
 constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
 size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * ((kPartialFloats + kStatsFloats) * sizeof(float) + 4 * 32); }
 
+template <typename Format, int NS, int RT, bool W, bool D>
+int LaunchTiles(gufo_cuda_ctx* ctx, const AttendArgs& a, const BatchArgs& b, int grid) {
+  using S = Shape<NS, RT>;
+  static std::atomic<bool> configured[64];
+  if (ctx->device >= 64 || !configured[ctx->device].load()) {
+    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT, W, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    if (ctx->device < 64) {
+      configured[ctx->device].store(true);
+    }
+  }
+  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT, W, D>, dim3(grid), dim3(kThreads), S::kBytes, ctx->stream,
+                                 D ? 1 : a.ranks, a, b));
+  ctx->launches.fetch_add(1);
+  return GUFO_CUDA_OK;
+}
+
 template <typename Format, int NS, int RT, bool W>
 int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t units, int rows) {
   using S = Shape<NS, RT>;
   const int blocks = Sms(ctx) * S::kBlocks;
   a.by_unit = units <= blocks;
+  static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
+                "a block's parts fit the scratch");
   // Short caches: a block a unit, and nothing to be shared out or joined, where the longest unit takes no
-  // longer than that: 384 rows (4 heads of 64 of 64 sequences of up to 333 rows: 9.8 us, 14.2 shared out; one
+  // longer than that: 384 rows (4 heads of 64 of 64 sequences of up to 333 rows: 9.0 us, 14.2 shared out; one
   // sequence of 500 rows, 2 heads of 256: 20.5, 10.9), more where there are units for two blocks in five at
   // least (64 sequences, 500 rows: 11.9, 15.2; 100 sequences, 1000 rows: 21.4, 22.9; 200 sequences, 2000 rows:
   // 66, 63; heads of 256, 128 sequences of 4, 500 rows: 27.9, 29.7; 1000 rows: 44.5, 40.9).
-  a.undivided = a.cache.capacity <= (units * 5 >= blocks * 2 ? (NS == 4 ? 512 : 1024) : 384);
-  static_assert(S::kBlocks * 2 * 8 * RT * S::kRowBytes <= static_cast<int>(kPartialFloats) && S::kBlocks * 2 * 8 * RT * 2 <= static_cast<int>(kStatsFloats),
-                "a block's parts fit the scratch");
-  static std::atomic<bool> configured[64];
-  if (ctx->device >= 64 || !configured[ctx->device].load()) {
-    GUFO_CUDA_TRY(cudaFuncSetAttribute(AttendKernel<Format, NS, RT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
-    if (ctx->device < 64) {
-      configured[ctx->device].store(true);
-    }
+  const int short_capacity = units * 5 >= blocks * 2 ? (NS == 4 ? 512 : 1024) : 384;
+  if (a.cache.capacity <= short_capacity) {
+    a.ranks = 1;
+    return LaunchTiles<Format, NS, RT, W, false>(ctx, a, b, static_cast<int>(units));
   }
-  GUFO_CUDA_TRY(LaunchOverlapped(AttendKernel<Format, NS, RT, W>, dim3(a.undivided ? static_cast<int>(units) : blocks), dim3(kThreads), S::kBytes,
-                                 ctx->stream, 1, a, b));
-  ctx->launches.fetch_add(1);
-  if (a.undivided) {
-    return GUFO_CUDA_OK;
+  // Few units of some length: a cluster of blocks a unit, no second launch. (8 heads on 2 of 256, 500 rows: 7.0
+  // us, 10.6 shared out; 1500: 10.9, 11.9; 1900: 12.8, 12.3. Heads of 128, 2000 rows: 10.3, 10.5; 3900: 15.7, 12.0.)
+  if (a.cache.capacity <= (NS == 4 ? 1536 : 2048) && units * kRanks <= blocks) {
+    a.ranks = kRanks;
+    return LaunchTiles<Format, NS, RT, W, false>(ctx, a, b, static_cast<int>(units) * kRanks);
+  }
+  if (const int rc = LaunchTiles<Format, NS, RT, W, true>(ctx, a, b, blocks); rc != GUFO_CUDA_OK) {
+    return rc;
   }
   const int cuts = a.by_unit ? static_cast<int>(units) : blocks;
   // Units of many parts: a block a row. (One sequence of 131000 rows, 111 parts: 63 us, 86 with four rows a

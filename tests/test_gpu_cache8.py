@@ -304,15 +304,17 @@ def test_attend_over_long_contexts(ctx, form, heads, kv_heads, head_dim, length,
         np.testing.assert_array_equal(attend(p, [length - tokens], [tokens], q, scratch=scratch), out)
 
 
+@pytest.mark.parametrize("capacity", [1040, 2064])
 @pytest.mark.parametrize("form", ["e4m3", "int8"])
 @pytest.mark.parametrize("heads, kv_heads, head_dim, most", [
     (4, 4, 64, 1), (4, 2, 48, 8), (12, 1, 64, 8), (32, 8, 128, 1), (8, 2, 112, 4), (6, 1, 128, 8), (8, 2, 256, 1), (8, 2, 256, 4),
     (9, 3, 192, 8), (40, 2, 256, 2)])
-def test_attend_shares_ragged_sequences_out(ctx, form, heads, kv_heads, head_dim, most):
-    """Sequences of one row to a thousand, whose tiles many blocks take parts of: every group of query rows, ragged."""
+def test_attend_shares_ragged_sequences_out(ctx, form, heads, kv_heads, head_dim, most, capacity):
+    """Sequences of one row to a thousand, whose tiles many blocks, or a cluster's, take parts of: every group of query rows,
+    ragged."""
     lengths = [9, 15, 1033, 700, 64, 65, 1, 400, 1040]
     tokens = [min(n, most) for n in (1, 2, 8, 3, 4, 8, 1, 5, 2)]
-    p = Pair(ctx, 9, kv_heads, head_dim, 1040, form)
+    p = Pair(ctx, 9, kv_heads, head_dim, capacity, form)
     p.fill(lengths)
     rows = sum(tokens)
     q, gate = (draw(5, rows, heads, head_dim) * 1.5).to(DEV), draw(6, rows, heads, head_dim).to(DEV)
@@ -328,7 +330,7 @@ def test_attend_shares_ragged_sequences_out(ctx, form, heads, kv_heads, head_dim
     got = p.gpu.weights.cpu().numpy()
     for slot in range(9):
         # (as in test_attend_adds_up_weights, for each of up to 8 tokens' 20 heads)
-        np.testing.assert_allclose(got[slot], given.get(slot, np.zeros((kv_heads, 1040))), rtol=2.0 ** -23, atol=3e-5 * 8)
+        np.testing.assert_allclose(got[slot], given.get(slot, np.zeros((kv_heads, capacity))), rtol=2.0 ** -23, atol=3e-5 * 8)
 
 
 @pytest.mark.parametrize("capacity", [400, 1040])
