@@ -5,7 +5,7 @@
 // whole numbers, so that nothing depends on the order of the atomics), then goes through the rows
 // in their order, writes down the ones that stay and moves their weights. Bound by latency: up
 // to 16384 rows are read once and stay in registers, and behind the first histogram only the
-// rows of one bin are looked at (64 heads of 2064 rows 11.5 us cold, 16 heads of 16384 rows 20).
+// rows of one bin are looked at (64 heads of 2064 rows 11 us cold, 16 heads of 16384 rows 20).
 //
 // Moving them. A warp makes one block of 16 rows: it gathers them, takes their largest
 // magnitude, and rounds what had another scale. In place, the rows a block receives come from

@@ -542,6 +542,42 @@ def test_calls_on_two_streams_and_in_graphs(ctx):
         part[0].close()
 
 
+@pytest.mark.parametrize("capacity", [320, 1024])
+def test_captured_calls_of_short_caches(capacity):
+    """A block, or a cluster of blocks, a sequence and head, captured once: lengths from none to all of the cache, and weights."""
+    stream = torch.cuda.Stream()
+    c = Context(0, stream.cuda_stream)
+    p = Pair(c, 2, 2, 80, capacity, "e4m3")
+    p.fill([capacity, capacity])
+    q, gate = draw(7, 3, 6, 80).to(DEV), draw(8, 3, 6, 80).to(DEV)
+    out = torch.empty(3, 6, 80, device=DEV)
+    at = ints(5, 5)
+    batch, scratch = p.gpu.batch(at, [1, 2]), p.gpu.scratch(6, 3, accumulate=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        p.gpu.attend_device(batch, q, out, scratch, gate=gate, accumulate=True)
+    for positions in ((5, 17), (-1, 62), (capacity - 1, -3), (capacity - 2, capacity), (63, 0), (0, capacity // 2)):
+        at.copy_(ints(*positions))
+        p.gpu.weights.zero_()
+        torch.cuda.synchronize()
+        first = None
+        for _ in range(3):
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            first = out.clone() if first is None else first
+            assert torch.equal(first, out)
+        given = check_attend(p, positions, [1, 2], q, out.cpu().numpy(), gate)
+        got = p.gpu.weights.cpu().numpy()
+        for slot in range(2):
+            np.testing.assert_allclose(got[slot], 3 * given.get(slot, np.zeros((2, capacity))), rtol=2.0 ** -22, atol=3e-5 * 6)
+    del graph
+    c.close()
+
+
 def test_a_new_cache_is_used_on_another_stream():
     """A cache made on a stream that is busy, and written on another: nothing clears it afterwards."""
     busy, other = torch.cuda.Stream(), torch.cuda.Stream()
