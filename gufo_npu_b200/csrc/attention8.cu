@@ -114,7 +114,7 @@ struct Shape {
   // 95 with two. Heads of 256, 16 query rows: 70 with three, 79 with two.)
   static constexpr int kBlocks = RT == 4 ? 2 : NS == 4 || RT == 2 ? 3 : 4;
   static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4)
+  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4, all with four digits)
   static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
   static_assert(kBlocks * (kBytes + 1024 + 2880) <= 228 * 1024 || RT == 4, "kBlocks fit an SM with what else is in shared memory");
@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
   using S = Shape<NS, RT>;
   constexpr int kTile = S::kTile;
+  constexpr int kDigits = NS == 1 ? 4 : 3;       // of queries as whole numbers
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores; then their weights' sum
   __shared__ int row_seen[8 * RT];
@@ -533,11 +534,13 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
       top = __reduce_max_sync(0xFFFFFFFFu, top);
       if constexpr (Format::kWhole) {
-        // Whole numbers of 24 bits, the largest as near to three signed bytes' most (base 256: 127 * 65793) as a
-        // power of two takes it: rounded to half of 2^-23 of the largest, of 2^-22 where its fraction is above
-        // 1.992. A row that is not finite: any, its factor is NaN.
-        const int e = min(max(static_cast<int>(top >> 23), 23), 254);
-        const int by = (top & 0x7FFFFFu) <= 0x7EFEFEu ? 149 - e : 148 - e;
+        // Whole numbers as three signed bytes, base 256, the largest as near to their most (127 * 65793) as a power
+        // of two takes it: rounded to half of 2^-23 of the largest, of 2^-22 where its fraction is above 1.992. Heads
+        // of 64, whose sums are short, show that rounding beside fp32's: a fourth byte, half of 2^-29 (64 sequences of
+        // up to 333 rows: 4e-7 -> 1.2e-7 off, fp32 2e-7; 9.0 -> 9.1 us). A row that is not finite: any, its factor is
+        // NaN.
+        const int e = min(max(static_cast<int>(top >> 23), kDigits == 4 ? 30 : 23), 254);
+        const int by = kDigits == 4 ? 156 - e : (top & 0x7FFFFFu) <= 0x7EFEFEu ? 149 - e : 148 - e;
         const float up = PowerOfTwo(by);
 #pragma unroll
         for (int i = 0; i < kTimes; ++i) {
@@ -546,20 +549,21 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             const int seg = f / 16, of = f % 16 / 4, j = f % 4;
             const int v[4] = {__float2int_rn(x[i].x * up), __float2int_rn(x[i].y * up), __float2int_rn(x[i].z * up),
                               __float2int_rn(x[i].w * up)};
-            uint32_t digits[3] = {0, 0, 0};
+            uint32_t digits[kDigits] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              // Offset by 128, the bytes of v + 0x808080 are the balanced digits.
-              const uint32_t z = (static_cast<uint32_t>(v[k]) + 0x808080u) ^ 0x808080u;
+              // Offset by 128 each, the bytes are the balanced digits.
+              constexpr uint32_t kOffset = kDigits == 4 ? 0x80808080u : 0x808080u;
+              const uint32_t z = (static_cast<uint32_t>(v[k]) + kOffset) ^ kOffset;
 #pragma unroll
-              for (int l = 0; l < 3; ++l) {
+              for (int l = 0; l < kDigits; ++l) {
                 digits[l] |= (z >> (8 * l) & 0xFFu) << (8 * k);
               }
             }
             uint32_t* to = reinterpret_cast<uint32_t*>(query);     // [rt][seg][digit][lane][j]
 #pragma unroll
-            for (int l = 0; l < 3; ++l) {
-              to[((((r / 8 * NS + seg) * 3 + l) * 32) + r % 8 * 4 + of) * 4 + j] = digits[l];
+            for (int l = 0; l < kDigits; ++l) {
+              to[((((r / 8 * NS + seg) * kDigits + l) * 32) + r % 8 * 4 + of) * 4 + j] = digits[l];
             }
           }
         }
@@ -637,11 +641,11 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
           s[rt][0] = s[rt][1] = s[rt][2] = s[rt][3] = 0.f;
         }
       } else if constexpr (Format::kWhole) {
-        int d[RT][3][4];      // by the queries' digits
+        int d[RT][kDigits][4];      // by the queries' digits
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-          for (int l = 0; l < 3; ++l) {
+          for (int l = 0; l < kDigits; ++l) {
             d[rt][l][0] = d[rt][l][1] = d[rt][l][2] = d[rt][l][3] = 0;
           }
         }
@@ -651,19 +655,24 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-            for (int l = 0; l < 3; ++l) {
-              const uint4 q = query[((rt * NS + seg) * 3 + l) * 32 + lane];
+            for (int l = 0; l < kDigits; ++l) {
+              const uint4 q = query[((rt * NS + seg) * kDigits + l) * 32 + lane];
               MmaWhole(d[rt][l], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
               MmaWhole(d[rt][l], k0.z, k1.z, k0.w, k1.w, q.z, q.w);
             }
           }
         }
-        // (A digit's sum is at most 256 * 128 * 127: two of them fit an int, the lowest a float.)
+        // (A digit's sum is at most 256 * 128 * 127, of four digits a quarter: two of them fit an int, the lowest a float.)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
+            if constexpr (kDigits == 4) {
+              s[rt][i] = fmaf(static_cast<float>(d[rt][3][i] * 256 + d[rt][2][i]), 65536.f,
+                              static_cast<float>(d[rt][1][i] * 256 + d[rt][0][i]));
+            } else {
+              s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
+            }
           }
         }
       } else {
