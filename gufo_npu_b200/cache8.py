@@ -163,6 +163,8 @@ class CudaCache8:
             slots = (C.c_int * batch.sequences)(*into_slots)
         if into is not None and into.ctx is not self.ctx:
             raise ValueError("cache8: both caches belong to one context")
+        if into is not None and not into.handle:      # (0 is the library's word for an eviction in place)
+            raise ValueError("cache8: into is closed")
         ctx = self._ctx_of(batch)
         ctx._check(_capi.native.cache8_evict(ctx._address, ctx.device, self.handle, batch.args, batch.sequences, self.kv_heads,
                                              budget, first, last, kept, held, into.handle if into is not None else 0, slots))
