@@ -236,8 +236,9 @@ void Frequencies(const gufo_cuda_rope_params& p, double* frequencies, double* ma
   };
   double low = 0.0, high = 0.0;
   if (by_parts) {
-    low = std::fmin(std::fmax(std::floor(pair_of(p.fast_turns)), 0.0), pairs - 1.0);
-    high = std::fmin(std::fmax(std::ceil(pair_of(p.slow_turns)), 0.0), pairs - 1.0);
+    // (The ramp may end behind the last pair, and keeps its slope there: held to 2 pairs - 1.)
+    low = std::fmin(std::fmax(std::floor(pair_of(p.fast_turns)), 0.0), p.rope_dim - 1.0);
+    high = std::fmin(std::fmax(std::ceil(pair_of(p.slow_turns)), 0.0), p.rope_dim - 1.0);
   }
   for (int i = 0; i < pairs; ++i) {
     double f = std::pow(p.theta, -static_cast<double>(i) / pairs);

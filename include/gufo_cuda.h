@@ -430,7 +430,8 @@ enum {
   /* Pairs that turn more than fast_turns times over original_positions as they are,
    * those that turn less than slow_turns times / factor, the ones between mixed in
    * proportion to the pair's number: low .. high, the pairs of fast_turns (rounded
-   * down) and slow_turns (rounded up) held inside 0 .. rope_dim / 2 - 1. */
+   * down) and slow_turns (rounded up), held inside 0 .. rope_dim - 1: where high lies
+   * behind the last pair, rope_dim / 2 - 1, no pair is divided by the whole factor. */
   GUFO_CUDA_ROPE_BY_PARTS = 2
 };
 typedef struct gufo_cuda_rope_params {
