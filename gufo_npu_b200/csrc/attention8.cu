@@ -1198,6 +1198,12 @@ WeightsKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batc
 int Sms(const gufo_cuda_ctx* ctx) { return ctx->sm_count < kMostSms ? ctx->sm_count : kMostSms; }
 constexpr size_t kPartialFloats = 2 * 2 * (32 * 256);     // of an SM
 constexpr size_t kStatsFloats = 4 * 2 * (32 * 2);
+// Items (groups of a sequence's query rows, each a unit for every KV head) that one launch takes: the
+// cost of all its units is counted in an int (ShareOut; tiles of a block, and what a unit costs besides).
+int MostItems(const gufo_cuda_cache8_config& c) {
+  return static_cast<int>(INT32_MAX / (static_cast<int64_t>(c.kv_heads) * (c.capacity / kCacheBlock + 1 + kMostUnitRows / kCacheBlock)));
+}
+constexpr int kMostItemRows = 32;
 size_t PartialBytes(int sms) { return static_cast<size_t>(sms) * ((kPartialFloats + kStatsFloats) * sizeof(float) + 4 * 32); }
 
 template <typename Format, int NS, int RT, bool W, bool D>
@@ -1290,7 +1296,11 @@ int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle,
     return rc;
   }
   const size_t rows = static_cast<size_t>(heads) * tokens;
-  if (accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / cache->c.capacity) {
+  // (However the tokens are spread over the cache's sequences.)
+  const int64_t group = heads > cache->c.kv_heads ? heads / cache->c.kv_heads : 1;
+  const int64_t each = static_cast<int64_t>(gufo::MostItems(cache->c)) * gufo::kMostItemRows / group;
+  if ((each < cache->c.capacity && tokens > each * cache->c.sequences) ||
+      (accumulate != 0 && rows > (static_cast<size_t>(1) << 48) / cache->c.capacity)) {
     return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend_scratch: too many query rows for one call");
   }
   *bytes = gufo::PartialBytes(gufo::Sms(ctx)) + (accumulate != 0 ? rows * (2 + static_cast<size_t>(cache->c.capacity)) * 4 : 0);
@@ -1370,8 +1380,11 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
   a.cuts = reinterpret_cast<gufo::Cut*>(a.stats + static_cast<size_t>(gufo::Sms(ctx)) * gufo::kStatsFloats);
   static_assert(sizeof(gufo::Cut) <= 32, "the scratch has 32 bytes a block for it");
   const int rt = rows_each <= 8 ? 1 : rows_each <= 16 ? 2 : 4;
-  if (tokens * a.group / (8 * rt) + batch->sequences > 65535) {
-    return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
+  static_assert(8 * 4 == gufo::kMostItemRows, "of the largest rt");
+  // (The longest sequence's: the others of a batch go to a launch of their own where they are too many together.)
+  const int most_items = gufo::MostItems(c);
+  if ((rows_each + 8 * rt - 1) / (8 * rt) > most_items) {
+    return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows of one sequence");
   }
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));
   const int group = a.group;
@@ -1380,9 +1393,6 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
       [&](const gufo::BatchArgs& b, int items) -> int {
         const int64_t units = static_cast<int64_t>(items) * c.kv_heads;
         const int rows = rows_each < 8 * rt ? static_cast<int>(rows_each) : 8 * rt;
-        if (units * (c.capacity / gufo::kCacheBlock + 1 + gufo::kMostUnitRows / gufo::kCacheBlock) > INT32_MAX) {
-          return Fail(GUFO_CUDA_TOO_LARGE, "cache8_attend: too many query rows for one call");
-        }
         const bool e4m3 = c.format == GUFO_CUDA_CACHE8_E4M3;
         const int run = a.scores != nullptr ? (e4m3 ? gufo::PickAttend<gufo::E4m3, true>(ctx, a, b, units, rows, ns, rt)
                                                     : gufo::PickAttend<gufo::Int8, true>(ctx, a, b, units, rows, ns, rt))
@@ -1397,7 +1407,8 @@ int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 handle, 
                                              dim3(gufo::kWeightsThreads), 0, ctx->stream, 1, a, b));
         ctx->launches.fetch_add(1);
         return GUFO_CUDA_OK;
-      });
+      },
+      most_items);
 }
 
 }  // extern "C"

@@ -60,10 +60,10 @@ __device__ __forceinline__ int PieceAt(int side, int row, int piece) {
   return pair * 512 + at * 32 + (piece & 1) * 16;
 }
 
-// Calls launch(args) for every run of at most kBatchSequences sequences with work; items(tokens)
-// says how many items a sequence has. Checks the batch (CheckBatch) has passed.
+// Calls launch(args) for every run of at most kBatchSequences sequences with work and `limit` items;
+// items(tokens) says how many items a sequence has, at most `limit`. Checks the batch (CheckBatch) has passed.
 template <typename Items, typename Launch>
-int ForEachRun(const gufo_cuda_cache8_batch& b, Items items, Launch launch) {
+int ForEachRun(const gufo_cuda_cache8_batch& b, Items items, Launch launch, int limit = INT32_MAX) {
   BatchArgs a;
   a.positions = b.positions;
   int row = 0;
@@ -73,6 +73,9 @@ int ForEachRun(const gufo_cuda_cache8_batch& b, Items items, Launch launch) {
     for (; i < b.sequences && a.sequences < kBatchSequences; ++i) {
       const int tokens = b.tokens != nullptr ? b.tokens[i] : 1;
       const int n = items(tokens);
+      if (n > limit - at) {
+        break;
+      }
       if (n > 0) {
         a.of[a.sequences] = {i, b.slots != nullptr ? b.slots[i] : i, tokens, row};
         a.first_item[a.sequences++] = at;

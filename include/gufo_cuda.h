@@ -541,6 +541,9 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
  * sees no row gets zeros. Sums of exp(score - largest score) times values are fp32: of values
  * near its largest they are infinite. fp32 on the device, strides in floats; heads is a multiple of
  * kv_heads. `out` overlaps none of the inputs.
+ * Of one sequence, tokens * (heads / kv_heads) / 32 (rounded up) * kv_heads * (capacity / 16 + 17) is
+ * less than 2^31 (a capacity of 131072: 8 million query rows): GUFO_CUDA_TOO_LARGE otherwise, and nothing
+ * is enqueued.
  * accumulate != 0 (caches with weights): adds the softmax weights, summed over the sequence's
  * tokens and the query heads of a KV head, to the rows' weights.
  * scratch: gufo_cuda_cache8_attend_scratch bytes, 16-byte aligned, whatever they hold; calls that
@@ -561,7 +564,8 @@ typedef struct gufo_cuda_cache8_attend_args {
   void* scratch;
   size_t scratch_bytes;
 } gufo_cuda_cache8_attend_args;
-/* Enough for calls of up to `tokens` query tokens in all. */
+/* Enough for calls of up to `tokens` query tokens in all; GUFO_CUDA_TOO_LARGE where no batch of the
+ * cache's sequences may have so many. */
 int gufo_cuda_cache8_attend_scratch(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache, int heads, int tokens,
                                     int accumulate, size_t* bytes);
 int gufo_cuda_cache8_attend_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
