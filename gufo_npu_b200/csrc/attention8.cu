@@ -2,8 +2,8 @@
 //
 // What bounds it. The cache is read once, two bytes a row and dimension of a KV head: far into
 // the contexts that is all the time there is, if loads are never waited for and the arithmetic
-// stays hidden under them: one int8 sequence of 131000 rows of 4 heads of 256 63 us, 4.3 TB/s, of
-// which the loop alone takes 4.6; half of all cycles issue, and three warps a scheduler do not cover
+// stays hidden under them: one int8 sequence of 131000 rows of 4 heads of 256 65 us, 4.1 TB/s, of
+// which the loop alone takes 4.5; half of all cycles issue, and three warps a scheduler do not cover
 // more of what instructions wait for one another. Short contexts are bound by latency (500 rows
 // 7 us), ragged batches by both (verify batch of 32 sequences 63 us: 23, and 3.4
 // TB/s behind them).
@@ -19,8 +19,8 @@
 //   S^T = K Q^T   [16 rows x 8 queries],     O^T = V^T P^T   [16 dimensions x 8 queries]
 // Codes become fp16 exactly, in registers. The fp32 operands (queries; probabilities) go in as
 // two fp16 halves, 22 bits of them, scaled by a power of two first so that small ones keep
-// their bits; each sixteen products' sum is added up in fp32, as the tensor core cuts off what
-// its adder does not hold. S^T comes out with a query's column in the lanes that O^T wants it
+// their bits (queries against int8 keys: as whole numbers of four digits); each sixteen products'
+// sum is added up in fp32, as the tensor core cuts off what its adder does not hold. S^T comes out with a query's column in the lanes that O^T wants it
 // in; P^T is turned into a B operand by movmatrix. A lane's dimensions are permuted (16 bytes
 // of a key row, 8 of a value row are its own), which a sum over all of them does not see and
 // the output undoes.
@@ -114,7 +114,7 @@ struct Shape {
   // 95 with two. Heads of 256, 16 query rows: 70 with three, 79 with two.)
   static constexpr int kBlocks = RT == 4 ? 2 : NS == 4 || RT == 2 ? 3 : 4;
   static constexpr int kShared = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (fp16; whole numbers take 3/4, all with four digits)
+  static constexpr int kQuery = RT * NS * 4 * 32 * 16;      // B operands, in the lanes' order (two fp16 halves, or four digits)
   static constexpr int kWeights = NS == 1 ? 0 : 2 * kWarps * RT * 32 * 16;   // the same of two tiles' weights
   static constexpr int kBytes = kShared + kQuery + kWeights;
   static_assert(kBlocks * (kBytes + 1024 + 2880) <= 228 * 1024 || RT == 4, "kBlocks fit an SM with what else is in shared memory");
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NS, RT>::kBlocks))
 AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ BatchArgs batch) {
   using S = Shape<NS, RT>;
   constexpr int kTile = S::kTile;
-  constexpr int kDigits = NS == 1 ? 4 : 3;       // of queries as whole numbers
+  constexpr int kDigits = 4;                 // of queries as whole numbers
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float row_factor[8 * RT];       // of a query row's scores; then their weights' sum
   __shared__ int row_seen[8 * RT];
@@ -534,13 +534,12 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
       }
       top = __reduce_max_sync(0xFFFFFFFFu, top);
       if constexpr (Format::kWhole) {
-        // Whole numbers as three signed bytes, base 256, the largest as near to their most (127 * 65793) as a power
-        // of two takes it: rounded to half of 2^-23 of the largest, of 2^-22 where its fraction is above 1.992. Heads
-        // of 64, whose sums are short, show that rounding beside fp32's: a fourth byte, half of 2^-29 (64 sequences of
-        // up to 333 rows: 4e-7 -> 1.2e-7 off, fp32 2e-7; 9.0 -> 9.1 us). A row that is not finite: any, its factor is
-        // NaN.
-        const int e = min(max(static_cast<int>(top >> 23), kDigits == 4 ? 30 : 23), 254);
-        const int by = kDigits == 4 ? 156 - e : (top & 0x7FFFFFu) <= 0x7EFEFEu ? 149 - e : 148 - e;
+        // Whole numbers as four signed bytes, base 256, the largest from 2^29 to 2^30: rounded to half of 2^-29 of
+        // it. What is smaller keeps as many bits less, and may meet the keys' largest channels, so three bytes are
+        // too few: queries inverse to keys of which 4 channels in 128 are a hundred times the others, 2e-6 off, this
+        // way 2e-8 (fp32 operations 2.4e-7). A row that is not finite: any, its factor is NaN.
+        const int e = min(max(static_cast<int>(top >> 23), 30), 254);
+        const int by = 156 - e;
         const float up = PowerOfTwo(by);
 #pragma unroll
         for (int i = 0; i < kTimes; ++i) {
@@ -553,7 +552,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               // Offset by 128 each, the bytes are the balanced digits.
-              constexpr uint32_t kOffset = kDigits == 4 ? 0x80808080u : 0x808080u;
+              constexpr uint32_t kOffset = 0x80808080u;
               const uint32_t z = (static_cast<uint32_t>(v[k]) + kOffset) ^ kOffset;
 #pragma unroll
               for (int l = 0; l < kDigits; ++l) {
@@ -662,17 +661,13 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
             }
           }
         }
-        // (A digit's sum is at most 256 * 128 * 127, of four digits a quarter: two of them fit an int, the lowest a float.)
+        // (A digit's sum is at most 256 * 128 * 127, the highest's half of that: two of them fit an int.)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (kDigits == 4) {
-              s[rt][i] = fmaf(static_cast<float>(d[rt][3][i] * 256 + d[rt][2][i]), 65536.f,
-                              static_cast<float>(d[rt][1][i] * 256 + d[rt][0][i]));
-            } else {
-              s[rt][i] = fmaf(static_cast<float>(d[rt][2][i] * 256 + d[rt][1][i]), 256.f, static_cast<float>(d[rt][0][i]));
-            }
+            s[rt][i] = fmaf(static_cast<float>(d[rt][3][i] * 256 + d[rt][2][i]), 65536.f,
+                            static_cast<float>(d[rt][1][i] * 256 + d[rt][0][i]));
           }
         }
       } else {

@@ -539,8 +539,11 @@ int gufo_cuda_cache8_rows_device(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache,
  * Token t of a sequence sees rows 0 .. positions[i] + t (the rows of an append with the same
  * batch included), or the first visible[...] rows where `visible` is given; a token that
  * sees no row gets zeros. Sums of exp(score - largest score) times values are fp32: of values
- * near its largest they are infinite. fp32 on the device, strides in floats; heads is a multiple of
- * kv_heads. `out` overlaps none of the inputs.
+ * near its largest they are infinite. Queries are held to 2^-22 of a value or 2^-39 of their row's
+ * largest, whichever is more (e4m3), or 2^-30 of the row's largest (int8); sums of sixteen products with
+ * e4m3 keys, and with values, to some 2^-22 of their magnitudes; a row's weight to 2^-22 of it or 2^-40 of the largest
+ * one's: what is below that adds nothing to `out`, and counts in the weights' sum.
+ * fp32 on the device, strides in floats; heads is a multiple of kv_heads. `out` overlaps none of the inputs.
  * Of one sequence, tokens * (heads / kv_heads) / 32 (rounded up) * kv_heads * (capacity / 16 + 17) is
  * less than 2^31 (a capacity of 131072: 8 million query rows): GUFO_CUDA_TOO_LARGE otherwise, and nothing
  * is enqueued.
