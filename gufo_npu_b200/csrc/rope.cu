@@ -4,10 +4,11 @@
 // pair's frequency.
 //
 // The angle. In turns: the frequency is kept as a 64-bit fraction of a turn per position,
-// the product with the position wraps around at whole turns by itself, and nothing is lost
-// however far the position is (fp32 angles are 0.06 off at a million positions). The nearest
-// quarter is split off as whole numbers, so what sincospif sees is an eighth of a turn at
-// most with 24 significant bits, near the zeros of both functions too.
+// the product with the position wraps around at whole turns by itself, and what is lost is the
+// fraction's own rounding times the position: 2^-33 of a turn at the farthest one, 2^-44 at a
+// million (fp32 angles are 0.06 off there). The nearest quarter is split off as whole numbers, so
+// what sincospif sees is an eighth of a turn at most with 24 significant bits (2^-28 of a turn off),
+// near the zeros of both functions too.
 //
 // What bounds it. The copy: 4 bytes in, 4 out per value (8000 tokens of 10 heads of 256 32 us, 5.2
 // TB/s; a decode step 3 us, a launch). A sine and cosine per pair would
@@ -43,7 +44,7 @@ struct RopeArgs {
   int lanes;      // of a row: a power of two
 };
 
-// Cosine and sine of `position` times the frequency, exact in the angle.
+// Cosine and sine of `position` times the frequency.
 __device__ __forceinline__ void Turn(unsigned long long per, int position, float magnitude, float* cs, float* sn) {
   const unsigned long long at = per * static_cast<unsigned long long>(static_cast<long long>(position));
   const unsigned quarter = static_cast<unsigned>((at + (1ull << 61)) >> 62);
@@ -227,7 +228,8 @@ int CheckRope(const gufo_cuda_rope_params* p) {
   return GUFO_CUDA_OK;
 }
 
-void Frequencies(const gufo_cuda_rope_params& p, double* frequencies, double* magnitude) {
+// Angles per position, in more than a double's bits: positions multiply what they are off by.
+void Frequencies(const gufo_cuda_rope_params& p, long double* frequencies, double* magnitude) {
   const int pairs = p.rope_dim / 2;
   const bool by_parts = p.scaling == GUFO_CUDA_ROPE_BY_PARTS;
   // The pair that turns `turns` times over the original positions.
@@ -241,12 +243,12 @@ void Frequencies(const gufo_cuda_rope_params& p, double* frequencies, double* ma
     high = std::fmin(std::fmax(std::ceil(pair_of(p.slow_turns)), 0.0), p.rope_dim - 1.0);
   }
   for (int i = 0; i < pairs; ++i) {
-    double f = std::pow(p.theta, -static_cast<double>(i) / pairs);
+    long double f = std::pow(static_cast<long double>(p.theta), -static_cast<long double>(i) / pairs);
     if (p.scaling == GUFO_CUDA_ROPE_LINEAR) {
       f /= p.factor;
     } else if (by_parts) {
-      const double slow = std::fmin(std::fmax((i - low) / std::fmax(high - low, 1e-3), 0.0), 1.0);
-      f = f * (1.0 - slow) + f / p.factor * slow;
+      const long double slow = std::fmin(std::fmax((i - low) / std::fmax(static_cast<long double>(high - low), 1e-3L), 0.0L), 1.0L);
+      f = f * (1.0L - slow) + f / p.factor * slow;
     }
     frequencies[i] = f;
   }
@@ -281,7 +283,11 @@ int gufo_cuda_rope_frequencies(const gufo_cuda_rope_params* params, double* freq
   if (frequencies == nullptr || magnitude == nullptr) {
     return Fail(GUFO_CUDA_BAD_ARGUMENT, "rope: null pointer");
   }
-  gufo::Frequencies(*params, frequencies, magnitude);
+  long double exact[gufo::kMaxRopeDim / 2];
+  gufo::Frequencies(*params, exact, magnitude);
+  for (int i = 0; i < params->rope_dim / 2; ++i) {
+    frequencies[i] = static_cast<double>(exact[i]);
+  }
   return GUFO_CUDA_OK;
 }
 
@@ -292,14 +298,15 @@ int gufo_cuda_rope_create(gufo_cuda_ctx* ctx, const gufo_cuda_rope_params* param
   if (const int rc = gufo::CheckRope(params); rc != GUFO_CUDA_OK) {
     return rc;
   }
-  double frequencies[gufo::kMaxRopeDim / 2], magnitude = 1.0;
+  long double frequencies[gufo::kMaxRopeDim / 2];
+  double magnitude = 1.0;
   gufo::Frequencies(*params, frequencies, &magnitude);
   unsigned long long turns[gufo::kMaxRopeDim / 2];
   const int pairs = params->rope_dim / 2;
   for (int i = 0; i < pairs; ++i) {
     // Positions are whole numbers: whole turns per position count for nothing.
-    const long double t = static_cast<long double>(frequencies[i]) / (2.0L * 3.14159265358979323846264338327950288L);
-    turns[i] = static_cast<unsigned long long>((t - std::floor(t)) * 0x1p64L);
+    const long double t = frequencies[i] / (2.0L * 3.14159265358979323846264338327950288L);
+    turns[i] = static_cast<unsigned long long>(std::rint((t - std::floor(t)) * 0x1p64L));   // (whole from a half on: below 2^64)
   }
   std::lock_guard<std::mutex> lock(ctx->mu);
   GUFO_CUDA_TRY(cudaSetDevice(ctx->device));

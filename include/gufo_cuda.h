@@ -469,8 +469,9 @@ typedef struct gufo_cuda_rope_rows {
 } gufo_cuda_rope_rows;
 #define GUFO_CUDA_ROPE_PARTS 4
 /* Turns the rows of 1 to GUFO_CUDA_ROPE_PARTS parts (queries and keys, for example) in
- * one launch: token t by positions[t] (device, any int). Angles are exact to some 2^-40
- * of a turn whatever the position. Device pointers; only enqueues. */
+ * one launch: token t by positions[t] (device, any int). Frequencies of up to a turn per
+ * position are held to 2^-64 of a turn, so angles are 2^-33 of a turn off at the farthest
+ * positions, and 2^-28, as fp32 within an eighth of a turn, at any. Device pointers; only enqueues. */
 int gufo_cuda_rope_device(gufo_cuda_ctx* ctx, gufo_cuda_rope rope,
                           const gufo_cuda_rope_rows* parts, int nparts,
                           const int* positions, int tokens);
