@@ -482,12 +482,17 @@ int gufo_cuda_rope_device(gufo_cuda_ctx* ctx, gufo_cuda_rope rope,
  * half of what the fp16 cache of gufo_cuda_attention_device holds. Sequence `slot`
  * has `capacity` rows of kv_heads * head_dim keys and values. Blocks of
  * GUFO_CUDA_CACHE8_BLOCK rows of a head share one scale for their keys and one for their
- * values: the smallest power of two (2^-126 or more) with which the block's largest
- * magnitude is no more than the format's largest code. A power of two, so that a scale
+ * values: the smallest power of two (2^-126 or more) with which the largest magnitude
+ * appended to the block since its first row is no more than the format's largest code. A power of two, so that a scale
  * that grows costs e4m3 codes nothing but what falls below their smallest value, and int8
  * codes one more rounding.
  * The caller keeps the number of rows that are held (as gufo_cuda_attention_args.position,
  * one count for all layers); it may go back (a draft that is not kept) at any time.
+ * What dropped rows did stays: the block in which they began keeps the scale that they
+ * gave it, its kept rows have been rounded to it and its next ones are (int8: a bit less
+ * for each doubling; e4m3: only what falls below its smallest value), until an append begins
+ * at the block's first row; and the weights that dropped tokens' queries added to rows
+ * ahead of them are not taken back.
  * The reference has no counterpart (its cache is fp16). */
 typedef int64_t gufo_cuda_cache8; /* opaque handle (> 0) */
 enum {
