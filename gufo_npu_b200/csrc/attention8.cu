@@ -121,11 +121,23 @@ struct Shape {
 };
 
 // Waits until a copy that this kernel asked for has landed; false, once, where it has not after
-// about a second: what comes of it is made NaN then, and nothing is waited for any more.
-__device__ __noinline__ bool LandedLate(uint32_t bar, uint32_t parity) {
+// about a second: what comes of it is made NaN then, and the warp waits for nothing any more and asks
+// for nothing. Ahead of that it waits as long again for the copies into its own ring that are under way
+// (slots `slot`, of this `phase`, up to the one that is filled next): they must not find the shared
+// memory of the next block of threads.
+template <int kSlots>
+__device__ __noinline__ bool LandedLate(uint32_t bar, uint32_t parity, uint32_t own, int slot, int fill_slot) {
   const long long began = clock64();
   while (!MbarTryWait(bar, parity)) {
     if (clock64() - began > kLandLimit) {
+      do {
+        while (!MbarTryWait(own + 8 * slot, parity) && clock64() - began < 2 * kLandLimit) {
+        }
+        if (++slot == kSlots) {
+          slot = 0;
+          parity ^= 1;
+        }
+      } while (slot != fill_slot);
       return false;
     }
   }
@@ -406,7 +418,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
   const auto wait_for = [&](int of_warp) {
     const uint32_t bar = SharedAddress(&bars[of_warp][slot]);
     if (!late && !MbarTryWait(bar, phase)) {
-      late = !LandedLate(bar, phase);
+      late = !LandedLate<S::kSlots>(bar, phase, SharedAddress(&bars[warp][0]), slot, fill_slot);
     }
   };
   const auto next_slot = [&]() {
@@ -476,7 +488,7 @@ AttendKernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Batch
     bool next_values = false;
     auto load = [&]() {
       if (next_tile < end_tile) {
-        if (lane == 0) {
+        if (lane == 0 && !late) {
           const int block = next_tile * NS + member;
           const uint32_t bar = SharedAddress(&bars[warp][fill_slot]);
           if (block * kCacheBlock < length) {
