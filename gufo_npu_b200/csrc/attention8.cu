@@ -3,9 +3,9 @@
 // What bounds it. The cache is read once, two bytes a row and dimension of a KV head: far into
 // the contexts that is all the time there is, if loads are never waited for and the arithmetic
 // stays hidden under them: one int8 sequence of 131000 rows of 4 heads of 256 65 us, 4.1 TB/s, of
-// which the loop alone takes 4.5; half of all cycles issue, and three warps a scheduler do not cover
+// which the loop alone takes 4.4; half of all cycles issue, and three warps a scheduler do not cover
 // more of what instructions wait for one another. Short contexts are bound by latency (500 rows
-// 7 us), ragged batches by both (verify batch of 32 sequences 63 us: 23, and 3.4
+// 7 us), ragged batches by both (verify batch of 32 sequences 64 us: 23, and 3.4
 // TB/s behind them).
 //
 // The arithmetic. A group of one, two or four warps (64 dimensions each) goes through tiles of
@@ -20,8 +20,9 @@
 // Codes become fp16 exactly, in registers. The fp32 operands (queries; probabilities) go in as
 // two fp16 halves, 22 bits of them, scaled by a power of two first so that small ones keep
 // their bits (queries against int8 keys: as whole numbers of four digits); each sixteen products'
-// sum is added up in fp32, as the tensor core cuts off what its adder does not hold. S^T comes out with a query's column in the lanes that O^T wants it
-// in; P^T is turned into a B operand by movmatrix. A lane's dimensions are permuted (16 bytes
+// sum is added up in fp32, as the tensor core cuts off what its adder does not hold. S^T comes out
+// with a query's column in the lanes that O^T wants it in; P^T is turned into a B operand by
+// movmatrix. A lane's dimensions are permuted (16 bytes
 // of a key row, 8 of a value row are its own), which a sum over all of them does not see and
 // the output undoes.
 // A block's weights are taken against the maximum that the group knew, or the block's own where
@@ -109,7 +110,8 @@ struct Shape {
   static constexpr int kSlots = NS == 4 ? 3 : NS == 2 ? 5 : 8;
   static constexpr int kRing = kWarps * kSlots * kSlot;
   static constexpr int kJoin = kGroups * 8 * RT * kRowBytes * 4;
-  // Of threads that an SM holds: as many as keep their sums in registers. (32 sequences of some 2000
+  // Of threads that an SM holds: as many as keep their sums in registers, but for 4 to 40 bytes that eleven of
+  // the 72 kernels spill (e4m3, heads of 256, 16 query rows: 40). (32 sequences of some 2000
   // rows, heads of 128: 16 query rows 66 us with four, 48 with three; 32 query rows 129 with three,
   // 95 with two. Heads of 256, 16 query rows: 70 with three, 79 with two.)
   static constexpr int kBlocks = RT == 4 ? 2 : NS == 4 || RT == 2 ? 3 : 4;
@@ -1256,8 +1258,8 @@ int LaunchAttend(gufo_cuda_ctx* ctx, AttendArgs a, const BatchArgs& b, int64_t u
     return rc;
   }
   const int cuts = a.by_unit ? static_cast<int>(units) : blocks;
-  // Units of many parts: a block a row. (One sequence of 131000 rows, 111 parts: 63 us, 86 with four rows a
-  // block; the verify batch of 8 sequences, 14 parts: 33, 38; of 32, 3: 73, 63.)
+  // Units of many parts: a block a row. (With three digits of int8 queries, one sequence of 131000 rows, 111
+  // parts: 63 us, 86 with four rows a block; the verify batch of 8 sequences, 14 parts: 33, 38; of 32, 3: 73, 63.)
   if (std::min<int64_t>(blocks / units, a.cache.capacity / S::kTile) > 8) {
     GUFO_CUDA_TRY(LaunchOverlapped(JoinKernel<1>, dim3(cuts, rows), dim3(kJoinThreads), 0, ctx->stream, 1, a, 8 * RT));
   } else {

@@ -112,7 +112,7 @@ AppendKernel(const __grid_constant__ AppendArgs a, const __grid_constant__ Batch
   if (joins) {
     exponent = max(exponent, ExponentOf(was));
   }
-  const float inverse = PowerOfTwo(-exponent);   // (exponent is -126 .. 120)
+  const float inverse = PowerOfTwo(-exponent);   // (exponent is -126 .. 121)
   if (row0 >= start && row0 + kCacheBlock <= end) {
     // A whole block: put together in shared memory and written sixteen bytes a thread. (The half
     // that a last single piece leaves of its pair holds zeros.)

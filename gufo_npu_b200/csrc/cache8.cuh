@@ -10,7 +10,7 @@ namespace gufo {
 constexpr int kCacheBlock = GUFO_CUDA_CACHE8_BLOCK;   // rows that share a scale
 constexpr int kCacheMaxSequences = 4096;
 constexpr int kCacheMaxDim = 256;
-constexpr int kBatchSequences = 128;   // of one launch: its arguments are 2 KB then
+constexpr int kBatchSequences = 128;   // of one launch: they are 2.6 KB of its arguments
 
 // A sequence of a call.
 struct BatchEntry {
@@ -25,6 +25,7 @@ struct BatchArgs {
   int sequences;
   const int* positions;
 };
+static_assert(sizeof(BatchArgs) <= 2600, "leaves room beside it in 4 KB of arguments");
 
 // What a kernel sees of a cache. A block of 16 rows of a head is their codes, then their scale and
 // 12 bytes of nothing: one contiguous copy. The codes stand by pairs of pieces (32 values), the 16

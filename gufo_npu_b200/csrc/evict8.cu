@@ -11,8 +11,8 @@
 // magnitude, and rounds what had another scale. In place, the rows a block receives come from
 // its own place or behind it, so blocks written in order overwrite nothing that is still wanted:
 // a cluster of thread blocks does the next 64 blocks of a head at a time, all read before any
-// is written (2048 rows of 64 heads of 128: 18 us cold, four rounds). Blocks that stay as they are are not touched. Into another cache there
-// is no order to keep, and every block is a warp of its own (2048 of 16384 rows, 16 heads of 256:
+// is written (2048 rows of 64 heads of 128: 18 us cold, two rounds). Blocks that stay as they are
+// are not touched. Into another cache there is no order to keep, and every block is a warp of its own (2048 of 16384 rows, 16 heads of 256:
 // 16 us cold).
 #include <cooperative_groups.h>
 

@@ -517,7 +517,7 @@ int gufo_cuda_cache8_weights(gufo_cuda_ctx* ctx, gufo_cuda_cache8 cache, float**
 
 /* The sequences of a call. Rows of all sequences follow one another in the arrays of the
  * call, tokens[i] of them for sequence i, which stand at positions[i] .. of slot slots[i].
- * No slot may come twice. */
+ * No slot may come twice, and all rows together are 2^30 at most. */
 typedef struct gufo_cuda_cache8_batch {
   int sequences;
   const int* slots;     /* host [sequences]; NULL: 0, 1, ... */
